@@ -22,6 +22,10 @@ LAYER_TYPES = ["NO_LAYER_TYPE", "INPUT", "CONV", "FC", "RESIDUAL", "BATCHNORM", 
 
 LDATA_FIELDS = ("type", "act", "H", "W", "stride", "tile_h", "tile_w", "num_ninst", "flop_per_output",
                 "parent0", "parent1", "mem_size")
+# ASPEN_B200_TYPE, ASPEN_B200_CACHE_* (include/aspen_b200.h)
+FP32, BF16, FP16 = range(3)
+CACHE_BAD_INDEX, CACHE_NO_PAGES, CACHE_TOO_LONG = 1, 2, 4
+
 NINST_FIELDS = ("pos_h", "pos_w", "tile_h", "tile_w", "num_parents", "num_children", "num_input_pos")
 
 EXPORTS = """apu_create_dnn apu_destroy_dnn apu_save_dnn_to_file apu_load_dnn_from_file apu_generate_nasm
@@ -36,7 +40,10 @@ aspen_b200_set_precision aspen_b200_set_device aspen_b200_dnn_num_layers aspen_b
 aspen_b200_dnn_layer_type aspen_b200_nasm_num_ldata aspen_b200_nasm_num_ninst aspen_b200_nasm_total_flops
 aspen_b200_nasm_ldata_info aspen_b200_nasm_ninst_info aspen_b200_nasm_ninst_parents aspen_b200_nasm_ninst_children
 aspen_b200_nasm_get_ldata_packed aspen_b200_group_time_runs aspen_b200_group_time_passes aspen_b200_dse_group_set_service aspen_b200_group_profile aspen_b200_generate_nasm aspen_b200_set_hidden_states aspen_b200_dnn_set_embedding
-aspen_b200_rpool_add_nasm_tokens aspen_b200_matmul_noalloc""".split()
+aspen_b200_rpool_add_nasm_tokens aspen_b200_matmul_noalloc
+aspen_b200_attention_prompt aspen_b200_cache_workspace aspen_b200_cache_extend aspen_b200_cache_append aspen_b200_cache_fork
+aspen_b200_cache_free aspen_b200_cache_compact aspen_b200_cache_copy aspen_b200_attention_decode_workspace
+aspen_b200_attention_decode""".split()
 
 
 def lib():
@@ -81,6 +88,12 @@ def lib():
         "aspen_b200_group_profile": (i, [vp, vp, C.POINTER(u)]),
         "aspen_b200_generate_nasm": (vp, [vp, u, u, C.POINTER(u)]),
         "aspen_b200_matmul_noalloc": (i, [vp, vp, vp, vp, u, u, u, i, vp]),
+        "aspen_b200_attention_prompt": (i, [vp, vp]),
+        "aspen_b200_cache_workspace": (C.c_size_t, [vp, u]), "aspen_b200_cache_extend": (i, [vp, vp, vp, u, vp, C.c_size_t, vp]),
+        "aspen_b200_cache_append": (i, [vp, u, vp, vp]), "aspen_b200_cache_fork": (i, [vp, vp, vp, u, vp, C.c_size_t, vp]),
+        "aspen_b200_cache_free": (i, [vp, vp, u, vp]), "aspen_b200_cache_compact": (i, [vp, vp, C.c_size_t, vp]),
+        "aspen_b200_cache_copy": (i, [vp, vp, vp, u, vp]),
+        "aspen_b200_attention_decode_workspace": (C.c_size_t, [vp, u, u]), "aspen_b200_attention_decode": (i, [vp, u, vp, vp]),
         "aspen_b200_dnn_set_embedding": (i, [vp, vp, u, vp, u]), "aspen_b200_rpool_add_nasm_tokens": (None, [vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
@@ -315,3 +328,75 @@ class DseGroup:
         if self.h:
             lib().dse_group_destroy(self.h)
             self.h = None
+
+
+def _struct(pointers: str, sizes: str, ints: str, unsigneds: str, floats: str = ""):
+    return ([(n, C.c_void_p) for n in pointers.split()] + [(n, C.c_size_t) for n in sizes.split()] + [(n, C.c_int) for n in ints.split()] +
+            [(n, C.c_uint) for n in unsigneds.split()] + [(n, C.c_float) for n in floats.split()])
+
+
+class PromptArgs(C.Structure):
+    """aspen_b200_prompt_t; pointers are device addresses."""
+    _fields_ = _struct("q k v out q_starts kv_starts", "q_row_stride q_head_stride k_row_stride k_head_stride v_row_stride v_head_stride out_row_stride out_head_stride",
+                       "type masked", "heads kv_heads head_dim sequences q_rows kv_rows", "scale")
+
+
+class AppendArgs(C.Structure):
+    """aspen_b200_append_t"""
+    _fields_ = _struct("k v slots starts", "k_row_stride k_head_stride v_row_stride v_head_stride", "", "entries rows")
+
+
+class DecodeArgs(C.Structure):
+    """aspen_b200_decode_t"""
+    _fields_ = _struct("q out slots workspace", "workspace_bytes q_row_stride q_head_stride out_row_stride out_head_stride", "", "entries heads", "scale")
+
+
+def _check(rc: int, what: str) -> None:
+    if rc != 0:
+        raise RuntimeError(f"{what} failed ({rc}): {last_error()}")
+
+
+def attention_prompt(args: PromptArgs, stream: int = 0) -> None:
+    """Enqueues attention over whole prompts, packed one behind the other."""
+    _check(lib().aspen_b200_attention_prompt(C.byref(args), stream), "aspen_b200_attention_prompt")
+
+
+class Cache(C.Structure):
+    """aspen_b200_cache_t and the calls on it: a paged key-value cache in device memory of the caller.  All pointers are device addresses;
+    every call enqueues on `stream` and returns."""
+    _fields_ = _struct("k v page_table lengths refs status", "layer_stride page_stride head_stride token_stride", "type",
+                       "layers pages page_size kv_heads head_dim sequences max_pages")
+
+    def workspace(self, entries: int = 0) -> int:
+        """Bytes for extend and fork of so many entries, and for compact."""
+        n = lib().aspen_b200_cache_workspace(C.byref(self), entries)
+        if n == 0:
+            raise RuntimeError("aspen_b200_cache_workspace failed: " + last_error())
+        return n
+
+    def extend(self, slots: int, starts: int, entries: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+        _check(lib().aspen_b200_cache_extend(C.byref(self), slots, starts, entries, workspace, workspace_bytes, stream), "aspen_b200_cache_extend")
+
+    def append(self, layer: int, args: AppendArgs, stream: int = 0) -> None:
+        _check(lib().aspen_b200_cache_append(C.byref(self), layer, C.byref(args), stream), "aspen_b200_cache_append")
+
+    def fork(self, sources: int, to: int, entries: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+        _check(lib().aspen_b200_cache_fork(C.byref(self), sources, to, entries, workspace, workspace_bytes, stream), "aspen_b200_cache_fork")
+
+    def free(self, slots: int, entries: int, stream: int = 0) -> None:
+        _check(lib().aspen_b200_cache_free(C.byref(self), slots, entries, stream), "aspen_b200_cache_free")
+
+    def compact(self, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+        _check(lib().aspen_b200_cache_compact(C.byref(self), workspace, workspace_bytes, stream), "aspen_b200_cache_compact")
+
+    def copy(self, sources: int, to: int, count: int, stream: int = 0) -> None:
+        _check(lib().aspen_b200_cache_copy(C.byref(self), sources, to, count, stream), "aspen_b200_cache_copy")
+
+    def decode_workspace(self, entries: int, heads: int) -> int:
+        n = lib().aspen_b200_attention_decode_workspace(C.byref(self), entries, heads)
+        if n == 0:
+            raise RuntimeError("aspen_b200_attention_decode_workspace failed: " + last_error())
+        return n
+
+    def decode(self, layer: int, args: DecodeArgs, stream: int = 0) -> None:
+        _check(lib().aspen_b200_attention_decode(C.byref(self), layer, C.byref(args), stream), "aspen_b200_attention_decode")

@@ -1,0 +1,636 @@
+// Attention of one new token of each sequence over the pages of its cache.
+//
+// out = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q k_j - max): one pass over the keys, the maximum and the sum running along (values already summed are scaled by
+// exp(old max - new max)).  Parts of a sequence give (max, sum, weighted values) that join the same way.
+//
+// What bounds it: reading the cache once.  A step of 16 keys is multiplied with all query heads of its key head, so each key and value is read once whatever the group.
+//     S^T [16 keys x 8 heads] = K Q^T, O^T [features x 8 heads] += V^T P^T, by mma.sync with the keys as the 16-row operand: 8 heads fill its columns where tcgen05 would want
+// 128 rows of queries, and a warp needs nobody else: keys and values go from memory to registers as 16-byte pieces (mma_sync.cuh), no shared memory, no barrier.  Pieces of the next
+// step are asked for before this one is multiplied.
+//
+// Cut: all (sequence, key head) items' steps stand in one line that is dealt to CTAs and then to their warps in equal shares, whatever the lengths (they are known on the
+// device only, and a captured call may see others each time).  A warp's whole items are finished in its registers; at most two it shares with its neighbours.  Shares are
+// joined in the CTA through shared memory, and those that cross CTAs by a second kernel, started early, in order of the steps: the same call gives the same bits.
+#include "mma_sync.cuh"
+
+#include <cuda_runtime.h>
+
+namespace {
+
+using attn::Pages;
+
+constexpr int STEP = 16;                        // keys of a step
+constexpr int JOINERS = 256;
+
+struct Args {
+    const char *q, *k, *v;
+    char *out;
+    const int *slots;
+    Pages at;
+    size_t q_row, q_head, out_row, out_head;    // in elements
+    unsigned entries, kv_heads, group, chunks, head_dim;    // chunks: of a group, each up to the kernel's HEADS
+    float scale;                                // with log2(e)
+    int *record;                                // [CTAs][2]: item that goes on behind the CTA (-1: none), last CTA that has some of it
+    float *part;                                // [CTAs][2][HEADS][DIM + 2]: what began before the CTA, and what goes on behind it
+};
+
+// Threads 0 ... 255 of a CTA: steps of all items, and where each thread's entries begin in the line.
+struct Line {
+    unsigned long long before[257];             // [i]: steps of the entries before thread i's; [256]: all
+    unsigned long long sums[8];
+};
+
+__device__ __forceinline__ unsigned steps_of(unsigned tokens) { return (tokens + STEP - 1) / STEP; }
+__device__ __forceinline__ int slot_of(const Args &a, unsigned e) { return a.slots ? a.slots[e] : (int)e; }
+
+template <int THREADS>
+__device__ void measure(const Args &a, unsigned each, Line &line) {
+    const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    unsigned long long mine = 0;
+    for (unsigned i = 0; i < each; i++) {
+        const unsigned e = threadIdx.x * each + i;
+        if (e < a.entries) mine += steps_of(attn::sequence_length(a.at, slot_of(a, e)));
+    }
+    mine *= a.kv_heads * a.chunks;
+    unsigned long long s = mine;
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const unsigned long long u = __shfl_up_sync(0xffffffffu, s, o); if (lane >= (unsigned)o) s += u; }
+    if (lane == 31) line.sums[warp] = s;
+    __syncthreads();
+    unsigned long long base = 0;
+    for (unsigned w = 0; w < warp; w++) base += line.sums[w];
+    line.before[threadIdx.x] = base + s - mine;
+    if (threadIdx.x == THREADS - 1) line.before[THREADS] = base + s;
+    __syncthreads();
+}
+
+// Running softmax of one item's heads in one warp.  Lane (g, t): heads 2 t and 2 t + 1 of each eight, the features of its pieces.
+template <int TYPE, int DIM, int HEADS>
+struct Running {
+    static constexpr int TILES = HEADS / 8, ROWS = DIM / 16;
+    float o[TILES][ROWS][4];                    // [features' 16-row tile]: (feature, head 2 t), (feature, 2 t + 1), (feature + 1, 2 t), (feature + 1, 2 t + 1)
+    float max[TILES][2], sum[TILES][2];         // sum: of this lane's keys only
+    __device__ __forceinline__ void clear() {
+        #pragma unroll
+        for (int n = 0; n < TILES; n++) {
+            #pragma unroll
+            for (int r = 0; r < ROWS; r++)
+                #pragma unroll
+                for (int i = 0; i < 4; i++) o[n][r][i] = 0.f;
+            max[n][0] = max[n][1] = -INFINITY;
+            sum[n][0] = sum[n][1] = 0.f;
+        }
+    }
+    __device__ __forceinline__ void add_up() {
+        #pragma unroll
+        for (int n = 0; n < TILES; n++)
+            #pragma unroll
+            for (int j = 0; j < 2; j++)
+                #pragma unroll
+                for (int m = 4; m < 32; m <<= 1) sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], m);
+    }
+    // First feature of this lane's piece p, and the values there: PIECE of them for head 2 t + j.
+    static constexpr int PIECE = TYPE == ASPEN_B200_FP32 ? 4 : 8, PIECES = DIM / (8 * PIECE);
+    static __device__ __forceinline__ int feature(int p, unsigned g) { return p * 8 * PIECE + (int)g * PIECE; }
+    __device__ __forceinline__ float value(int n, int p, int x, int j) const { return o[n][p * (PIECE / 2) + x / 2][(x & 1) * 2 + j]; }
+};
+
+template <int TYPE>
+__device__ __forceinline__ void store_piece(char *at, const float *v) {
+    if (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float4 *>(at) = make_float4(v[0], v[1], v[2], v[3]);
+    else {
+        typedef mma::Of<TYPE == ASPEN_B200_FP32 ? ASPEN_B200_BF16 : TYPE> T;
+        *reinterpret_cast<uint4 *>(at) = make_uint4(T::pack(v[0], v[1]), T::pack(v[2], v[3]), T::pack(v[4], v[5]), T::pack(v[6], v[7]));
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ void store_value(char *at, float v) {
+    if (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float *>(at) = v;
+    else if (TYPE == ASPEN_B200_BF16) *reinterpret_cast<__nv_bfloat16 *>(at) = __float2bfloat16_rn(v);
+    else *reinterpret_cast<__half *>(at) = __float2half_rn(v);
+}
+
+__device__ __forceinline__ uint4 load_piece(const char *p, bool ok) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (ok) asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// An item and its steps from `begin` to `end`.
+struct Share {
+    unsigned entry, kv_head, chunk, begin, end, tokens;
+    int slot;
+};
+
+template <int TYPE, int DIM, int HEADS>
+struct Kernel {
+    static constexpr int SIZE = TYPE == ASPEN_B200_FP32 ? 4 : 2, VALUES = 16 / SIZE;
+    static constexpr int WIDTH = DIM < 512 / (SIZE * 2) ? DIM : 512 / (SIZE * 2);      // features of a buffer of eight pieces: 128 of 16 bits, 64 of 32
+    static constexpr int CHUNKS = DIM / WIDTH, PIECES = WIDTH / (4 * VALUES);   // pieces of a lane and row of keys
+    static constexpr int THREADS = 256, WARPS = THREADS / 32;
+    static constexpr int ROW = DIM + 2;         // floats of a partial result of one head: values, maximum, sum
+    static constexpr unsigned SMEM = WARPS * 2 * HEADS * ROW * 4;
+    typedef Running<TYPE, DIM, HEADS> Run;
+
+    // Byte offset of the row of key `lane % 32` behind `first`; -1 if there is none.
+    static __device__ __forceinline__ long long row_of(const Args &a, const Share &s, unsigned first, unsigned lane) {
+        const unsigned key = first + lane;
+        if (key >= s.tokens) return -1;
+        const long long at = attn::token_offset(a.at, s.slot, key);
+        return at < 0 ? -1 : (at + (long long)(s.kv_head * a.at.head_stride)) * SIZE;
+    }
+
+    // Keys: rows g and g + 8 of the step.  Values: rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+    static __device__ __forceinline__ void load_keys(uint4 *buf, const char *base, long long row0, long long row8, int c, unsigned t, unsigned head_dim) {
+        #pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const unsigned f = c * WIDTH + i * 4 * VALUES + t * VALUES;
+            buf[2 * i] = load_piece(base + row0 + f * SIZE, row0 >= 0 && f < head_dim);
+            buf[2 * i + 1] = load_piece(base + row8 + f * SIZE, row8 >= 0 && f < head_dim);
+        }
+    }
+    static constexpr int VPIECES = WIDTH / (8 * VALUES);
+    static __device__ __forceinline__ void load_values(uint4 *buf, const char *base, const long long *row, int c, unsigned g, unsigned head_dim) {
+        #pragma unroll
+        for (int i = 0; i < VPIECES; i++) {
+            const unsigned f = c * WIDTH + i * 8 * VALUES + g * VALUES;
+            #pragma unroll
+            for (int r = 0; r < 4; r++) buf[4 * i + r] = load_piece(base + row[r] + f * SIZE, row[r] >= 0 && f < head_dim);
+        }
+    }
+    static constexpr int TILES = HEADS / 8;
+    static __device__ __forceinline__ void multiply_keys(float (*s)[4], const uint4 *buf, const uint4 (*q)[DIM / (4 * VALUES)], int c) {
+        #pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const uint4 x = buf[2 * i], y = buf[2 * i + 1];
+            #pragma unroll
+            for (int n = 0; n < TILES; n++) {
+                const uint4 b = q[n][c * PIECES + i];
+                if constexpr (TYPE == ASPEN_B200_FP32) {
+                    const unsigned a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w}, b0[2] = {b.x, b.y}, b1[2] = {b.z, b.w};
+                    mma::tf32x3(s[n], a0, b0);
+                    mma::tf32x3(s[n], a1, b1);
+                } else {
+                    mma::Of<TYPE>::step(s[n], x.x, y.x, x.y, y.y, b.x, b.y);
+                    mma::Of<TYPE>::step(s[n], x.z, y.z, x.w, y.w, b.z, b.w);
+                }
+            }
+        }
+    }
+    // p: weights as the column operand, [tile][key half][2] (16-bit: one k = 16 step, [0][0], [0][1] -> b0, b1)
+    static __device__ __forceinline__ void multiply_values(Run &run, const uint4 *buf, const unsigned (*p)[4], int c) {
+        #pragma unroll
+        for (int i = 0; i < VPIECES; i++) {
+            const uint4 &k0 = buf[4 * i], &k1 = buf[4 * i + 1], &k8 = buf[4 * i + 2], &k9 = buf[4 * i + 3];
+            const unsigned w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w}, w8[4] = {k8.x, k8.y, k8.z, k8.w}, w9[4] = {k9.x, k9.y, k9.z, k9.w};
+            if constexpr (TYPE == ASPEN_B200_FP32) {
+                #pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const unsigned lo[4] = {w0[2 * j], w0[2 * j + 1], w1[2 * j], w1[2 * j + 1]}, hi[4] = {w8[2 * j], w8[2 * j + 1], w9[2 * j], w9[2 * j + 1]};
+                    #pragma unroll
+                    for (int n = 0; n < TILES; n++) {
+                        float *o = run.o[n][(c * VPIECES + i) * 2 + j];
+                        mma::tf32x3(o, lo, p[n]);
+                        mma::tf32x3(o, hi, p[n] + 2);
+                    }
+                }
+            } else {
+                #pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const unsigned a0 = mma::pair_of(w0[j], w1[j], false), a1 = mma::pair_of(w0[j], w1[j], true);
+                    const unsigned a2 = mma::pair_of(w8[j], w9[j], false), a3 = mma::pair_of(w8[j], w9[j], true);
+                    #pragma unroll
+                    for (int n = 0; n < TILES; n++) mma::Of<TYPE>::step(run.o[n][(c * VPIECES + i) * 4 + j], a0, a1, a2, a3, p[n][0], p[n][1]);
+                }
+            }
+        }
+    }
+
+    // One step's scores: running maximum and sum, and the weights as an operand.
+    static __device__ __forceinline__ void weigh(Run &run, float (*s)[4], bool ok0, bool ok8, float scale, unsigned lane, unsigned (*p)[4]) {
+        #pragma unroll
+        for (int n = 0; n < TILES; n++) {
+            float x[4], w[4];
+            #pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = (i < 2 ? ok0 : ok8) ? s[n][i] * scale : -INFINITY;
+            float down[2];
+            #pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float m = fmaxf(x[j], x[2 + j]);
+                #pragma unroll
+                for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                m = fmaxf(m, run.max[n][j]);
+                const float ref = m == -INFINITY ? 0.f : m;
+                down[j] = mma::exp2_fast(run.max[n][j] - ref);
+                run.max[n][j] = m;
+                w[j] = mma::exp2_fast(x[j] - ref);
+                w[2 + j] = mma::exp2_fast(x[2 + j] - ref);
+                run.sum[n][j] = run.sum[n][j] * down[j] + (w[j] + w[2 + j]);
+            }
+            if (__any_sync(0xffffffffu, down[0] != 1.f || down[1] != 1.f)) {
+                #pragma unroll
+                for (int r = 0; r < Run::ROWS; r++)
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++) run.o[n][r][i] *= down[i & 1];
+            }
+            if constexpr (TYPE == ASPEN_B200_FP32) {
+                // lane (g, t) wants keys 2 t and 2 t + 1 of each eight for head g; lane (key, g / 2) has them
+                const unsigned from = 8 * (lane & 3) + (lane >> 3);
+                const bool odd = lane >> 2 & 1u;
+                #pragma unroll
+                for (int h = 0; h < 2; h++)
+                    #pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const float u = __shfl_sync(0xffffffffu, w[2 * h], from + 4 * k), v = __shfl_sync(0xffffffffu, w[2 * h + 1], from + 4 * k);
+                        p[n][2 * h + k] = __float_as_uint(odd ? v : u);
+                    }
+            } else {
+                p[n][0] = mma::transpose8(mma::Of<TYPE>::pack(w[0], w[1]));
+                p[n][1] = mma::transpose8(mma::Of<TYPE>::pack(w[2], w[3]));
+            }
+        }
+    }
+
+    static __device__ __forceinline__ long long from_lane(long long v, unsigned lane) { return __shfl_sync(0xffffffffu, v, lane); }
+
+    // All steps of a share, in one warp.
+    static __device__ __forceinline__ void walk(const Args &a, const Share &s, Run &run) {
+        const unsigned lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+        uint4 q[TILES][DIM / (4 * VALUES)];
+        #pragma unroll
+        for (int n = 0; n < TILES; n++) {
+            const unsigned in_group = s.chunk * HEADS + n * 8 + g;
+            const char *row = a.q + ((size_t)s.entry * a.q_row + (size_t)(s.kv_head * a.group + in_group) * a.q_head) * SIZE;
+            #pragma unroll
+            for (int i = 0; i < DIM / (4 * VALUES); i++) {
+                const unsigned f = i * 4 * VALUES + t * VALUES;
+                q[n][i] = load_piece(row + f * SIZE, in_group < a.group && f < a.head_dim);
+            }
+        }
+        run.clear();
+        // rows of two steps: lanes 0 ... 15 the first one's keys, 16 ... 31 the second one's
+        unsigned step = s.begin;
+        long long rows = row_of(a, s, step * STEP, lane);
+        uint4 buf[2][8];
+        // buffers in turn: all chunks of a step's keys, then all of its values; each is filled again as soon as it has been multiplied
+        long long key0 = from_lane(rows, g), key8 = from_lane(rows, g + 8), value[4];
+        bool second = false;
+        auto values_of = [&](unsigned at) {
+            value[0] = from_lane(rows, at + 2 * t); value[1] = from_lane(rows, at + 2 * t + 1);
+            value[2] = from_lane(rows, at + 2 * t + 8); value[3] = from_lane(rows, at + 2 * t + 9);
+        };
+        values_of(0);
+        load_keys(buf[0], a.k, key0, key8, 0, t, a.head_dim);
+        if (CHUNKS > 1) load_keys(buf[1], a.k, key0, key8, 1, t, a.head_dim);
+        else load_values(buf[1], a.v, value, 0, g, a.head_dim);
+        long long later = -1;
+        #pragma unroll 1
+        for (; step < s.end; step++) {
+            const bool ok0 = key0 >= 0, ok8 = key8 >= 0, more = step + 1 < s.end;
+            if (!second && step + 2 < s.end) later = row_of(a, s, (step + 2) * STEP, lane);
+            float score[TILES][4];
+            #pragma unroll
+            for (int n = 0; n < TILES; n++)
+                #pragma unroll
+                for (int i = 0; i < 4; i++) score[n][i] = 0.f;
+            #pragma unroll
+            for (int c = 0; c < CHUNKS; c++) {
+                multiply_keys(score, buf[c % 2], q, c);
+                if (c + 2 < CHUNKS) load_keys(buf[c % 2], a.k, key0, key8, c + 2, t, a.head_dim);
+                else if (CHUNKS > 1) load_values(buf[c % 2], a.v, value, c + 2 - CHUNKS, g, a.head_dim);
+            }
+            // the next step's rows
+            long long next0 = -1, next8 = -1;
+            if (more) {
+                const unsigned at = second ? 0u : 16u;
+                if (second) rows = later;
+                next0 = from_lane(rows, at + g);
+                next8 = from_lane(rows, at + g + 8);
+            }
+            if (CHUNKS == 1 && more) load_keys(buf[0], a.k, next0, next8, 0, t, a.head_dim);
+            unsigned p[TILES][4];
+            weigh(run, score, ok0, ok8, a.scale, lane, p);
+            if (CHUNKS == 1) {
+                multiply_values(run, buf[1], p, 0);
+                if (more) { values_of(second ? 0u : 16u); load_values(buf[1], a.v, value, 0, g, a.head_dim); }
+            } else {
+                #pragma unroll
+                for (int c = 0; c < CHUNKS; c++) {
+                    multiply_values(run, buf[c % 2], p, c);
+                    if (c + 2 < CHUNKS) load_values(buf[c % 2], a.v, value, c + 2, g, a.head_dim);
+                    else if (more) load_keys(buf[c % 2], a.k, next0, next8, c + 2 - CHUNKS, t, a.head_dim);
+                }
+                if (more) values_of(second ? 0u : 16u);
+            }
+            key0 = next0;
+            key8 = next8;
+            second = !second;
+        }
+        run.add_up();
+    }
+
+    static __device__ __forceinline__ char *out_of(const Args &a, unsigned entry, unsigned kv_head, unsigned in_group) {
+        return a.out + ((size_t)entry * a.out_row + (size_t)(kv_head * a.group + in_group) * a.out_head) * SIZE;
+    }
+    // A whole item's outputs from one warp's registers.
+    static __device__ __forceinline__ void finish(const Args &a, const Share &s, const Run &run) {
+        const unsigned g = threadIdx.x % 32 >> 2, t = threadIdx.x & 3;
+        #pragma unroll
+        for (int n = 0; n < TILES; n++)
+            #pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const unsigned in_group = s.chunk * HEADS + n * 8 + 2 * t + j;
+                const float inv = run.sum[n][j] == 0.f ? 0.f : 1.f / run.sum[n][j];
+                if (in_group >= a.group) continue;
+                char *row = out_of(a, s.entry, s.kv_head, in_group);
+                #pragma unroll
+                for (int i = 0; i < Run::PIECES; i++) {
+                    const unsigned f = Run::feature(i, g);
+                    float v[Run::PIECE];
+                    #pragma unroll
+                    for (int x = 0; x < Run::PIECE; x++) v[x] = run.value(n, i, x, j) * inv;
+                    if (f < a.head_dim) store_piece<TYPE>(row + f * SIZE, v);
+                }
+            }
+    }
+    // A shared item's part to the warp's place in shared memory.
+    static __device__ __forceinline__ void keep(float *at, const Run &run) {
+        const unsigned g = threadIdx.x % 32 >> 2, t = threadIdx.x & 3;
+        #pragma unroll
+        for (int n = 0; n < TILES; n++)
+            #pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float *row = at + (n * 8 + 2 * t + j) * ROW;
+                #pragma unroll
+                for (int i = 0; i < Run::PIECES; i++)
+                    #pragma unroll
+                    for (int x = 0; x < Run::PIECE; x += 2)
+                        *reinterpret_cast<float2 *>(row + Run::feature(i, g) + x) = make_float2(run.value(n, i, x, j), run.value(n, i, x + 1, j));
+                if (g == 0) *reinterpret_cast<float2 *>(row + DIM) = make_float2(run.max[n][j], run.sum[n][j]);
+            }
+    }
+};
+
+// Value f of head r from `count` partial results, `stride` floats apart, joined in order; the maximum and the sum too.
+template <int ROW, int DIM>
+__device__ __forceinline__ float join(const float *first, size_t stride, unsigned count, int r, int f, float &max, float &sum) {
+    first += r * ROW;
+    max = -INFINITY;
+    for (unsigned i = 0; i < count; i++) max = fmaxf(max, first[i * stride + DIM]);
+    const float ref = max == -INFINITY ? 0.f : max;
+    float v = 0.f;
+    sum = 0.f;
+    #pragma unroll 4
+    for (unsigned i = 0; i < count; i++) {
+        const float *p = first + i * stride;
+        const float w = mma::exp2_fast(p[DIM] - ref);
+        sum = fmaf(w, p[DIM + 1], sum);
+        v = fmaf(w, p[f], v);
+    }
+    return v;
+}
+
+template <int TYPE, int DIM, int HEADS, int CTAS>
+__global__ void __launch_bounds__(256, CTAS) decode_kernel(const Args a) {
+    typedef Kernel<TYPE, DIM, HEADS> K;
+    typedef typename K::Run Run;
+    extern __shared__ float kept[];             // [warp][2][HEADS][ROW]
+    __shared__ Line line;
+    __shared__ int item_of[K::WARPS * 2], whole_of[K::WARPS * 2];      // of the kept parts: the item (-1: none); bit 0: has its begin, bit 1: its end
+    const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const unsigned each = (a.entries + 255) / 256, items = a.kv_heads * a.chunks;
+    measure<256>(a, each, line);
+    const unsigned long long all = line.before[256];
+    if (threadIdx.x < K::WARPS * 2) item_of[threadIdx.x] = -1;
+    // sequences without tokens
+    for (unsigned e = blockIdx.x; e < a.entries; e += gridDim.x) {
+        const int slot = slot_of(a, e);
+        if (attn::sequence_length(a.at, slot) != 0) continue;
+        for (unsigned i = threadIdx.x; i < a.kv_heads * a.group * a.head_dim; i += 256)
+            store_value<TYPE>(a.out + ((size_t)e * a.out_row + (size_t)(i / a.head_dim) * a.out_head + i % a.head_dim) * K::SIZE, 0.f);
+        if (threadIdx.x == 0 && (slot < 0 || (unsigned)slot >= a.at.sequences)) atomicOr(a.at.status, ASPEN_B200_CACHE_BAD_INDEX);
+    }
+    __syncthreads();
+    // CTAs that get a share: a step for each of their warps at least, so that little is joined where little is to do
+    const unsigned ctas = (unsigned)min((unsigned long long)gridDim.x, (all + K::WARPS - 1) / K::WARPS);
+    if (blockIdx.x < ctas) {
+        const unsigned long long cta0 = attn::first_step(all, blockIdx.x, ctas), cta1 = attn::first_step(all, blockIdx.x + 1, ctas);
+        const unsigned long long steps = cta1 - cta0;
+        unsigned long long pos = cta0 + attn::first_step(steps, warp, K::WARPS);
+        const unsigned long long end = cta0 + attn::first_step(steps, warp + 1, K::WARPS);
+        if (pos < end) {
+            unsigned lo = 0, hi = 256;          // the last thread whose entries begin at pos or before
+            while (hi - lo > 1) { const unsigned mid = (lo + hi) / 2; if (line.before[mid] <= pos) lo = mid; else hi = mid; }
+            unsigned e = lo * each;
+            unsigned long long base = line.before[lo];
+            while (pos < end) {
+                Share s;
+                unsigned n;
+                // bounded by the number of entries: `end` does not lie behind the last one's steps
+                for (;; e++) {
+                    s.slot = slot_of(a, e);
+                    s.tokens = attn::sequence_length(a.at, s.slot);
+                    n = steps_of(s.tokens);
+                    if (base + (unsigned long long)n * items > pos || e + 1 >= a.entries) break;
+                    base += (unsigned long long)n * items;
+                }
+                const unsigned long long rel = pos - base;
+                if (rel >= (unsigned long long)n * items) break;           // lengths that changed under the call
+                const unsigned item = (unsigned)(rel / n);
+                s.entry = e;
+                s.kv_head = item / a.chunks;
+                s.chunk = item - s.kv_head * a.chunks;
+                s.begin = (unsigned)(rel - (unsigned long long)item * n);
+                s.end = (unsigned)min((unsigned long long)n, s.begin + (end - pos));
+                Run run;
+                K::walk(a, s, run);
+                if (s.begin == 0 && s.end == n) K::finish(a, s, run);
+                else {
+                    // the one that began before this warp's share, or the one that goes on behind it
+                    const unsigned place = warp * 2 + (s.begin != 0 ? 0 : 1);
+                    K::keep(kept + (size_t)place * HEADS * K::ROW, run);
+                    if (lane == 0) { item_of[place] = (int)(e * items + item); whole_of[place] = (s.begin == 0 ? 1 : 0) | (s.end == n ? 2 : 0); }
+                }
+                pos += s.end - s.begin;
+            }
+        }
+    }
+    __syncthreads();
+    // Parts of one item stand next to each other; those of all warps, in order.
+    if (threadIdx.x == 0) a.record[2 * blockIdx.x] = -1;
+    __syncthreads();
+    for (unsigned i = 0; i < K::WARPS * 2;) {
+        const int item = item_of[i];
+        if (item < 0) { i++; continue; }
+        // the parts behind this one that are of the same item (places that are empty lie between them: a warp's second place when its first one goes on)
+        unsigned places[K::WARPS * 2], count = 0, last = i;
+        for (unsigned j = i; j < K::WARPS * 2; j++)
+            if (item_of[j] == item) { places[count++] = j; last = j; }
+        const bool begins = whole_of[i] & 1, ends = whole_of[last] & 2;
+        const unsigned e = (unsigned)item / items, rest = (unsigned)item % items, kv_head = rest / a.chunks, chunk = rest % a.chunks;
+        float *const part = a.part + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * HEADS * K::ROW;
+        for (unsigned x = threadIdx.x; x < HEADS * DIM; x += 256) {
+            const unsigned r = x / DIM, f = x % DIM;
+            float max = -INFINITY, sum = 0.f, v = 0.f;
+            for (unsigned j = 0; j < count; j++) max = fmaxf(max, kept[(places[j] * HEADS + r) * K::ROW + DIM]);
+            const float ref = max == -INFINITY ? 0.f : max;
+            for (unsigned j = 0; j < count; j++) {
+                const float *p = kept + (places[j] * HEADS + r) * K::ROW;
+                const float w = mma::exp2_fast(p[DIM] - ref);
+                sum = fmaf(w, p[DIM + 1], sum);
+                v = fmaf(w, p[f], v);
+            }
+            if (begins && ends) {
+                const unsigned in_group = chunk * HEADS + r;
+                if (in_group < a.group && f < a.head_dim) store_value<TYPE>(K::out_of(a, e, kv_head, in_group) + f * K::SIZE, sum == 0.f ? 0.f : v / sum);
+            } else {
+                part[r * K::ROW + f] = v;
+                if (f == 0) { part[r * K::ROW + DIM] = max; part[r * K::ROW + DIM + 1] = sum; }
+            }
+        }
+        if (begins && !ends && threadIdx.x == 0) {
+            // where the item's last step is
+            const unsigned owner = e / each;
+            unsigned long long base = line.before[owner];
+            for (unsigned j = owner * each; j < e; j++) base += (unsigned long long)steps_of(attn::sequence_length(a.at, slot_of(a, j))) * items;
+            const unsigned n = steps_of(attn::sequence_length(a.at, slot_of(a, e)));
+            a.record[2 * blockIdx.x] = item;
+            a.record[2 * blockIdx.x + 1] = (int)attn::part_of_step(all, base + (unsigned long long)(rest + 1) * n - 1, ctas);
+        }
+        i = last + 1;
+    }
+}
+
+// Items that several CTAs had a part of: CTA b joins the one that began in CTA b and went on.
+template <int TYPE, int DIM, int HEADS>
+__global__ void __launch_bounds__(JOINERS) join_kernel(const Args a) {
+    typedef Kernel<TYPE, DIM, HEADS> K;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int item = a.record[2 * blockIdx.x];
+    if (item < 0) return;
+    const unsigned count = (unsigned)a.record[2 * blockIdx.x + 1] - blockIdx.x, items = a.kv_heads * a.chunks;    // CTAs behind this one
+    const unsigned e = (unsigned)item / items, rest = (unsigned)item % items, kv_head = rest / a.chunks, chunk = rest % a.chunks;
+    constexpr size_t SLOT = (size_t)HEADS * K::ROW;
+    const float *const mine = a.part + ((size_t)blockIdx.x * 2 + 1) * SLOT;
+    for (unsigned x = threadIdx.x; x < HEADS * DIM; x += JOINERS) {
+        const unsigned r = x / DIM, f = x % DIM, in_group = chunk * HEADS + r;
+        if (in_group >= a.group || f >= a.head_dim) continue;
+        float m, s;
+        // the others' parts that began before their CTA: every second place from here on
+        const float v = join<K::ROW, DIM>(mine + SLOT, 2 * SLOT, count, r, f, m, s);
+        const float *p = mine + r * K::ROW;
+        const float max = fmaxf(m, p[DIM]), ref = max == -INFINITY ? 0.f : max;
+        const float w0 = mma::exp2_fast(p[DIM] - ref), w1 = mma::exp2_fast(m - ref);
+        const float sum = fmaf(w0, p[DIM + 1], w1 * s), value = fmaf(w0, p[f], w1 * v);
+        store_value<TYPE>(K::out_of(a, e, kv_head, in_group) + f * K::SIZE, sum == 0.f ? 0.f : value / sum);
+    }
+}
+
+// Heads of a group that one pass over the keys serves: eight columns of a product, or sixteen (features permitting: the sums of 256 take the registers).
+unsigned heads_of_pass(unsigned group, unsigned dim) { return group <= 8 || dim == 256 ? 8 : 16; }
+unsigned dim_of(unsigned head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+// CTAs on an SM: registers for that many (three for heads of up to 128 features and 8 heads).
+unsigned ctas_of(unsigned heads, unsigned dim, int type) { return dim == 256 || (heads == 16 && dim == 128) ? 1 : type == ASPEN_B200_FP32 && dim == 128 ? 1 : 2; }
+
+size_t workspace_bytes(unsigned sms, unsigned heads, unsigned dim, int type) {
+    const size_t ctas = (size_t)sms * ctas_of(heads, dim, type);
+    return ctas * 16 + ctas * 2 * heads * (dim + 2) * 4;
+}
+
+template <int TYPE, int DIM, int HEADS, int CTAS>
+cudaError_t launch(const Args &a, unsigned sms, cudaStream_t stream) {
+    typedef Kernel<TYPE, DIM, HEADS> K;
+    cudaError_t err = cudaFuncSetAttribute(decode_kernel<TYPE, DIM, HEADS, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, K::SMEM);
+    if (err != cudaSuccess) return err;
+    decode_kernel<TYPE, DIM, HEADS, CTAS><<<sms * CTAS, 256, K::SMEM, stream>>>(a);
+    if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms * CTAS);
+    cfg.blockDim = dim3(JOINERS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join_kernel<TYPE, DIM, HEADS>, a);
+}
+template <int TYPE>
+cudaError_t launch(const Args &a, unsigned heads, unsigned dim, unsigned sms, cudaStream_t stream) {
+    constexpr int WIDE = TYPE == ASPEN_B200_FP32 ? 1 : 2;
+    if (dim == 64) return heads == 8 ? launch<TYPE, 64, 8, 2>(a, sms, stream) : launch<TYPE, 64, 16, 2>(a, sms, stream);
+    if (dim == 128) return heads == 8 ? launch<TYPE, 128, 8, WIDE>(a, sms, stream) : launch<TYPE, 128, 16, 1>(a, sms, stream);
+    return launch<TYPE, 256, 8, 1>(a, sms, stream);
+}
+
+int check_heads(const aspen_b200_cache_t *cache, unsigned entries, unsigned heads, const char *what) {
+    const int rc = attn::check_cache(cache, what, false);
+    if (rc) return rc;
+    if (!heads || heads % cache->kv_heads) { ASPEN_ERR("%s: %u heads of queries, %u of keys\n", what, heads, cache->kv_heads); return -1; }
+    if ((unsigned long long)entries * heads > 0x7fffffffull || heads > 0xffffu) { ASPEN_ERR("%s: %u x %u rows of queries\n", what, entries, heads); return -2; }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" size_t aspen_b200_attention_decode_workspace(const aspen_b200_cache_t *cache, unsigned int entries, unsigned int heads) {
+    const char *what = "aspen_b200_attention_decode_workspace";
+    if (check_heads(cache, entries, heads, what)) return 0;
+    const int sms = attn::sm_count(what);
+    if (sms < 0) return 0;
+    const unsigned dim = dim_of(cache->head_dim);
+    return workspace_bytes((unsigned)sms, heads_of_pass(heads / cache->kv_heads, dim), dim, cache->type);
+}
+
+extern "C" int aspen_b200_attention_decode(const aspen_b200_cache_t *cache, unsigned int layer, const aspen_b200_decode_t *d, void *cuda_stream) {
+    const char *what = "aspen_b200_attention_decode";
+    if (!d) { ASPEN_ERR("%s: no arguments\n", what); return -1; }
+    int rc = check_heads(cache, d->entries, d->heads, what);
+    if (rc) return rc;
+    if (layer >= cache->layers) { ASPEN_ERR("%s: layer %u of %u\n", what, layer, cache->layers); return -1; }
+    if (!d->entries) return 0;
+    if (!(d->scale - d->scale == 0.f)) { ASPEN_ERR("%s: scale is not finite\n", what); return -1; }
+    if (!d->slots && d->entries > cache->sequences) { ASPEN_ERR("%s: %u entries, %u sequences\n", what, d->entries, cache->sequences); return -1; }
+    if ((rc = attn::check_rows(d->q, d->q_row_stride, d->q_head_stride, cache->type, "q", what)) ||
+        (rc = attn::check_rows(d->out, d->out_row_stride, d->out_head_stride, cache->type, "out", what))) return rc;
+    if (!d->workspace || reinterpret_cast<uintptr_t>(d->workspace) % 16) { ASPEN_ERR("%s: no workspace, or not on a 16-byte boundary\n", what); return -1; }
+    const int sms = attn::sm_count(what);
+    if (sms < 0) return sms;
+    const unsigned group = d->heads / cache->kv_heads, dim = dim_of(cache->head_dim), heads = heads_of_pass(group, dim);
+    const size_t need = workspace_bytes((unsigned)sms, heads, dim, cache->type);
+    if (d->workspace_bytes < need) { ASPEN_ERR("%s: a workspace of %zu bytes; %zu are needed\n", what, d->workspace_bytes, need); return -1; }
+    const attn::Named all[] = {{cache->k, "the cache's k"}, {cache->v, "the cache's v"}, {cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->status, "status"},
+                               {d->q, "q"}, {d->out, "out"}, {d->slots, "slots"}, {d->workspace, "workspace"}};
+    if ((rc = attn::check_device(all, 9, what))) return rc;
+    Args a;
+    a.at = attn::pages_of(*cache);
+    const size_t size = attn::type_size(cache->type), skip = layer * attn::packed(cache->layer_stride, a.at.page_stride * cache->pages) * size;
+    a.k = static_cast<const char *>(cache->k) + skip;
+    a.v = static_cast<const char *>(cache->v) + skip;
+    a.q = static_cast<const char *>(d->q);
+    a.out = static_cast<char *>(d->out);
+    a.slots = d->slots;
+    a.q_row = attn::packed(d->q_row_stride, (size_t)d->heads * cache->head_dim);
+    a.q_head = attn::packed(d->q_head_stride, cache->head_dim);
+    a.out_row = attn::packed(d->out_row_stride, (size_t)d->heads * cache->head_dim);
+    a.out_head = attn::packed(d->out_head_stride, cache->head_dim);
+    a.entries = d->entries;
+    a.kv_heads = cache->kv_heads;
+    a.group = group;
+    a.chunks = (group + heads - 1) / heads;
+    a.head_dim = cache->head_dim;
+    a.scale = d->scale * 1.4426950408889634f;
+    const size_t ctas = (size_t)sms * ctas_of(heads, dim, cache->type);
+    a.record = static_cast<int *>(d->workspace);
+    a.part = reinterpret_cast<float *>(static_cast<char *>(d->workspace) + ctas * 16);
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    cudaError_t err;
+    switch (cache->type) {
+        case ASPEN_B200_FP32: err = launch<ASPEN_B200_FP32>(a, heads, dim, (unsigned)sms, stream); break;
+        case ASPEN_B200_BF16: err = launch<ASPEN_B200_BF16>(a, heads, dim, (unsigned)sms, stream); break;
+        default: err = launch<ASPEN_B200_FP16>(a, heads, dim, (unsigned)sms, stream); break;
+    }
+    if (err != cudaSuccess) { cudaGetLastError(); ASPEN_ERR("%s: %s\n", what, cudaGetErrorString(err)); return -3; }
+    return 0;
+}

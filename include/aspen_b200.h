@@ -275,6 +275,105 @@ void aspen_b200_set_hidden_states(int keep);
 int aspen_b200_matmul_noalloc(const float *x_dev, const float *w_dev, const float *bias_dev, float *out_dev,
                               unsigned int n_cols, unsigned int k, unsigned int m, int activation, void *cuda_stream);
 
+/* ---- attention without allocation, and a paged key-value cache -------------------------------------------------------------
+ *
+ * No counterpart in the reference, whose attention layers run a whole sequence of one fixed length in every pass.  These calls are for programs that
+ * generate text: a prompt of any length is attended to once, its keys and values stay in pages, and every further token reads them there.
+ *
+ * As with aspen_b200_matmul_noalloc all memory is DEVICE memory of the caller, on the current device, and nothing is allocated.  Unlike it
+ * the calls do not wait: they enqueue one or two kernels on `cuda_stream` (a cudaStream_t, NULL = default) and return, and can be captured into a graph.
+ * What follows from device memory (lengths, indices) is therefore checked on the device: nothing out of range is read or written, and the cache's status word
+ * says that it happened.  Calls on several streams may run at once if they share no memory that one of them writes; each needs a workspace of its own
+ * while it runs, and so does a captured graph.
+ * Return values: 0, -1 bad arguments, -2 too large, -3 CUDA error or no sm_100 device (see aspen_b200_last_error); on failure nothing is enqueued but where
+ * a CUDA launch itself fails.
+ *
+ * Types: queries, keys, values, outputs and the cache of one call have the same.  Scores, softmax and sums are fp32, rounded once to the output's type; the
+ * weights are rounded to bf16 / fp16 before they multiply 16-bit values.  fp32 operands are split into parts that tensor cores hold (a product is
+ * off by 2^-20 of itself at most); an infinity among them makes the outputs that see it NaN.
+ * Heads have 8 ... 256 features, a multiple of 8; `heads` is a multiple of `kv_heads`, head h reads key head h / (heads / kv_heads).
+ * Strides are in elements, 0 = packed; features are contiguous, and every row starts on a 16-byte boundary. */
+typedef enum { ASPEN_B200_FP32, ASPEN_B200_BF16, ASPEN_B200_FP16, ASPEN_B200_NUM_TYPES } ASPEN_B200_TYPE;
+
+/* Attention over whole prompts, sequences packed one behind the other: rows q_starts[s] ... q_starts[s + 1] - 1 of q and out belong to sequence s, rows
+ * kv_starts[s] ... kv_starts[s + 1] - 1 of k and v are what it attends to.  out = softmax(scale * q k^T) v.  masked = 1: a sequence's last query sees all of
+ * its keys, the one before it all but the last, and so on; with more queries than keys the first ones see none.  A row that sees nothing becomes zeros.
+ * Rows of no sequence are neither read into a result nor written.  Starts outside 0 ... q_rows (kv_rows) are taken as the nearest one inside, a sequence that would
+ * end before it starts is empty; sequences must not share rows of out.  Values behind a query's last key, but within its sequence, must be finite (they are
+ * multiplied by zero). */
+typedef struct {
+    const void *q, *k, *v;         /* [q_rows][heads][head_dim], [kv_rows][kv_heads][head_dim] twice */
+    void *out;                     /* [q_rows][heads][head_dim]; not q, k or v */
+    const int *q_starts, *kv_starts;        /* [sequences + 1]; may be the same */
+    size_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride, out_row_stride, out_head_stride;
+    int type, masked;
+    unsigned int heads, kv_heads, head_dim, sequences, q_rows, kv_rows;
+    float scale;
+} aspen_b200_prompt_t;
+int aspen_b200_attention_prompt(const aspen_b200_prompt_t *prompt, void *cuda_stream);
+
+/* A cache of the keys and values of up to `sequences` sequences, in pages of page_size tokens that they take from one pool.  A program fills the description once,
+ * sets page_table to -1 and lengths, refs and *status to 0, and from then on leaves them to the calls below.
+ *     k, v         [layers][pages][kv_heads][page_size][head_dim], or with other strides
+ *     page_table   [sequences][max_pages]: token t of sequence s is row t % page_size of page page_table[s][t / page_size], in every layer
+ *     lengths      [sequences]: tokens
+ *     refs         [pages]: how often page_table names the page; 0 = free
+ *     status       a word to which the calls add ASPEN_B200_CACHE_* bits; the caller clears it */
+typedef struct {
+    void *k, *v;
+    int *page_table, *lengths, *refs, *status;
+    size_t layer_stride, page_stride, head_stride, token_stride;
+    int type;
+    unsigned int layers, pages, page_size, kv_heads, head_dim, sequences, max_pages;
+} aspen_b200_cache_t;
+#define ASPEN_B200_CACHE_BAD_INDEX 1    /* a sequence or page that does not exist, named twice where it must not be, or a fork onto one that is not empty */
+#define ASPEN_B200_CACHE_NO_PAGES 2     /* the pool has too few free pages, or one sequence asked for more than 2^21 at once */
+#define ASPEN_B200_CACHE_TOO_LONG 4     /* a sequence would need more than max_pages pages */
+
+/* Bytes of workspace of extend, fork (entries: how many are given) and compact (0); 0 on bad arguments. */
+size_t aspen_b200_cache_workspace(const aspen_b200_cache_t *cache, unsigned int entries);
+/* Room for new tokens: entry i adds starts[i + 1] - starts[i] of them (starts NULL: one) to sequence slots[i] (slots NULL: i).  Pages are taken lowest number
+ * first, in the order of the entries.  If an index is bad, a sequence is named twice or gets too long, or the pages do not suffice, nothing changes but the status. */
+int aspen_b200_cache_extend(const aspen_b200_cache_t *cache, const int *slots, const int *starts, unsigned int entries, void *workspace,
+                            size_t workspace_bytes, void *cuda_stream);
+/* Writes keys and values of one layer behind an extend with the same slots and starts: row starts[i] + j is the token j of the starts[i + 1] - starts[i] that
+ * sequence slots[i] was extended by last, as its length says.  Rows that have no such place are left out (status). */
+typedef struct {
+    const void *k, *v;             /* [rows][kv_heads][head_dim] */
+    const int *slots, *starts;     /* [entries], [entries + 1], or NULL as in extend */
+    size_t k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    unsigned int entries, rows;
+} aspen_b200_append_t;
+int aspen_b200_cache_append(const aspen_b200_cache_t *cache, unsigned int layer, const aspen_b200_append_t *append, void *cuda_stream);
+/* Sequence to[i] becomes a copy of sequence from[i] as it was before the call: full pages are shared, the tokens of a last page that is not full are copied in all
+ * layers.  A sequence may be forked many times; each to[i] must be empty and named once, else (or without enough pages) nothing changes but the status. */
+int aspen_b200_cache_fork(const aspen_b200_cache_t *cache, const int *from, const int *to, unsigned int entries, void *workspace, size_t workspace_bytes,
+                          void *cuda_stream);
+/* Gives back the pages of the sequences, which become empty.  One that is named twice is freed once. */
+int aspen_b200_cache_free(const aspen_b200_cache_t *cache, const int *slots, unsigned int entries, void *cuda_stream);
+/* Moves pages so that those in use are the lowest ones: with n in use, those numbered n and above go, in order, to the free ones below n, in order. */
+int aspen_b200_cache_compact(const aspen_b200_cache_t *cache, void *workspace, size_t workspace_bytes, void *cuda_stream);
+/* Copies page from[i] to page to[i] in all layers; page_table and refs stay.  No page may be in `to` twice, or in both. */
+int aspen_b200_cache_copy(const aspen_b200_cache_t *cache, const int *from, const int *to, unsigned int count, void *cuda_stream);
+
+/* Attention of one new token each over the cache of one layer: out[i] = softmax(scale * q[i] K^T) V over all lengths[slots[i]] tokens of sequence slots[i] (the
+ * new one's key and value have been appended before).  An empty sequence, or one that does not exist, gives zeros; tokens whose page does not exist are left
+ * out.  A sequence may be named more than once.  The work is split over all SMs by what the lengths say on the device, and joined in a fixed order: the same call gives
+ * the same bits, a sequence beside others not always the same ones as alone.
+ * workspace: aspen_b200_attention_decode_workspace bytes (0 on bad arguments or without a device). */
+typedef struct {
+    const void *q;                 /* [entries][heads][head_dim] */
+    void *out;                     /* the same */
+    const int *slots;              /* [entries], or NULL: entry i is sequence i */
+    void *workspace;
+    size_t workspace_bytes;
+    size_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    unsigned int entries, heads;
+    float scale;
+} aspen_b200_decode_t;
+size_t aspen_b200_attention_decode_workspace(const aspen_b200_cache_t *cache, unsigned int entries, unsigned int heads);
+int aspen_b200_attention_decode(const aspen_b200_cache_t *cache, unsigned int layer, const aspen_b200_decode_t *decode, void *cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

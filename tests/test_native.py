@@ -141,3 +141,7 @@ def test_sets_of_graphs_that_are_run_in_turn_are_kept(workdir):
 def test_a_launch_of_several_graphs_has_the_small_ones_done_first(workdir):
     api.lib()
     passes(build("merge_claims", workdir, f"-L{LIBDIR}", "-laspen_b200", f"-Wl,-rpath,{LIBDIR}"))
+
+
+def test_places_in_the_paged_cache_and_shares_of_the_work(workdir):
+    passes(build("attention_index", workdir))
