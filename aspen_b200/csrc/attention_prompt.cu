@@ -5,6 +5,7 @@
 // prompt_rows (any type, any head): a warp has 16 queries, its operands and sums in registers as mma.sync takes them (mma_sync.cuh); keys and values of a tile go through
 // shared memory for the four warps of a CTA, asked for one tile ahead.  Rows in shared memory are 64 (keys) and 16 bytes (values) longer than a power of two, so that the 16-byte pieces
 // that eight lanes read together lie in different banks.
+#include "attention_tc.cuh"
 #include "mma_sync.cuh"
 
 #include <cuda_runtime.h>
@@ -28,16 +29,17 @@ struct Block {
 
 __device__ __forceinline__ int clamped(const int *starts, unsigned i, unsigned rows) { return min(max(starts[i], 0), (int)rows); }
 
-// Block `index` of all sequences' blocks of `size` queries, counted from the first sequence; a sequence's last one first, because with a mask it has most
-// keys.  Every warp finds it for itself, 32 sequences a turn.  False: there are not so many.
-__device__ __forceinline__ bool find_block(const Args &a, unsigned index, unsigned size, Block &b) {
+// Piece `index` of all sequences, `pieces(queries)` of one, counted from the first sequence; a sequence's last one first, because with a mask it has most keys.
+// Every warp finds it for itself, 32 sequences a turn.  Returns the piece's number in its sequence, -1: there are not so many.
+template <typename Pieces>
+__device__ __forceinline__ int find_piece(const Args &a, unsigned index, const Pieces &pieces, int &q_first, int &queries, int &k_first, int &keys) {
     const unsigned lane = threadIdx.x % 32;
     unsigned long long before = 0;
     for (unsigned s0 = 0; s0 < a.sequences; s0 += 32) {
         const unsigned s = s0 + lane;
         int q0 = 0, q1 = 0;
         if (s < a.sequences) { q0 = clamped(a.q_starts, s, a.q_rows); q1 = max(q0, clamped(a.q_starts, s + 1, a.q_rows)); }
-        const unsigned n = ((unsigned)(q1 - q0) + size - 1) / size;
+        const unsigned n = pieces((unsigned)(q1 - q0));
         unsigned long long sum = n;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const unsigned long long u = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= (unsigned)o) sum += u; }
@@ -45,18 +47,21 @@ __device__ __forceinline__ bool find_block(const Args &a, unsigned index, unsign
         if (here) {
             const int at = __ffs(here) - 1;
             const unsigned rank = (unsigned)(before + sum - 1 - index);           // of lane `at`: n - 1 for the first index of its sequence, 0 for the last
-            const unsigned back = __shfl_sync(0xffffffffu, rank, at), blocks = __shfl_sync(0xffffffffu, n, at);
-            b.q0 = __shfl_sync(0xffffffffu, q0, at);
-            b.queries = __shfl_sync(0xffffffffu, q1, at) - b.q0;
-            b.first = (int)((back < blocks ? back : 0u) * size);
+            q_first = __shfl_sync(0xffffffffu, q0, at);
+            queries = __shfl_sync(0xffffffffu, q1, at) - q_first;
             const unsigned mine = s0 + at;
-            b.k0 = clamped(a.kv_starts, mine, a.kv_rows);
-            b.keys = max(0, clamped(a.kv_starts, mine + 1, a.kv_rows) - b.k0);
-            return true;
+            k_first = clamped(a.kv_starts, mine, a.kv_rows);
+            keys = max(0, clamped(a.kv_starts, mine + 1, a.kv_rows) - k_first);
+            return (int)__shfl_sync(0xffffffffu, rank, at);
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    return false;
+    return -1;
+}
+__device__ __forceinline__ bool find_block(const Args &a, unsigned index, unsigned size, Block &b) {
+    const int i = find_piece(a, index, [=](unsigned queries) { return (queries + size - 1) / size; }, b.q0, b.queries, b.k0, b.keys);
+    b.first = i * (int)size;
+    return i >= 0;
 }
 
 __device__ __forceinline__ unsigned shared_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -258,6 +263,345 @@ cudaError_t launch_rows(const Args &a, cudaStream_t stream) {
     return a.head_dim <= 64 ? launch_rows<TYPE, 64>(a, stream) : a.head_dim <= 128 ? launch_rows<TYPE, 128>(a, stream) : launch_rows<TYPE, 256>(a, stream);
 }
 
+// ---- tcgen05 (attention_tc.cuh) ----
+
+// Tiles of a head of keys in a sequence: block by block of 128 queries, the heads of the group side by side; a job is two neighbours.
+__device__ __forceinline__ bool find_job(const Args &a, unsigned index, unsigned kv_heads, fused::Job &job) {
+    const unsigned group = a.group;
+    const int pair = find_piece(a, index / kv_heads, [=](unsigned queries) { return ((queries + fused::TILE - 1) / fused::TILE * group + 1) / 2; }, job.q0, job.queries, job.k0, job.keys);
+    if (pair < 0) return false;
+    job.kv_head = index % kv_heads;
+    #pragma unroll
+    for (int w = 0; w < 2; w++) {
+        const unsigned tile = (unsigned)pair * 2 + w, block = tile / group;
+        job.head[w] = job.kv_head * group + (tile - block * group);
+        job.first[w] = (int)(block * fused::TILE);
+        const bool there = job.first[w] < job.queries;
+        job.steps[w] = there ? (job.end(w, a.masked) + (int)fused::TILE - 1) / (int)fused::TILE : 0;
+        if (!there) job.first[w] = -1;
+    }
+    return true;
+}
+
+template <int TYPE, int DIM>
+__global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                                                                   const Args a, unsigned kv_heads) {
+    using namespace fused;
+    typedef Shape<DIM> H;
+    extern __shared__ char raw[];
+    const unsigned base = (tc::smem_u32(raw) + 1023u) & ~1023u;
+    char *const smem = raw + (base - tc::smem_u32(raw));
+    const unsigned q_at = base, k_at = base + 2 * H::BYTES, v_at = k_at + H::STAGES * H::BYTES;
+    __shared__ Barriers sh;
+    const unsigned warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;
+    unsigned *const gave_up = &sh.gave_up;
+    if (threadIdx.x == 0) {
+        sh.gave_up = 0u;
+        for (int w = 0; w < 2; w++) {
+            tc::mbar_init(&sh.q_full[w], 1u); tc::mbar_init(&sh.q_empty[w], 1u); tc::mbar_init(&sh.s_full[w], 1u); tc::mbar_init(&sh.o_full[w], 1u);
+            tc::mbar_init(&sh.s_free[w], 4u); tc::mbar_init(&sh.p_full[w], 4u);
+        }
+        for (int s = 0; s < 4; s++) { tc::mbar_init(&sh.k_full[s], 1u); tc::mbar_init(&sh.k_empty[s], 1u); tc::mbar_init(&sh.v_full[s], 1u); tc::mbar_init(&sh.v_empty[s], 1u); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tc::fence_proxy_async_smem();
+    }
+    if (warp == 9) tc::tmem_alloc(&sh.tmem, 512u);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const unsigned tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+    // Registers: 128 x (2 x 232 + 40) = 384 x 168, what the launch holds
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        bool ok = true;
+        if (warp == 8) {
+            unsigned stage = 0, lap = 0, q_uses[2] = {0, 0};
+            for (unsigned index = blockIdx.x; ok; index += gridDim.x) {
+                Job job;
+                if (!find_job(a, index, kv_heads, job)) break;
+                const int steps = job.both();
+                for (int j = 0; j < steps && ok; j++) {
+                    ok = warp_wait(&sh.k_empty[stage], (lap & 1u) ^ 1u, gave_up);
+                    if (!ok) break;
+                    if (tc::elect_one()) {
+                        tc::mbar_arrive_expect_tx(&sh.k_full[stage], H::BYTES);
+                        #pragma unroll
+                        for (int c = 0; c < H::CHUNKS; c++)
+                            tc::tma_load_3d(k_at + stage * H::BYTES + c * H::CHUNK_BYTES, &k_map, c * 64, (int)job.kv_head, job.k0 + j * (int)TILE, &sh.k_full[stage]);
+                    }
+                    __syncwarp();
+                    if (j == 0)
+                        for (int w = 0; w < 2 && ok; w++) {
+                            if (job.steps[w] == 0) continue;
+                            ok = warp_wait(&sh.q_empty[w], (q_uses[w] & 1u) ^ 1u, gave_up);
+                            q_uses[w]++;
+                            if (ok && tc::elect_one()) {
+                                tc::mbar_arrive_expect_tx(&sh.q_full[w], H::BYTES);
+                                #pragma unroll
+                                for (int c = 0; c < H::CHUNKS; c++)
+                                    tc::tma_load_3d(q_at + w * H::BYTES + c * H::CHUNK_BYTES, &q_map, c * 64, (int)job.head[w], job.q0 + job.first[w], &sh.q_full[w]);
+                            }
+                            __syncwarp();
+                        }
+                    ok = ok && warp_wait(&sh.v_empty[stage], (lap & 1u) ^ 1u, gave_up);
+                    if (!ok) break;
+                    if (tc::elect_one()) {
+                        tc::mbar_arrive_expect_tx(&sh.v_full[stage], H::BYTES);
+                        #pragma unroll
+                        for (int c = 0; c < H::CHUNKS; c++)
+                            tc::tma_load_3d(v_at + stage * H::BYTES + c * H::CHUNK_BYTES, &v_map, c * 64, (int)job.kv_head, job.k0 + j * (int)TILE, &sh.v_full[stage]);
+                    }
+                    __syncwarp();
+                    if (++stage == H::STAGES) { stage = 0; lap++; }
+                }
+            }
+        } else if (warp == 9) {
+            constexpr unsigned FORMAT = TYPE == ASPEN_B200_BF16 ? 1u : 0u;
+            constexpr unsigned IDESC = 1u << 4 | FORMAT << 7 | FORMAT << 10 | (128u >> 4) << 24;       // sums fp32, 128 rows
+            constexpr unsigned IDESC_S = IDESC | (128u >> 3) << 17, IDESC_O = IDESC | ((unsigned)DIM >> 3) << 17 | 1u << 16;      // the second operand of PV: features contiguous
+            unsigned stage = 0, lap = 0, q_uses[2] = {0, 0}, done[2] = {0, 0};
+            // scores of tile w over the keys of a stage
+            auto scores = [&](int w, unsigned st, bool last) {
+                if (tc::elect_one()) {
+                    #pragma unroll
+                    for (int c = 0; c < H::CHUNKS; c++)
+                        #pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            mma_ss(tmem + H::S + w * 128, tc::umma_desc_low(q_at + w * H::BYTES + c * H::CHUNK_BYTES + k * 32), tc::umma_desc_low(k_at + st * H::BYTES + c * H::CHUNK_BYTES + k * 32), IDESC_S, c + k);
+                    tc::tc_commit(&sh.s_full[w]);
+                    if (last) tc::tc_commit(&sh.q_empty[w]);
+                }
+                __syncwarp();
+            };
+            auto values = [&](int w, unsigned st, bool first) {
+                if (tc::elect_one()) {
+                    #pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        mma_ts(tmem + H::O + w * DIM, tmem + H::P + w * H::P_APART + k * 8, (v_at + st * H::BYTES + k * 2048) >> 4 | (H::CHUNK_BYTES >> 4) << 16, IDESC_O, first ? k : 1);
+                    tc::tc_commit(&sh.o_full[w]);
+                }
+                __syncwarp();
+            };
+            auto release = [&](unsigned long long *bar) { if (tc::elect_one()) tc::tc_commit(bar); __syncwarp(); };
+            for (unsigned index = blockIdx.x; ok; index += gridDim.x) {
+                Job job;
+                if (!find_job(a, index, kv_heads, job)) break;
+                const int steps = job.both();
+                if (steps == 0) continue;
+                ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
+                for (int w = 0; w < 2 && ok; w++) {
+                    if (job.steps[w] == 0) continue;
+                    ok = warp_wait(&sh.q_full[w], q_uses[w] & 1u, gave_up);
+                    q_uses[w]++;
+                    // a tile's softmax has read its last scores: it has given their weights, or (weights of their own) said so
+                    if (H::OWN_P) ok = ok && warp_wait(&sh.s_free[w], (done[w] & 1u) ^ 1u, gave_up);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    scores(w, stage, job.steps[w] == 1);
+                }
+                if (!ok) break;
+                release(&sh.k_empty[stage]);
+                for (int j = 0; j < steps && ok; j++) {
+                    const unsigned here = stage, at = lap;
+                    if (++stage == H::STAGES) { stage = 0; lap++; }
+                    const bool more = j + 1 < steps;
+                    if (H::OWN_P && more) {
+                        ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
+                        for (int w = 0; w < 2 && ok; w++) {
+                            if (j + 1 >= job.steps[w]) continue;
+                            ok = warp_wait(&sh.s_free[w], done[w] & 1u, gave_up);
+                            if (!ok) break;
+                            tc::tc_fence_after();
+                            scores(w, stage, j + 2 == job.steps[w]);
+                        }
+                        if (!ok) break;
+                        release(&sh.k_empty[stage]);
+                    }
+                    ok = warp_wait(&sh.v_full[here], at & 1u, gave_up);
+                    if (!ok) break;
+                    if (job.keys < (j + 1) * (int)TILE) {
+                        const int from = job.keys - j * (int)TILE;
+                        char *const v = smem + (v_at - base) + here * H::BYTES;
+                        for (int i = from * 8 + (int)lane; i < (int)TILE * 8; i += 32)
+                            #pragma unroll
+                            for (int c = 0; c < H::CHUNKS; c++) *reinterpret_cast<uint4 *>(v + c * H::CHUNK_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        tc::fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (!H::OWN_P && more) ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
+                    for (int w = 0; w < 2 && ok; w++) {
+                        if (j >= job.steps[w]) continue;
+                        ok = warp_wait(&sh.p_full[w], done[w] & 1u, gave_up);
+                        if (!ok) break;
+                        done[w]++;
+                        tc::tc_fence_after();
+                        values(w, here, j == 0);
+                        if (!H::OWN_P && j + 1 < job.steps[w]) scores(w, stage, j + 2 == job.steps[w]);
+                    }
+                    if (!ok) break;
+                    release(&sh.v_empty[here]);
+                    if (!H::OWN_P && more) release(&sh.k_empty[stage]);
+                }
+            }
+        }
+        __syncwarp();
+        tc::tc_fence_before();
+        __syncthreads();
+        if (warp == 9) {
+            if (sh.gave_up) {
+                // copies and MMAs may still be in flight; they take microseconds
+                unsigned long long t0, now;
+                asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+                do { __nanosleep(1000); asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now)); } while (now - t0 < 2000000ull);
+            }
+            tc::tc_fence_after();
+            tc::tmem_dealloc(tmem, 512u);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const int w = (int)(warp >> 2);
+        const unsigned row = (warp & 3u) * 32u + lane, lanes = tmem + ((warp & 3u) << 21), s_at = lanes + H::S + w * 128, p_at = lanes + H::P + w * H::P_APART, o_at = lanes + H::O + w * DIM;
+        unsigned done = 0;
+        bool ok = true;
+        for (unsigned index = blockIdx.x;; index += gridDim.x) {
+            Job job;
+            if (!find_job(a, index, kv_heads, job)) break;
+            if (job.first[w] < 0) continue;
+            const int query = job.first[w] + (int)row, steps = job.steps[w];
+            const int seen = a.masked ? min(job.keys, query + job.behind() + 1) : job.keys;              // first key that the row does not see
+            const int warp_seen = __shfl_sync(0xffffffffu, seen, 0);                                      // of the warp's first row, which sees least
+            float max = -INFINITY, sum = 0.f;
+            for (int j = 0; j < steps && ok; j++) {
+                ok = warp_wait(&sh.s_full[w], done & 1u, gave_up);
+                if (!ok) break;
+                tc::tc_fence_after();
+                float s[128];
+                #pragma unroll
+                for (int i = 0; i < 4; i++) ld32(s_at + i * 32, s + i * 32);
+                #pragma unroll
+                for (int i = 0; i < 4; i++) ld_done32(s + i * 32);
+                if (H::OWN_P) {
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&sh.s_free[w]);
+                }
+                if (warp_seen < (j + 1) * (int)TILE) {
+                    const int left = seen - j * (int)TILE;
+                    #pragma unroll
+                    for (int i = 0; i < 128; i++) s[i] = i < left ? s[i] : -INFINITY;
+                }
+                float m0 = max3(s[0], s[1], s[2]), m1 = max3(s[3], s[4], s[5]), m2 = max3(s[6], s[7], s[8]), m3 = max3(s[9], s[10], s[11]);
+                #pragma unroll
+                for (int i = 12; i < 124; i += 8) { m0 = max3(m0, s[i], s[i + 1]); m1 = max3(m1, s[i + 2], s[i + 3]); m2 = max3(m2, s[i + 4], s[i + 5]); m3 = max3(m3, s[i + 6], s[i + 7]); }
+                m0 = max3(m0, s[124], s[125]); m1 = max3(m1, s[126], s[127]);
+                const float most = fmaxf(max3(m0, m1, m2), m3);
+                // both -inf: not a number, and nothing to do
+                if (__any_sync(0xffffffffu, (most - max) * a.scale > 8.f)) {
+                    const float next = fmaxf(max, most), down = next == -INFINITY ? 1.f : mma::exp2_fast((max - next) * a.scale);
+                    if (j > 0) {
+                        if (H::OWN_P) ok = warp_wait(&sh.o_full[w], (done & 1u) ^ 1u, gave_up);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        #pragma unroll
+                        for (int i = 0; i < DIM; i += 32) {
+                            float o[32];
+                            ld32(o_at + i, o);
+                            ld_done32(o);
+                            #pragma unroll
+                            for (int x = 0; x < 32; x++) o[x] *= down;
+                            st32(o_at + i, reinterpret_cast<unsigned *>(o));
+                        }
+                    }
+                    sum *= down;
+                    max = next;
+                }
+                const float ref = max == -INFINITY ? 0.f : -max * a.scale;
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                #pragma unroll
+                for (int i = 0; i < 128; i++) { s[i] = mma::exp2_fast(fmaf(s[i], a.scale, ref)); part[i & 3] += s[i]; }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                // the weights' place is free: the product before has been through (in the place of the scores: it was before these)
+                if (H::OWN_P && j > 0) {
+                    ok = warp_wait(&sh.o_full[w], (done & 1u) ^ 1u, gave_up);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                }
+                #pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    unsigned p[32];
+                    #pragma unroll
+                    for (int i = 0; i < 32; i++) p[i] = mma::Of<TYPE>::pack(s[h * 64 + 2 * i], s[h * 64 + 2 * i + 1]);
+                    st32(p_at + h * 32, p);
+                }
+                st_done();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sh.p_full[w]);
+                done++;
+            }
+            // outputs: a row a thread
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            if (ok && steps > 0) ok = warp_wait(&sh.o_full[w], (done & 1u) ^ 1u, gave_up);
+            tc::tc_fence_after();
+            const bool mine = query < job.queries;
+            char *const out = a.out + ((size_t)(job.q0 + query) * a.out_row + job.head[w] * a.out_head) * 2;
+            #pragma unroll
+            for (int i = 0; i < DIM; i += 32) {
+                float o[32];
+                if (ok && steps > 0) { ld32(o_at + i, o); ld_done32(o); }
+                unsigned p[16];
+                #pragma unroll
+                for (int x = 0; x < 16; x++) p[x] = !ok ? 0x7fff7fffu : steps == 0 ? 0u : mma::Of<TYPE>::pack(o[2 * x] * inv, o[2 * x + 1] * inv);
+                #pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (mine && i + 8 * x < (int)a.head_dim) *reinterpret_cast<uint4 *>(out + (i + 8 * x) * 2) = make_uint4(p[4 * x], p[4 * x + 1], p[4 * x + 2], p[4 * x + 3]);
+            }
+        }
+        __syncwarp();
+        tc::tc_fence_before();
+        __syncthreads();
+    }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess ? (EncodeFn)p : nullptr;
+    }();
+    return fn;
+}
+// (feature, head, row) of a 16-bit matrix, boxes of 64 features of 128 rows; zeros outside.
+bool encode(CUtensorMap *map, int type, const char *p, unsigned dim, unsigned heads, unsigned rows, size_t head, size_t row) {
+    const cuuint64_t dims[3] = {dim, heads, rows}, strides[2] = {head * 2, row * 2};
+    const cuuint32_t box[3] = {64, 1, fused::TILE}, one[3] = {1, 1, 1};
+    return encode_fn()(map, type == ASPEN_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<char *>(p), dims, strides, box, one,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int TYPE, int DIM>
+cudaError_t launch_tiles(const Args &a, const CUtensorMap *maps, unsigned sms, cudaStream_t stream) {
+    cudaError_t err = cudaFuncSetAttribute(prompt_tiles<TYPE, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, fused::Shape<DIM>::SMEM);
+    if (err != cudaSuccess) return err;
+    const unsigned long long kv_heads = a.heads / a.group, sequences = a.sequences < a.q_rows ? a.sequences : a.q_rows;
+    const unsigned long long jobs = ((a.q_rows / fused::TILE + sequences) * a.group + sequences) / 2 * kv_heads;       // at most
+    prompt_tiles<TYPE, DIM><<<(unsigned)(jobs < sms ? jobs : sms), fused::THREADS, fused::Shape<DIM>::SMEM, stream>>>(maps[0], maps[1], maps[2], a, (unsigned)kv_heads);
+    return cudaGetLastError();
+}
+// False: not a call for these kernels.
+bool try_tiles(const Args &a, int type, unsigned sms, cudaStream_t stream, cudaError_t *err) {
+    if (type == ASPEN_B200_FP32 || a.head_dim > 128 || !a.kv_rows || !(a.scale > 0.f) || !encode_fn()) return false;      // a row's largest score is its largest product only for a scale above 0
+    const unsigned kv_heads = a.heads / a.group;
+    CUtensorMap maps[3];
+    if (!encode(&maps[0], type, a.q, a.head_dim, a.heads, a.q_rows, a.q_head, a.q_row) || !encode(&maps[1], type, a.k, a.head_dim, kv_heads, a.kv_rows, a.k_head, a.k_row) ||
+        !encode(&maps[2], type, a.v, a.head_dim, kv_heads, a.kv_rows, a.v_head, a.v_row)) return false;
+    if (a.head_dim <= 64) *err = type == ASPEN_B200_BF16 ? launch_tiles<ASPEN_B200_BF16, 64>(a, maps, sms, stream) : launch_tiles<ASPEN_B200_FP16, 64>(a, maps, sms, stream);
+    else *err = type == ASPEN_B200_BF16 ? launch_tiles<ASPEN_B200_BF16, 128>(a, maps, sms, stream) : launch_tiles<ASPEN_B200_FP16, 128>(a, maps, sms, stream);
+    return true;
+}
+
 }  // namespace
 
 extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *cuda_stream) {
@@ -302,7 +646,9 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     a.masked = p->masked != 0;
     a.scale = p->scale * 1.4426950408889634f;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-    const cudaError_t err = p->type == ASPEN_B200_FP32 ? launch_rows<ASPEN_B200_FP32>(a, stream) : p->type == ASPEN_B200_BF16 ? launch_rows<ASPEN_B200_BF16>(a, stream) : launch_rows<ASPEN_B200_FP16>(a, stream);
+    cudaError_t err = cudaSuccess;
+    if (!try_tiles(a, p->type, (unsigned)sms, stream, &err))
+        err = p->type == ASPEN_B200_FP32 ? launch_rows<ASPEN_B200_FP32>(a, stream) : p->type == ASPEN_B200_BF16 ? launch_rows<ASPEN_B200_BF16>(a, stream) : launch_rows<ASPEN_B200_FP16>(a, stream);
     if (err != cudaSuccess) { cudaGetLastError(); ASPEN_ERR("%s: %s\n", what, cudaGetErrorString(err)); return -3; }
     return 0;
 }

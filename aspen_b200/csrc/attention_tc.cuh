@@ -1,0 +1,122 @@
+// Attention over whole prompts on tcgen05, 16-bit types, heads of up to 128 features.
+//
+// A CTA takes two tiles of 128 queries that see the same head of keys (two heads of a group, or two blocks of a head's queries) and walks their keys, 128 a step:
+//     S [128 queries x 128 keys] = Q K^T     both operands in shared memory, K-major, scores in TMEM
+//     P = exp2(S - max)                      a thread a query: its row of scores from TMEM to registers, weights back to TMEM as 16-bit pairs
+//     O [128 queries x features] += P V      P from TMEM, V as it lies in memory (features contiguous: the MN-major operand), sums in TMEM
+// The running maximum is followed loosely: O and the sum are scaled again only when a row's maximum has grown by more than 2^8 (weights up to 256 are as exact as weights up to 1),
+// so the sums in TMEM are hardly ever read before the end.
+//
+// Warps: 0 - 3 and 4 - 7 the softmax of the two tiles, 8 TMA, 9 MMA; nothing but mbarriers connects them, and while one tile's scores are weighed the other's are multiplied.  TMEM, 512
+// columns: scores 2 x 128, sums 2 x features, and with 64 features weights 2 x 64 of their own, so that the next scores are there before the weights of these have been
+// multiplied; with 128 the weights take the place of their scores.
+//
+// What bounds it: a step of two tiles is 2048 cycles of the tensor pipe with 128 features, 1024 with 64, and 2048 of the unit for exp2.
+//
+// Values behind the end of a sequence are another one's, or nobody's: the MMA warp sets them to zero in shared memory, since 0 x NaN would reach every row.
+//
+// Every wait is bounded (2 s) and is for another role of the CTA; if one runs out all roles leave, TMEM is freed and the CTA's rows of out that are not done become NaN.
+#pragma once
+#include "tiles_tc.cuh"
+
+#include <cuda.h>
+
+namespace fused {
+
+constexpr unsigned THREADS = 384, TILE = 128;
+constexpr unsigned long long LIMIT_NS = 2000000000ull;
+
+template <int DIM>
+struct Shape {
+    static constexpr int CHUNKS = DIM / 64;                         // of 64 features: 128 bytes, the swizzle's width
+    static constexpr int CHUNK_BYTES = TILE * 128, BYTES = CHUNKS * CHUNK_BYTES;    // of a tile of queries, keys or values
+    static constexpr int STAGES = DIM == 64 ? 4 : 2;
+    static constexpr int SMEM = 2 * BYTES + 2 * STAGES * BYTES + 2048;
+    static constexpr bool OWN_P = DIM == 64;
+    static constexpr unsigned S = 0, O = 256, P = OWN_P ? 384 : 0, P_APART = OWN_P ? 64 : 128;      // TMEM columns
+};
+
+struct Barriers {
+    unsigned long long q_full[2], q_empty[2], k_full[4], k_empty[4], v_full[4], v_empty[4];
+    unsigned long long s_full[2], s_free[2], p_full[2], o_full[2];
+    unsigned gave_up, tmem;
+};
+
+__device__ __forceinline__ bool wait(unsigned long long *bar, unsigned parity, unsigned *gave_up) {
+    #pragma unroll 1
+    for (unsigned spin = 0; spin < 4096u; spin++)
+        if (tc::mbar_try_wait(bar, parity)) return true;
+    unsigned long long t0, now;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+    #pragma unroll 1
+    for (unsigned spin = 1;; spin++) {
+        if (tc::mbar_try_wait(bar, parity)) return true;
+        if ((spin & 255u) == 0u) {
+            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+            if (*(volatile unsigned *)gave_up != 0u) return false;
+            if (now - t0 > LIMIT_NS) { atomicExch(gave_up, 1u); return false; }
+        }
+    }
+}
+// A warp's lanes wait, and give up, together.
+__device__ __forceinline__ bool warp_wait(unsigned long long *bar, unsigned parity, unsigned *gave_up) { return __all_sync(0xffffffffu, wait(bar, parity, gave_up)); }
+
+// Both operands in shared memory, K-major, 128-byte swizzle; or A in TMEM and B with features contiguous (MN-major): 64 features of a row side by side, the next 64
+// CHUNK_BYTES on, eight keys 1024 bytes.
+__device__ __forceinline__ void mma_ss(unsigned d, unsigned a, unsigned b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(tc::UMMA_DESC_HIGH) : "memory");
+}
+__device__ __forceinline__ void mma_ts(unsigned d, unsigned a, unsigned b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(tc::UMMA_DESC_HIGH) : "memory");
+}
+
+// 32 columns of the warp's lanes, not waited for.
+__device__ __forceinline__ void ld32(unsigned at, float *v) {
+    unsigned *r = reinterpret_cast<unsigned *>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(at) : "memory");
+}
+// The loads before are done; what they loaded is used behind this only.
+__device__ __forceinline__ void ld_done32(float *v) {
+    unsigned *r = reinterpret_cast<unsigned *>(v);
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]) : : "memory");
+    asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) : : "memory");
+}
+__device__ __forceinline__ void st32(unsigned at, const unsigned *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+
+// A CTA's work: two tiles of queries of one sequence and one head of keys.
+struct Job {
+    int q0, queries, k0, keys;
+    unsigned kv_head, head[2];
+    int first[2], steps[2];                        // first query of a tile; steps of 128 keys, 0: no such tile
+    __device__ __forceinline__ int both() const { return max(steps[0], steps[1]); }
+    __device__ __forceinline__ int behind() const { return keys - queries; }
+    __device__ __forceinline__ int end(int w, int masked) const { return masked ? max(0, min(keys, min(queries, first[w] + (int)TILE) + behind())) : keys; }
+};
+
+}  // namespace fused
