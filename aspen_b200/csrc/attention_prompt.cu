@@ -270,18 +270,35 @@ __device__ __forceinline__ bool find_job(const Args &a, unsigned index, unsigned
     const unsigned group = a.group;
     const int pair = find_piece(a, index / kv_heads, [=](unsigned queries) { return ((queries + fused::TILE - 1) / fused::TILE * group + 1) / 2; }, job.q0, job.queries, job.k0, job.keys);
     if (pair < 0) return false;
-    job.kv_head = index % kv_heads;
+    job.kv_head = (int)(index % kv_heads);
     #pragma unroll
     for (int w = 0; w < 2; w++) {
         const unsigned tile = (unsigned)pair * 2 + w, block = tile / group;
-        job.head[w] = job.kv_head * group + (tile - block * group);
+        job.head[w] = job.kv_head * (int)group + (int)(tile - block * group);
         job.first[w] = (int)(block * fused::TILE);
         const bool there = job.first[w] < job.queries;
         job.steps[w] = there ? (job.end(w, a.masked) + (int)fused::TILE - 1) / (int)fused::TILE : 0;
         if (!there) job.first[w] = -1;
     }
+    job.live = 1;
     return true;
 }
+
+// A role's walk through the jobs.
+struct Walk {
+    fused::Shared *sh;
+    unsigned slot = 0, lap = 0;
+    __device__ __forceinline__ const fused::Job &job() const { return sh->jobs[slot]; }
+    __device__ __forceinline__ bool next() {
+        if (!fused::warp_wait(&sh->job_full[slot], lap & 1u, &sh->gave_up)) return false;
+        return tc::uniform(job().live) != 0;
+    }
+    __device__ __forceinline__ void done() {
+        __syncwarp();
+        if (threadIdx.x % 32 == 0) tc::mbar_arrive(&sh->job_empty[slot]);
+        if (++slot == fused::JOBS) { slot = 0; lap++; }
+    }
+};
 
 template <int TYPE, int DIM>
 __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -291,55 +308,134 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
     extern __shared__ char raw[];
     const unsigned base = (tc::smem_u32(raw) + 1023u) & ~1023u;
     char *const smem = raw + (base - tc::smem_u32(raw));
-    const unsigned q_at = base, k_at = base + 2 * H::BYTES, v_at = k_at + H::STAGES * H::BYTES;
-    __shared__ Barriers sh;
+    const unsigned q_at = base, k_at = base + 2 * H::QUERIES * H::BYTES, v_at = k_at + H::STAGES * H::BYTES;
+    __shared__ __align__(16) Shared sh;
     const unsigned warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;
     unsigned *const gave_up = &sh.gave_up;
     if (threadIdx.x == 0) {
         sh.gave_up = 0u;
+        tc::mbar_init(&sh.answered, 1u); tc::mbar_init(&sh.wanted, 1u);
+        for (unsigned i = 0; i < JOBS; i++) { tc::mbar_init(&sh.job_full[i], 1u); tc::mbar_init(&sh.job_empty[i], 14u); }
         for (int w = 0; w < 2; w++) {
-            tc::mbar_init(&sh.q_full[w], 1u); tc::mbar_init(&sh.q_empty[w], 1u); tc::mbar_init(&sh.s_full[w], 1u); tc::mbar_init(&sh.o_full[w], 1u);
-            tc::mbar_init(&sh.s_free[w], 4u); tc::mbar_init(&sh.p_full[w], 4u);
+            for (int b = 0; b < 2; b++) { tc::mbar_init(&sh.q_full[b][w], 1u); tc::mbar_init(&sh.q_empty[b][w], 1u); }
+            tc::mbar_init(&sh.s_full[w], 1u); tc::mbar_init(&sh.o_full[w], 1u); tc::mbar_init(&sh.o_done[w], 1u);
+            tc::mbar_init(&sh.s_free[w], 4u); tc::mbar_init(&sh.p_full[w][0], 4u); tc::mbar_init(&sh.p_full[w][1], 4u); tc::mbar_init(&sh.o_free[w], 4u); tc::mbar_init(&sh.l_full[w], 4u);
         }
         for (int s = 0; s < 4; s++) { tc::mbar_init(&sh.k_full[s], 1u); tc::mbar_init(&sh.k_empty[s], 1u); tc::mbar_init(&sh.v_full[s], 1u); tc::mbar_init(&sh.v_empty[s], 1u); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tc::fence_proxy_async_smem();
     }
     if (warp == 9) tc::tmem_alloc(&sh.tmem, 512u);
+    Job begin;
+    bool found = false;
+    if (warp == 10) found = find_job(a, blockIdx.x, kv_heads, begin);       // beside the rest of the beginning
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
-    // Registers: 128 x (2 x 232 + 40) = 384 x 168, what the launch holds
-    if (warp >= 8) {
+    // Registers: 128 x (2 x 200 + 40 + 72) = 512 x 128, what the launch holds
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const unsigned quarter = warp & 3u, row = quarter * 32u + lane, lanes = tmem + (quarter << 21);
+        uint4 *const turn = reinterpret_cast<uint4 *>(smem + (2 * H::QUERIES + 2 * H::STAGES) * H::BYTES + quarter * 2048);
+        unsigned done = 0;                             // a bit for each tile: the parity of its jobs
+        bool ok = true;
+        for (Walk walk{&sh}; walk.next(); walk.done()) {
+            const Job &job = walk.job();
+            #pragma unroll 1
+            for (int w = 0; w < 2; w++) {
+                const int first = job.first[w], steps = job.steps[w];
+                if (first < 0) continue;
+                float factor = 0.f;
+                if (steps > 0) {
+                    ok = ok && warp_wait(&sh.l_full[w], done >> w & 1u, gave_up) && warp_wait(&sh.o_done[w], done >> w & 1u, gave_up);
+                    done ^= 1u << w;
+                    tc::tc_fence_after();
+                    factor = sh.factor[w][row];
+                }
+                char *const out = a.out + ((size_t)(job.q0 + first) * a.out_row + job.head[w] * a.out_head) * 2;
+                const int left = job.queries - first;
+                // 32 features at a time: a thread has its row's, and stores 16 bytes each of eight rows
+                #pragma unroll 1
+                for (int i = 0; i < DIM; i += 32) {
+                    float o[32];
+                    if (ok && steps > 0) { ld32(lanes + H::O + w * DIM + i, o); ld_done32(o); }
+                    unsigned p[16];
+                    #pragma unroll
+                    for (int x = 0; x < 16; x++) p[x] = !ok ? 0x7fff7fffu : steps == 0 ? 0u : mma::Of<TYPE>::pack(o[2 * x] * factor, o[2 * x + 1] * factor);
+                    if (i + 32 == DIM && steps > 0) {
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&sh.o_free[w]);
+                    }
+                    __syncwarp();
+                    #pragma unroll
+                    for (unsigned x = 0; x < 4; x++) turn[lane * 4 + (x ^ (lane >> 1 & 3u))] = make_uint4(p[4 * x], p[4 * x + 1], p[4 * x + 2], p[4 * x + 3]);
+                    __syncwarp();
+                    const unsigned f = i + (lane & 3u) * 8;
+                    #pragma unroll
+                    for (unsigned x = 0; x < 4; x++) {
+                        const unsigned r = x * 8 + (lane >> 2), q = quarter * 32 + r;
+                        if ((int)q < left && f < a.head_dim) *reinterpret_cast<uint4 *>(out + (q * a.out_row + f) * 2) = turn[r * 4 + ((lane & 3u) ^ (r >> 1 & 3u))];
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        tc::tc_fence_before();
+        __syncthreads();
+    } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         bool ok = true;
-        if (warp == 8) {
+        if (warp == 10) {
+            unsigned index, slot = 0, lap = 0, asked = 0, wanted = 0;
+            while (true) {
+                if (found) {
+                    ok = warp_wait(&sh.job_empty[slot], (lap & 1u) ^ 1u, gave_up);
+                    if (ok && lane == 0) { sh.jobs[slot] = begin; tc::mbar_arrive(&sh.job_full[slot]); }
+                    __syncwarp();
+                    if (++slot == JOBS) { slot = 0; lap++; }
+                    if (begin.both() > 0) ok = ok && warp_wait(&sh.wanted, wanted++ & 1u, gave_up);
+                    if (!ok) break;
+                }
+                if (lane == 0) ask_for_work(&sh);
+                __syncwarp();
+                ok = warp_wait(&sh.answered, asked++ & 1u, gave_up);
+                if (!ok) break;
+                const bool more = given_work(&sh, index);
+                tc::fence_proxy_async_smem();          // the answer has been read before the next one is written
+                __syncwarp();
+                if (!more) break;
+                found = find_job(a, index, kv_heads, begin);
+            }
+            if (warp_wait(&sh.job_empty[slot], (lap & 1u) ^ 1u, gave_up) && lane == 0) { sh.jobs[slot].live = 0; tc::mbar_arrive(&sh.job_full[slot]); }
+            __syncwarp();
+        } else if (warp == 8) {
             unsigned stage = 0, lap = 0, q_uses[2] = {0, 0};
-            for (unsigned index = blockIdx.x; ok; index += gridDim.x) {
-                Job job;
-                if (!find_job(a, index, kv_heads, job)) break;
-                const int steps = job.both();
-                for (int j = 0; j < steps && ok; j++) {
+            for (Walk walk{&sh}; ok && walk.next(); walk.done()) {
+                const Job &job = walk.job();
+                const int steps = tc::uniform(job.both()), k0 = tc::uniform(job.k0), kv_head = tc::uniform(job.kv_head);
+                for (int j = 0; j < steps; j++) {
                     ok = warp_wait(&sh.k_empty[stage], (lap & 1u) ^ 1u, gave_up);
                     if (!ok) break;
                     if (tc::elect_one()) {
                         tc::mbar_arrive_expect_tx(&sh.k_full[stage], H::BYTES);
                         #pragma unroll
-                        for (int c = 0; c < H::CHUNKS; c++)
-                            tc::tma_load_3d(k_at + stage * H::BYTES + c * H::CHUNK_BYTES, &k_map, c * 64, (int)job.kv_head, job.k0 + j * (int)TILE, &sh.k_full[stage]);
+                        for (int c = 0; c < H::CHUNKS; c++) tc::tma_load_3d(k_at + stage * H::BYTES + c * H::CHUNK_BYTES, &k_map, c * 64, kv_head, k0 + j * (int)TILE, &sh.k_full[stage]);
                     }
                     __syncwarp();
                     if (j == 0)
-                        for (int w = 0; w < 2 && ok; w++) {
-                            if (job.steps[w] == 0) continue;
-                            ok = warp_wait(&sh.q_empty[w], (q_uses[w] & 1u) ^ 1u, gave_up);
+                        #pragma unroll
+                        for (int w = 0; w < 2; w++) {
+                            if (!ok || tc::uniform(job.steps[w]) == 0) continue;
+                            const unsigned b = q_uses[w] % H::QUERIES, use = q_uses[w] / H::QUERIES;
+                            ok = warp_wait(&sh.q_empty[b][w], (use & 1u) ^ 1u, gave_up);
                             q_uses[w]++;
                             if (ok && tc::elect_one()) {
-                                tc::mbar_arrive_expect_tx(&sh.q_full[w], H::BYTES);
+                                tc::mbar_arrive_expect_tx(&sh.q_full[b][w], H::BYTES);
                                 #pragma unroll
                                 for (int c = 0; c < H::CHUNKS; c++)
-                                    tc::tma_load_3d(q_at + w * H::BYTES + c * H::CHUNK_BYTES, &q_map, c * 64, (int)job.head[w], job.q0 + job.first[w], &sh.q_full[w]);
+                                    tc::tma_load_3d(q_at + (b * 2 + w) * H::BYTES + c * H::CHUNK_BYTES, &q_map, c * 64, job.head[w], job.q0 + job.first[w], &sh.q_full[b][w]);
                             }
                             __syncwarp();
                         }
@@ -348,79 +444,99 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                     if (tc::elect_one()) {
                         tc::mbar_arrive_expect_tx(&sh.v_full[stage], H::BYTES);
                         #pragma unroll
-                        for (int c = 0; c < H::CHUNKS; c++)
-                            tc::tma_load_3d(v_at + stage * H::BYTES + c * H::CHUNK_BYTES, &v_map, c * 64, (int)job.kv_head, job.k0 + j * (int)TILE, &sh.v_full[stage]);
+                        for (int c = 0; c < H::CHUNKS; c++) tc::tma_load_3d(v_at + stage * H::BYTES + c * H::CHUNK_BYTES, &v_map, c * 64, kv_head, k0 + j * (int)TILE, &sh.v_full[stage]);
                     }
                     __syncwarp();
                     if (++stage == H::STAGES) { stage = 0; lap++; }
                 }
+                if (!ok) break;
             }
         } else if (warp == 9) {
             constexpr unsigned FORMAT = TYPE == ASPEN_B200_BF16 ? 1u : 0u;
             constexpr unsigned IDESC = 1u << 4 | FORMAT << 7 | FORMAT << 10 | (128u >> 4) << 24;       // sums fp32, 128 rows
             constexpr unsigned IDESC_S = IDESC | (128u >> 3) << 17, IDESC_O = IDESC | ((unsigned)DIM >> 3) << 17 | 1u << 16;      // the second operand of PV: features contiguous
-            unsigned stage = 0, lap = 0, q_uses[2] = {0, 0}, done[2] = {0, 0};
-            // scores of tile w over the keys of a stage
-            auto scores = [&](int w, unsigned st, bool last) {
+            unsigned stage = 0, lap = 0, q_uses[2] = {0, 0}, asked[2] = {0, 0}, done[2] = {0, 0}, outs[2] = {0, 0};
+            Walk walk{&sh};
+            // Steps of the job in work and of the next one.  Only the next is looked for while one is in work: the one behind it takes the place of the one in work.
+            int steps[2], next[2] = {0, 0}, keys = 0, next_keys = 0;
+            bool live = true, begun = false;          // begun: the next one's first scores have been asked for
+            auto look = [&]() {
+                next[0] = next[1] = 0;
+                live = walk.next();
+                if (!live) return;
+                const Job &job = walk.job();
+                next[0] = tc::uniform(job.steps[0]);
+                next[1] = tc::uniform(job.steps[1]);
+                next_keys = tc::uniform(job.keys);
+                walk.done();
+            };
+            // scores of tile w over the keys of stage `st`; the job's first or last ones
+            auto scores = [&](int w, unsigned st, bool first, bool last) {
+                const unsigned use = q_uses[w], b = use % H::QUERIES;
+                if (first) ok = ok && warp_wait(&sh.q_full[b][w], use / H::QUERIES & 1u, gave_up);
+                // a tile's softmax has read its scores before: it has given their weights, or (weights of their own) said so
+                if (H::OWN_P) ok = ok && warp_wait(&sh.s_free[w], (asked[w] & 1u) ^ 1u, gave_up);
+                asked[w]++;
+                if (last) q_uses[w]++;
+                if (!ok) return;
+                tc::tc_fence_after();
+                const unsigned q = q_at + (b * 2 + w) * H::BYTES;
                 if (tc::elect_one()) {
                     #pragma unroll
                     for (int c = 0; c < H::CHUNKS; c++)
                         #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            mma_ss(tmem + H::S + w * 128, tc::umma_desc_low(q_at + w * H::BYTES + c * H::CHUNK_BYTES + k * 32), tc::umma_desc_low(k_at + st * H::BYTES + c * H::CHUNK_BYTES + k * 32), IDESC_S, c + k);
+                            mma_ss(tmem + H::S + w * 128, tc::umma_desc_low(q + c * H::CHUNK_BYTES + k * 32), tc::umma_desc_low(k_at + st * H::BYTES + c * H::CHUNK_BYTES + k * 32), IDESC_S, c + k);
                     tc::tc_commit(&sh.s_full[w]);
-                    if (last) tc::tc_commit(&sh.q_empty[w]);
+                    if (last) tc::tc_commit(&sh.q_empty[b][w]);
                 }
                 __syncwarp();
             };
-            auto values = [&](int w, unsigned st, bool first) {
+            // keys 16 from ... of the step
+            auto values = [&](int w, unsigned st, bool first, bool last, int from, int to) {
                 if (tc::elect_one()) {
                     #pragma unroll
-                    for (int k = 0; k < 8; k++)
+                    for (int k = from; k < to; k++)
                         mma_ts(tmem + H::O + w * DIM, tmem + H::P + w * H::P_APART + k * 8, (v_at + st * H::BYTES + k * 2048) >> 4 | (H::CHUNK_BYTES >> 4) << 16, IDESC_O, first ? k : 1);
-                    tc::tc_commit(&sh.o_full[w]);
+                    if (to == 8) { tc::tc_commit(&sh.o_full[w]); if (last) tc::tc_commit(&sh.o_done[w]); }
                 }
                 __syncwarp();
             };
             auto release = [&](unsigned long long *bar) { if (tc::elect_one()) tc::tc_commit(bar); __syncwarp(); };
-            for (unsigned index = blockIdx.x; ok; index += gridDim.x) {
-                Job job;
-                if (!find_job(a, index, kv_heads, job)) break;
-                const int steps = job.both();
-                if (steps == 0) continue;
-                ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
-                for (int w = 0; w < 2 && ok; w++) {
-                    if (job.steps[w] == 0) continue;
-                    ok = warp_wait(&sh.q_full[w], q_uses[w] & 1u, gave_up);
-                    q_uses[w]++;
-                    // a tile's softmax has read its last scores: it has given their weights, or (weights of their own) said so
-                    if (H::OWN_P) ok = ok && warp_wait(&sh.s_free[w], (done[w] & 1u) ^ 1u, gave_up);
+            for (look(); ok && live;) {
+                if (!next[0] && !next[1]) { look(); continue; }
+                if (!begun) {
+                    ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
+                    #pragma unroll
+                    for (int w = 0; w < 2; w++) if (next[w]) scores(w, stage, true, next[w] == 1);
                     if (!ok) break;
-                    tc::tc_fence_after();
-                    scores(w, stage, job.steps[w] == 1);
+                    release(&sh.k_empty[stage]);
                 }
-                if (!ok) break;
-                release(&sh.k_empty[stage]);
-                for (int j = 0; j < steps && ok; j++) {
+                begun = false;
+                steps[0] = next[0]; steps[1] = next[1]; keys = next_keys;
+                const int all = max(steps[0], steps[1]);
+                for (int j = 0; j < all; j++) {
                     const unsigned here = stage, at = lap;
                     if (++stage == H::STAGES) { stage = 0; lap++; }
-                    const bool more = j + 1 < steps;
+                    // the scores to ask for now: the next step's, or the next job's first ones
+                    const bool turn = j + 1 == all;
+                    if (j == max(0, all - 3) && lane == 0) tc::mbar_arrive(&sh.wanted);
+                    if (turn) look();
+                    const int then = turn ? 0 : j + 1, until0 = turn ? next[0] : steps[0], until1 = turn ? next[1] : steps[1];
+                    const bool more = then < until0 || then < until1;
+                    begun = turn && more;
+                    if (more) ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
+                    if (!ok) break;
                     if (H::OWN_P && more) {
-                        ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
-                        for (int w = 0; w < 2 && ok; w++) {
-                            if (j + 1 >= job.steps[w]) continue;
-                            ok = warp_wait(&sh.s_free[w], done[w] & 1u, gave_up);
-                            if (!ok) break;
-                            tc::tc_fence_after();
-                            scores(w, stage, j + 2 == job.steps[w]);
-                        }
+                        #pragma unroll
+                        for (int w = 0; w < 2; w++) { const int until = w ? until1 : until0; if (then < until) scores(w, stage, turn, then + 1 == until); }
                         if (!ok) break;
                         release(&sh.k_empty[stage]);
                     }
                     ok = warp_wait(&sh.v_full[here], at & 1u, gave_up);
                     if (!ok) break;
-                    if (job.keys < (j + 1) * (int)TILE) {
-                        const int from = job.keys - j * (int)TILE;
+                    if (keys < (j + 1) * (int)TILE) {
+                        const int from = keys - j * (int)TILE;
                         char *const v = smem + (v_at - base) + here * H::BYTES;
                         for (int i = from * 8 + (int)lane; i < (int)TILE * 8; i += 32)
                             #pragma unroll
@@ -428,15 +544,22 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                         tc::fence_proxy_async_smem();
                         __syncwarp();
                     }
-                    if (!H::OWN_P && more) ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
-                    for (int w = 0; w < 2 && ok; w++) {
-                        if (j >= job.steps[w]) continue;
-                        ok = warp_wait(&sh.p_full[w], done[w] & 1u, gave_up);
-                        if (!ok) break;
-                        done[w]++;
-                        tc::tc_fence_after();
-                        values(w, here, j == 0);
-                        if (!H::OWN_P && j + 1 < job.steps[w]) scores(w, stage, j + 2 == job.steps[w]);
+                    #pragma unroll
+                    for (int w = 0; w < 2; w++) {
+                        const int until = w ? until1 : until0;
+                        if (ok && j < steps[w]) {
+                            if (j == 0) { ok = warp_wait(&sh.o_free[w], (outs[w] & 1u) ^ 1u, gave_up); outs[w]++; }        // the job before has been written out
+                            ok = ok && warp_wait(&sh.p_full[w][0], done[w] & 1u, gave_up);
+                            if (!ok) continue;
+                            tc::tc_fence_after();
+                            values(w, here, j == 0, false, 0, 6);
+                            ok = warp_wait(&sh.p_full[w][1], done[w] & 1u, gave_up);
+                            if (!ok) continue;
+                            done[w]++;
+                            tc::tc_fence_after();
+                            values(w, here, false, j + 1 == steps[w], 6, 8);
+                        }
+                        if (!H::OWN_P && ok && then < until) scores(w, stage, turn, then + 1 == until);
                     }
                     if (!ok) break;
                     release(&sh.v_empty[here]);
@@ -458,19 +581,23 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
             tc::tmem_dealloc(tmem, 512u);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int w = (int)(warp >> 2);
         const unsigned row = (warp & 3u) * 32u + lane, lanes = tmem + ((warp & 3u) << 21), s_at = lanes + H::S + w * 128, p_at = lanes + H::P + w * H::P_APART, o_at = lanes + H::O + w * DIM;
-        unsigned done = 0;
+        const Pair scale2 = pair(a.scale, a.scale);
+        unsigned done = 0, outs = 0;
         bool ok = true;
-        for (unsigned index = blockIdx.x;; index += gridDim.x) {
-            Job job;
-            if (!find_job(a, index, kv_heads, job)) break;
-            if (job.first[w] < 0) continue;
-            const int query = job.first[w] + (int)row, steps = job.steps[w];
+        for (Walk walk{&sh}; ok && walk.next(); walk.done()) {
+            const Job &job = walk.job();
+            const int first = job.first[w], steps = tc::uniform(job.steps[w]);
+            if (first < 0 || steps == 0) continue;
+            const int query = first + (int)row;
             const int seen = a.masked ? min(job.keys, query + job.behind() + 1) : job.keys;              // first key that the row does not see
-            const int warp_seen = __shfl_sync(0xffffffffu, seen, 0);                                      // of the warp's first row, which sees least
+            const int least_seen = __shfl_sync(0xffffffffu, seen, 0), most_seen = __shfl_sync(0xffffffffu, seen, 31);       // of the warp's rows
             float max = -INFINITY, sum = 0.f;
+            // a NaN stays the maximum, and so it becomes if a score is infinite: then all weights of the row are NaN
+            auto grow = [&](float most) { max = max2(max, most); if (max == INFINITY) max = NAN; };
+            #pragma unroll 1
             for (int j = 0; j < steps && ok; j++) {
                 ok = warp_wait(&sh.s_full[w], done & 1u, gave_up);
                 if (!ok) break;
@@ -485,77 +612,72 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&sh.s_free[w]);
                 }
-                if (warp_seen < (j + 1) * (int)TILE) {
-                    const int left = seen - j * (int)TILE;
+                const int key0 = j * (int)TILE;
+                if (least_seen < key0 + (int)TILE) {
                     #pragma unroll
-                    for (int i = 0; i < 128; i++) s[i] = i < left ? s[i] : -INFINITY;
+                    for (int h = 0; h < 4; h++) {
+                        if (least_seen >= key0 + 32 * (h + 1)) continue;
+                        const int left = seen - key0 - 32 * h;
+                        #pragma unroll
+                        for (int i = 0; i < 32; i++) s[h * 32 + i] = i < left ? s[h * 32 + i] : -INFINITY;
+                    }
                 }
                 float m0 = max3(s[0], s[1], s[2]), m1 = max3(s[3], s[4], s[5]), m2 = max3(s[6], s[7], s[8]), m3 = max3(s[9], s[10], s[11]);
                 #pragma unroll
                 for (int i = 12; i < 124; i += 8) { m0 = max3(m0, s[i], s[i + 1]); m1 = max3(m1, s[i + 2], s[i + 3]); m2 = max3(m2, s[i + 4], s[i + 5]); m3 = max3(m3, s[i + 6], s[i + 7]); }
                 m0 = max3(m0, s[124], s[125]); m1 = max3(m1, s[126], s[127]);
-                const float most = fmaxf(max3(m0, m1, m2), m3);
-                // both -inf: not a number, and nothing to do
-                if (__any_sync(0xffffffffu, (most - max) * a.scale > 8.f)) {
-                    const float next = fmaxf(max, most), down = next == -INFINITY ? 1.f : mma::exp2_fast((max - next) * a.scale);
-                    if (j > 0) {
-                        if (H::OWN_P) ok = warp_wait(&sh.o_full[w], (done & 1u) ^ 1u, gave_up);
-                        if (!ok) break;
-                        tc::tc_fence_after();
+                const float top = max2(max3(m0, m1, m2), m3);
+                if (H::OWN_P && done > 0) { ok = warp_wait(&sh.o_full[w], (done & 1u) ^ 1u, gave_up); tc::tc_fence_after(); }
+                if (j == 0) grow(top);
+                else if (__any_sync(0xffffffffu, (top - max) * a.scale > 8.f || (top != top && max == max))) {
+                    const float before = max;
+                    grow(top);
+                    const float down = max == -INFINITY ? 1.f : mma::exp2_fast((before - max) * a.scale);
+                    #pragma unroll 1
+                    for (int i = 0; i < DIM; i += 16) {
+                        float o[16];
+                        ld16(o_at + i, o);
+                        ld_done16(o);
                         #pragma unroll
-                        for (int i = 0; i < DIM; i += 32) {
-                            float o[32];
-                            ld32(o_at + i, o);
-                            ld_done32(o);
-                            #pragma unroll
-                            for (int x = 0; x < 32; x++) o[x] *= down;
-                            st32(o_at + i, reinterpret_cast<unsigned *>(o));
-                        }
+                        for (int x = 0; x < 16; x++) o[x] *= down;
+                        st16(o_at + i, reinterpret_cast<unsigned *>(o));
                     }
                     sum *= down;
-                    max = next;
                 }
                 const float ref = max == -INFINITY ? 0.f : -max * a.scale;
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                const Pair ref2 = pair(ref, ref);
+                Pair part[4] = {0ull, 0ull, 0ull, 0ull};
                 #pragma unroll
-                for (int i = 0; i < 128; i++) { s[i] = mma::exp2_fast(fmaf(s[i], a.scale, ref)); part[i & 3] += s[i]; }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                // the weights' place is free: the product before has been through (in the place of the scores: it was before these)
-                if (H::OWN_P && j > 0) {
-                    ok = warp_wait(&sh.o_full[w], (done & 1u) ^ 1u, gave_up);
-                    if (!ok) break;
-                    tc::tc_fence_after();
-                }
-                #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    unsigned p[32];
+                for (int h = 0; h < 4; h++) {
+                    unsigned p[16];
                     #pragma unroll
-                    for (int i = 0; i < 32; i++) p[i] = mma::Of<TYPE>::pack(s[h * 64 + 2 * i], s[h * 64 + 2 * i + 1]);
-                    st32(p_at + h * 32, p);
+                    for (int i = 0; i < 16; i++) {
+                        const Pair x = fma2(pair(s[h * 32 + 2 * i], s[h * 32 + 2 * i + 1]), scale2, ref2);
+                        float y0, y1;
+                        unpair(x, y0, y1);
+                        y0 = mma::exp2_fast(y0); y1 = mma::exp2_fast(y1);
+                        part[i & 3] = add2(part[i & 3], pair(y0, y1));
+                        p[i] = mma::Of<TYPE>::pack(y0, y1);
+                    }
+                    st16(p_at + h * 16, p);
+                    if (h >= 2) {
+                        st_done();
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&sh.p_full[w][h - 2]);
+                    }
                 }
-                st_done();
-                tc::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&sh.p_full[w]);
+                float x0, x1;
+                unpair(add2(add2(part[0], part[1]), add2(part[2], part[3])), x0, x1);
+                sum += x0 + x1;
                 done++;
             }
-            // outputs: a row a thread
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            if (ok && steps > 0) ok = warp_wait(&sh.o_full[w], (done & 1u) ^ 1u, gave_up);
-            tc::tc_fence_after();
-            const bool mine = query < job.queries;
-            char *const out = a.out + ((size_t)(job.q0 + query) * a.out_row + job.head[w] * a.out_head) * 2;
-            #pragma unroll
-            for (int i = 0; i < DIM; i += 32) {
-                float o[32];
-                if (ok && steps > 0) { ld32(o_at + i, o); ld_done32(o); }
-                unsigned p[16];
-                #pragma unroll
-                for (int x = 0; x < 16; x++) p[x] = !ok ? 0x7fff7fffu : steps == 0 ? 0u : mma::Of<TYPE>::pack(o[2 * x] * inv, o[2 * x + 1] * inv);
-                #pragma unroll
-                for (int x = 0; x < 4; x++)
-                    if (mine && i + 8 * x < (int)a.head_dim) *reinterpret_cast<uint4 *>(out + (i + 8 * x) * 2) = make_uint4(p[4 * x], p[4 * x + 1], p[4 * x + 2], p[4 * x + 3]);
-            }
+            // what the outputs are multiplied with, once the job before's have been
+            ok = ok && warp_wait(&sh.o_free[w], (outs & 1u) ^ 1u, gave_up);
+            outs++;
+            if (ok) sh.factor[w][row] = sum == 0.f ? 0.f : 1.f / sum;
+            __syncwarp();
+            if (lane == 0 && ok) tc::mbar_arrive(&sh.l_full[w]);
         }
         __syncwarp();
         tc::tc_fence_before();
@@ -582,23 +704,24 @@ bool encode(CUtensorMap *map, int type, const char *p, unsigned dim, unsigned he
 }
 
 template <int TYPE, int DIM>
-cudaError_t launch_tiles(const Args &a, const CUtensorMap *maps, unsigned sms, cudaStream_t stream) {
+cudaError_t launch_tiles(const Args &a, const CUtensorMap *maps, cudaStream_t stream) {
     cudaError_t err = cudaFuncSetAttribute(prompt_tiles<TYPE, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, fused::Shape<DIM>::SMEM);
     if (err != cudaSuccess) return err;
     const unsigned long long kv_heads = a.heads / a.group, sequences = a.sequences < a.q_rows ? a.sequences : a.q_rows;
     const unsigned long long jobs = ((a.q_rows / fused::TILE + sequences) * a.group + sequences) / 2 * kv_heads;       // at most
-    prompt_tiles<TYPE, DIM><<<(unsigned)(jobs < sms ? jobs : sms), fused::THREADS, fused::Shape<DIM>::SMEM, stream>>>(maps[0], maps[1], maps[2], a, (unsigned)kv_heads);
+    if (jobs > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+    prompt_tiles<TYPE, DIM><<<(unsigned)jobs, fused::THREADS, fused::Shape<DIM>::SMEM, stream>>>(maps[0], maps[1], maps[2], a, (unsigned)kv_heads);
     return cudaGetLastError();
 }
 // False: not a call for these kernels.
-bool try_tiles(const Args &a, int type, unsigned sms, cudaStream_t stream, cudaError_t *err) {
+bool try_tiles(const Args &a, int type, cudaStream_t stream, cudaError_t *err) {
     if (type == ASPEN_B200_FP32 || a.head_dim > 128 || !a.kv_rows || !(a.scale > 0.f) || !encode_fn()) return false;      // a row's largest score is its largest product only for a scale above 0
     const unsigned kv_heads = a.heads / a.group;
     CUtensorMap maps[3];
     if (!encode(&maps[0], type, a.q, a.head_dim, a.heads, a.q_rows, a.q_head, a.q_row) || !encode(&maps[1], type, a.k, a.head_dim, kv_heads, a.kv_rows, a.k_head, a.k_row) ||
         !encode(&maps[2], type, a.v, a.head_dim, kv_heads, a.kv_rows, a.v_head, a.v_row)) return false;
-    if (a.head_dim <= 64) *err = type == ASPEN_B200_BF16 ? launch_tiles<ASPEN_B200_BF16, 64>(a, maps, sms, stream) : launch_tiles<ASPEN_B200_FP16, 64>(a, maps, sms, stream);
-    else *err = type == ASPEN_B200_BF16 ? launch_tiles<ASPEN_B200_BF16, 128>(a, maps, sms, stream) : launch_tiles<ASPEN_B200_FP16, 128>(a, maps, sms, stream);
+    if (a.head_dim <= 64) *err = type == ASPEN_B200_BF16 ? launch_tiles<ASPEN_B200_BF16, 64>(a, maps, stream) : launch_tiles<ASPEN_B200_FP16, 64>(a, maps, stream);
+    else *err = type == ASPEN_B200_BF16 ? launch_tiles<ASPEN_B200_BF16, 128>(a, maps, stream) : launch_tiles<ASPEN_B200_FP16, 128>(a, maps, stream);
     return true;
 }
 
@@ -647,7 +770,7 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     a.scale = p->scale * 1.4426950408889634f;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t err = cudaSuccess;
-    if (!try_tiles(a, p->type, (unsigned)sms, stream, &err))
+    if (!try_tiles(a, p->type, stream, &err))
         err = p->type == ASPEN_B200_FP32 ? launch_rows<ASPEN_B200_FP32>(a, stream) : p->type == ASPEN_B200_BF16 ? launch_rows<ASPEN_B200_BF16>(a, stream) : launch_rows<ASPEN_B200_FP16>(a, stream);
     if (err != cudaSuccess) { cudaGetLastError(); ASPEN_ERR("%s: %s\n", what, cudaGetErrorString(err)); return -3; }
     return 0;

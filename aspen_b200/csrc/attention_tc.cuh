@@ -4,18 +4,28 @@
 //     S [128 queries x 128 keys] = Q K^T     both operands in shared memory, K-major, scores in TMEM
 //     P = exp2(S - max)                      a thread a query: its row of scores from TMEM to registers, weights back to TMEM as 16-bit pairs
 //     O [128 queries x features] += P V      P from TMEM, V as it lies in memory (features contiguous: the MN-major operand), sums in TMEM
-// The running maximum is followed loosely: O and the sum are scaled again only when a row's maximum has grown by more than 2^8 (weights up to 256 are as exact as weights up to 1),
-// so the sums in TMEM are hardly ever read before the end.
+// The maximum is followed loosely: O and the sum are scaled again only when a row's maximum has grown by more than 2^8 (weights up to 256 are as exact as weights up to 1), so the
+// sums in TMEM are hardly ever read before the end.
 //
-// Warps: 0 - 3 and 4 - 7 the softmax of the two tiles, 8 TMA, 9 MMA; nothing but mbarriers connects them, and while one tile's scores are weighed the other's are multiplied.  TMEM, 512
-// columns: scores 2 x 128, sums 2 x features, and with 64 features weights 2 x 64 of their own, so that the next scores are there before the weights of these have been
-// multiplied; with 128 the weights take the place of their scores.
+// Warps: 0 - 3 and 4 - 7 the softmax of the two tiles, 8 TMA, 9 MMA, 10 finds the work, 12 - 15 write outputs; nothing but mbarriers connects them, and while one tile's scores are weighed
+// the other's are multiplied.  The first three quarters of a tile's weights are multiplied while the last one is computed.  TMEM, 512 columns: scores 2 x 128, sums 2 x features, and with 64
+// features weights 2 x 64 of their own, so that the next scores, the next job's too, are there before the weights of these have been multiplied; with 128 the weights take the place of their
+// scores.
 //
-// What bounds it: a step of two tiles is 2048 cycles of the tensor pipe with 128 features, 1024 with 64, and 2048 of the unit for exp2.
+// A CTA takes job after job: heavy and light ones, whatever the lengths, so the hardware deals them (a running CTA takes over the work of one that has not begun).  The next one is asked
+// for three steps before this one ends, and its queries and keys come in under the last steps.  (Asked for at once, CTAs held up to three jobs: of 24 packed prompts one had 8 steps and
+// another 25; dealt in turn, 4 prompts of 1231 to 4096 tokens took 152 units of time where 120 are possible.)
+//
+// What bounds it.  With 128 features a step of two tiles takes 2048 cycles of the tensor pipe at best, and as many of shared memory (Q and K are read from there for each
+// product, 128 bytes a cycle; the copies of K and V come on top); with 64 features 1024, and 2048 of the unit for exp2.  4 prompts of 1231 to 4096 tokens, 32 heads over 8 of
+// 128: 234 us, 1070 TFLOP/s of visible products, 3700 cycles a step: the chain of a tile (scores from TMEM 100, maximum 270, exponentials and sums 1250, then its products 900)
+// is as long as that with the other tile's in between.  24 packed prompts of 12 heads of 64: 55 us.
+// Tried and slower: two threads a query (16 warps: registers), a quarter of the exponentials by polynomials in packed multiply-adds (FMA and ALU then take what the exp2 unit gives; their
+// second copy of the code costs instruction fetches), weights from the maximum of the step before with a second try (the same), 32 keys a turn in a loop (24 packed prompts 72 us).
 //
 // Values behind the end of a sequence are another one's, or nobody's: the MMA warp sets them to zero in shared memory, since 0 x NaN would reach every row.
 //
-// Every wait is bounded (2 s) and is for another role of the CTA; if one runs out all roles leave, TMEM is freed and the CTA's rows of out that are not done become NaN.
+// Every wait is bounded (2 s) and is for another role of the CTA; if one runs out all roles leave, TMEM is freed and the rows of out that were in work become NaN.
 #pragma once
 #include "tiles_tc.cuh"
 
@@ -23,24 +33,55 @@
 
 namespace fused {
 
-constexpr unsigned THREADS = 384, TILE = 128;
+constexpr unsigned THREADS = 512, TILE = 128;
 constexpr unsigned long long LIMIT_NS = 2000000000ull;
 
 template <int DIM>
 struct Shape {
     static constexpr int CHUNKS = DIM / 64;                         // of 64 features: 128 bytes, the swizzle's width
     static constexpr int CHUNK_BYTES = TILE * 128, BYTES = CHUNKS * CHUNK_BYTES;    // of a tile of queries, keys or values
-    static constexpr int STAGES = DIM == 64 ? 4 : 2;
-    static constexpr int SMEM = 2 * BYTES + 2 * STAGES * BYTES + 2048;
+    static constexpr int STAGES = DIM == 64 ? 4 : 2, QUERIES = DIM == 64 ? 2 : 1;     // buffers: keys and values; queries of both tiles
+    static constexpr int OUT_BYTES = 4 * 2048;                      // where a warp turns its outputs round
+    static constexpr int SMEM = 2 * QUERIES * BYTES + 2 * STAGES * BYTES + OUT_BYTES + 1024;
     static constexpr bool OWN_P = DIM == 64;
     static constexpr unsigned S = 0, O = 256, P = OWN_P ? 384 : 0, P_APART = OWN_P ? 64 : 128;      // TMEM columns
 };
 
-struct Barriers {
-    unsigned long long q_full[2], q_empty[2], k_full[4], k_empty[4], v_full[4], v_empty[4];
-    unsigned long long s_full[2], s_free[2], p_full[2], o_full[2];
+// A CTA's work: two tiles of queries of one sequence and one head of keys.
+struct Job {
+    int q0, queries, k0, keys;
+    int kv_head, head[2];
+    int first[2], steps[2];                        // first query of a tile, -1: no such tile; steps of 128 keys
+    int live;                                      // 0: there are no more
+    __device__ __forceinline__ int both() const { return max(steps[0], steps[1]); }
+    __device__ __forceinline__ int behind() const { return keys - queries; }
+    __device__ __forceinline__ int end(int w, int masked) const { return masked ? max(0, min(keys, min(queries, first[w] + (int)TILE) + behind())) : keys; }
+};
+constexpr unsigned JOBS = 2;                       // the one in work and the next
+
+struct Shared {
+    uint4 answer;                                  // to a request for another CTA's work
+    unsigned long long answered, wanted, job_full[JOBS], job_empty[JOBS];
+    unsigned long long q_full[2][2], q_empty[2][2], k_full[4], k_empty[4], v_full[4], v_empty[4];      // q: [buffer][tile]
+    unsigned long long s_full[2], s_free[2], p_full[2][2], o_full[2];
+    unsigned long long o_done[2], o_free[2], l_full[2];                                                // a job's sums: complete, read; the rows' factors
+    Job jobs[JOBS];
+    float factor[2][TILE];
     unsigned gave_up, tmem;
 };
+
+// The hardware deals the CTAs of the grid; one that runs asks for the next that has not begun, which then never does.
+__device__ __forceinline__ void ask_for_work(Shared *sh) {
+    tc::mbar_arrive_expect_tx(&sh->answered, 16u);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(tc::smem_u32(&sh->answer)), "r"(tc::smem_u32(&sh->answered)) : "memory");
+}
+// The number of the CTA whose work this one has been given; false: none is left.
+__device__ __forceinline__ bool given_work(Shared *sh, unsigned &index) {
+    unsigned yes;
+    asm volatile("{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%2];\n\tclusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\t"
+                 "mov.u32 %1, 0;\n\t@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}" : "=r"(yes), "=r"(index) : "r"(tc::smem_u32(&sh->answer)) : "memory");
+    return yes != 0u;
+}
 
 __device__ __forceinline__ bool wait(unsigned long long *bar, unsigned parity, unsigned *gave_up) {
     #pragma unroll 1
@@ -96,27 +137,32 @@ __device__ __forceinline__ void ld_done32(float *v) {
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]) : : "memory");
     asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) : : "memory");
 }
-__device__ __forceinline__ void st32(unsigned at, const unsigned *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+__device__ __forceinline__ void ld16(unsigned at, float *v) {
+    unsigned *r = reinterpret_cast<unsigned *>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ld_done16(float *v) {
+    unsigned *r = reinterpret_cast<unsigned *>(v);
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) : : "memory");
+}
+__device__ __forceinline__ void st16(unsigned at, const unsigned *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                  ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+typedef unsigned long long Pair;         // two fp32 values
+__device__ __forceinline__ Pair pair(float x, float y) { Pair p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y)); return p; }
+__device__ __forceinline__ void unpair(Pair p, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { Pair d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) { Pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
 
-// A CTA's work: two tiles of queries of one sequence and one head of keys.
-struct Job {
-    int q0, queries, k0, keys;
-    unsigned kv_head, head[2];
-    int first[2], steps[2];                        // first query of a tile; steps of 128 keys, 0: no such tile
-    __device__ __forceinline__ int both() const { return max(steps[0], steps[1]); }
-    __device__ __forceinline__ int behind() const { return keys - queries; }
-    __device__ __forceinline__ int end(int w, int masked) const { return masked ? max(0, min(keys, min(queries, first[w] + (int)TILE) + behind())) : keys; }
-};
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+__device__ __forceinline__ float max2(float a, float b) { float d; asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b)); return d; }
 
 }  // namespace fused
