@@ -20,7 +20,13 @@ namespace {
 using attn::Pages;
 
 constexpr int STEP = 16;                        // keys of a step
-constexpr int JOINERS = 256;
+
+// Heads of a group that one pass over the keys serves: eight columns of a product, or sixteen where their sums leave room in the registers.
+constexpr unsigned heads_of_pass(unsigned group, unsigned dim, int type) { return group <= 8 || dim == 256 || (type == ASPEN_B200_FP32 && dim == 128) ? 8 : 16; }
+constexpr unsigned dim_of(unsigned head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+// Threads of a CTA and CTAs on an SM: the warps that the registers are enough for.  16 with 120 registers (16 bits, 64 features), 12 with 168, 8 with 255.
+constexpr int ctas_of(int type, unsigned dim) { return type != ASPEN_B200_FP32 && dim == 64 ? 2 : 1; }
+constexpr int threads_of(int type, unsigned dim, unsigned heads) { return heads == 8 && dim == (type == ASPEN_B200_FP32 ? 64 : 128) ? 384 : 256; }
 
 struct Args {
     const char *q, *k, *v;
@@ -31,20 +37,21 @@ struct Args {
     unsigned entries, kv_heads, group, chunks, head_dim;    // chunks: of a group, each up to the kernel's HEADS
     float scale;                                // with log2(e)
     int *record;                                // [CTAs][2]: item that goes on behind the CTA (-1: none), last CTA that has some of it
-    float *part;                                // [CTAs][2][HEADS][DIM + 2]: what began before the CTA, and what goes on behind it
+    float *part;                                // [CTAs][2][HEADS][DIM + 4]: what began before the CTA, and what goes on behind it
 };
 
-// Threads 0 ... 255 of a CTA: steps of all items, and where each thread's entries begin in the line.
+// Steps of all items, and where each thread's entries begin in the line.
+template <int THREADS>
 struct Line {
-    unsigned long long before[257];             // [i]: steps of the entries before thread i's; [256]: all
-    unsigned long long sums[8];
+    unsigned long long before[THREADS + 1];     // [i]: steps of the entries before thread i's; [THREADS]: all
+    unsigned long long sums[THREADS / 32];
 };
 
 __device__ __forceinline__ unsigned steps_of(unsigned tokens) { return (tokens + STEP - 1) / STEP; }
 __device__ __forceinline__ int slot_of(const Args &a, unsigned e) { return a.slots ? a.slots[e] : (int)e; }
 
 template <int THREADS>
-__device__ void measure(const Args &a, unsigned each, Line &line) {
+__device__ void measure(const Args &a, unsigned each, Line<THREADS> &line) {
     const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     unsigned long long mine = 0;
     for (unsigned i = 0; i < each; i++) {
@@ -90,7 +97,7 @@ struct Running {
                 for (int m = 4; m < 32; m <<= 1) sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], m);
     }
     // First feature of this lane's piece p, and the values there: PIECE of them for head 2 t + j.
-    static constexpr int PIECE = TYPE == ASPEN_B200_FP32 ? 4 : 8, PIECES = DIM / (8 * PIECE);
+    static constexpr int PIECE = TYPE == ASPEN_B200_FP32 || DIM == 64 ? 8 : 16, PIECES = DIM / (8 * PIECE);
     static __device__ __forceinline__ int feature(int p, unsigned g) { return p * 8 * PIECE + (int)g * PIECE; }
     __device__ __forceinline__ float value(int n, int p, int x, int j) const { return o[n][p * (PIECE / 2) + x / 2][(x & 1) * 2 + j]; }
 };
@@ -110,10 +117,28 @@ __device__ __forceinline__ void store_value(char *at, float v) {
     else *reinterpret_cast<__half *>(at) = __float2half_rn(v);
 }
 
-__device__ __forceinline__ uint4 load_piece(const char *p, bool ok) {
+__device__ __forceinline__ uint4 load16(const char *p, bool ok) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (ok) asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
+}
+// A lane's 32 bytes of a row: one load where every row starts on a 32-byte boundary (WIDE), else two.
+struct Piece { unsigned w[8]; };
+template <bool WIDE, int BYTES>
+__device__ __forceinline__ void load_piece(Piece &v, const char *p, bool ok, int left) {
+    if (WIDE && BYTES == 32) {
+        #pragma unroll
+        for (int i = 0; i < 8; i++) v.w[i] = 0u;
+        if (ok && left > 0)
+            asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7]) : "l"(p));
+    } else {
+        #pragma unroll
+        for (int h = 0; h < BYTES / 16; h++) {
+            const uint4 x = load16(p + h * 16, ok && left > h * 16);
+            v.w[4 * h] = x.x; v.w[4 * h + 1] = x.y; v.w[4 * h + 2] = x.z; v.w[4 * h + 3] = x.w;
+        }
+    }
 }
 
 // An item and its steps from `begin` to `end`.
@@ -122,15 +147,18 @@ struct Share {
     int slot;
 };
 
-template <int TYPE, int DIM, int HEADS>
+template <int TYPE, int DIM, int HEADS, bool WIDE>
 struct Kernel {
-    static constexpr int SIZE = TYPE == ASPEN_B200_FP32 ? 4 : 2, VALUES = 16 / SIZE;
-    static constexpr int WIDTH = DIM < 512 / (SIZE * 2) ? DIM : 512 / (SIZE * 2);      // features of a buffer of eight pieces: 128 of 16 bits, 64 of 32
-    static constexpr int CHUNKS = DIM / WIDTH, PIECES = WIDTH / (4 * VALUES);   // pieces of a lane and row of keys
-    static constexpr int THREADS = 256, WARPS = THREADS / 32;
-    static constexpr int ROW = DIM + 2;         // floats of a partial result of one head: values, maximum, sum
+    static constexpr int SIZE = TYPE == ASPEN_B200_FP32 ? 4 : 2, ROW_BYTES = DIM * SIZE;
+    // Bytes of a lane's piece of a row: of keys (four lanes to a row), of values (eight).  A buffer is what is on its way together: 128 bytes a lane.
+    static constexpr int KEY_PIECE = 32, VALUE_PIECE = ROW_BYTES / 8 < 32 ? ROW_BYTES / 8 : 32;
+    static constexpr int CHUNK = ROW_BYTES < 256 ? ROW_BYTES : 256, CHUNKS = ROW_BYTES / CHUNK;       // bytes of a row in a buffer
+    static constexpr int KEYS = CHUNK / (4 * KEY_PIECE), VALUES = CHUNK / (8 * VALUE_PIECE);          // pieces of a row
+    static constexpr int THREADS = threads_of(TYPE, DIM, HEADS), WARPS = THREADS / 32;
+    static constexpr int ROW = DIM + 4;         // floats of a partial result of one head: values, maximum, sum
     static constexpr unsigned SMEM = WARPS * 2 * HEADS * ROW * 4;
     typedef Running<TYPE, DIM, HEADS> Run;
+    struct Buffer { Piece p[4]; };
 
     // Byte offset of the row of key `lane % 32` behind `first`; -1 if there is none.
     static __device__ __forceinline__ long long row_of(const Args &a, const Share &s, unsigned first, unsigned lane) {
@@ -141,66 +169,70 @@ struct Kernel {
     }
 
     // Keys: rows g and g + 8 of the step.  Values: rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
-    static __device__ __forceinline__ void load_keys(uint4 *buf, const char *base, long long row0, long long row8, int c, unsigned t, unsigned head_dim) {
+    static __device__ __forceinline__ void load_keys(Buffer &buf, const char *base, long long row0, long long row8, int c, unsigned t, unsigned head_dim) {
         #pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const unsigned f = c * WIDTH + i * 4 * VALUES + t * VALUES;
-            buf[2 * i] = load_piece(base + row0 + f * SIZE, row0 >= 0 && f < head_dim);
-            buf[2 * i + 1] = load_piece(base + row8 + f * SIZE, row8 >= 0 && f < head_dim);
+        for (int i = 0; i < KEYS; i++) {
+            const int at = c * CHUNK + (i * 4 + (int)t) * KEY_PIECE, left = (int)head_dim * SIZE - at;
+            load_piece<WIDE, KEY_PIECE>(buf.p[2 * i], base + row0 + at, row0 >= 0, left);
+            load_piece<WIDE, KEY_PIECE>(buf.p[2 * i + 1], base + row8 + at, row8 >= 0, left);
         }
     }
-    static constexpr int VPIECES = WIDTH / (8 * VALUES);
-    static __device__ __forceinline__ void load_values(uint4 *buf, const char *base, const long long *row, int c, unsigned g, unsigned head_dim) {
+    static __device__ __forceinline__ void load_values(Buffer &buf, const char *base, const long long *row, int c, unsigned g, unsigned head_dim) {
         #pragma unroll
-        for (int i = 0; i < VPIECES; i++) {
-            const unsigned f = c * WIDTH + i * 8 * VALUES + g * VALUES;
+        for (int i = 0; i < VALUES; i++) {
+            const int at = c * CHUNK + (i * 8 + (int)g) * VALUE_PIECE, left = (int)head_dim * SIZE - at;
             #pragma unroll
-            for (int r = 0; r < 4; r++) buf[4 * i + r] = load_piece(base + row[r] + f * SIZE, row[r] >= 0 && f < head_dim);
+            for (int r = 0; r < 4; r++) load_piece<WIDE, VALUE_PIECE>(buf.p[4 * i + r], base + row[r] + at, row[r] >= 0, left);
         }
     }
-    static constexpr int TILES = HEADS / 8;
-    static __device__ __forceinline__ void multiply_keys(float (*s)[4], const uint4 *buf, const uint4 (*q)[DIM / (4 * VALUES)], int c) {
+    static constexpr int TILES = HEADS / 8, QUERY_PIECES = ROW_BYTES / (4 * KEY_PIECE);
+    static __device__ __forceinline__ void multiply_keys(float (*s)[4], const Buffer &buf, const Piece (*q)[QUERY_PIECES], int c) {
         #pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const uint4 x = buf[2 * i], y = buf[2 * i + 1];
+        for (int i = 0; i < KEYS; i++) {
+            const unsigned *x = buf.p[2 * i].w, *y = buf.p[2 * i + 1].w;
             #pragma unroll
             for (int n = 0; n < TILES; n++) {
-                const uint4 b = q[n][c * PIECES + i];
+                const unsigned *b = q[n][c * KEYS + i].w;
                 if constexpr (TYPE == ASPEN_B200_FP32) {
-                    const unsigned a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w}, b0[2] = {b.x, b.y}, b1[2] = {b.z, b.w};
-                    mma::tf32x3(s[n], a0, b0);
-                    mma::tf32x3(s[n], a1, b1);
+                    // sums of eight features are added outside: the tensor cores cut off what they add to a sum
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+                    #pragma unroll
+                    for (int k = 0; k < 8; k += 2) { const unsigned u[4] = {x[k], y[k], x[k + 1], y[k + 1]}; mma::tf32x3(part, u, b + k); }
+                    #pragma unroll
+                    for (int k = 0; k < 4; k++) s[n][k] += part[k];
                 } else {
-                    mma::Of<TYPE>::step(s[n], x.x, y.x, x.y, y.y, b.x, b.y);
-                    mma::Of<TYPE>::step(s[n], x.z, y.z, x.w, y.w, b.z, b.w);
+                    #pragma unroll
+                    for (int k = 0; k < 8; k += 2) mma::Of<TYPE>::step(s[n], x[k], y[k], x[k + 1], y[k + 1], b[k], b[k + 1]);
                 }
             }
         }
     }
-    // p: weights as the column operand, [tile][key half][2] (16-bit: one k = 16 step, [0][0], [0][1] -> b0, b1)
-    static __device__ __forceinline__ void multiply_values(Run &run, const uint4 *buf, const unsigned (*p)[4], int c) {
+    // p: weights as the column operand, 16-bit: one k = 16 step; fp32: two of k = 8
+    static __device__ __forceinline__ void multiply_values(Run &run, const Buffer &buf, const unsigned (*p)[4], int c) {
         #pragma unroll
-        for (int i = 0; i < VPIECES; i++) {
-            const uint4 &k0 = buf[4 * i], &k1 = buf[4 * i + 1], &k8 = buf[4 * i + 2], &k9 = buf[4 * i + 3];
-            const unsigned w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w}, w8[4] = {k8.x, k8.y, k8.z, k8.w}, w9[4] = {k9.x, k9.y, k9.z, k9.w};
+        for (int i = 0; i < VALUES; i++) {
+            const unsigned *w0 = buf.p[4 * i].w, *w1 = buf.p[4 * i + 1].w, *w8 = buf.p[4 * i + 2].w, *w9 = buf.p[4 * i + 3].w;
+            constexpr int WORDS = VALUE_PIECE / 4;
             if constexpr (TYPE == ASPEN_B200_FP32) {
                 #pragma unroll
-                for (int j = 0; j < 2; j++) {
+                for (int j = 0; j < WORDS / 2; j++) {
                     const unsigned lo[4] = {w0[2 * j], w0[2 * j + 1], w1[2 * j], w1[2 * j + 1]}, hi[4] = {w8[2 * j], w8[2 * j + 1], w9[2 * j], w9[2 * j + 1]};
                     #pragma unroll
                     for (int n = 0; n < TILES; n++) {
-                        float *o = run.o[n][(c * VPIECES + i) * 2 + j];
-                        mma::tf32x3(o, lo, p[n]);
-                        mma::tf32x3(o, hi, p[n] + 2);
+                        float part[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma::tf32x3(part, lo, p[n]);
+                        mma::tf32x3(part, hi, p[n] + 2);
+                        #pragma unroll
+                        for (int k = 0; k < 4; k++) run.o[n][(c * VALUES + i) * (WORDS / 2) + j][k] += part[k];
                     }
                 }
             } else {
                 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                for (int j = 0; j < WORDS; j++) {
                     const unsigned a0 = mma::pair_of(w0[j], w1[j], false), a1 = mma::pair_of(w0[j], w1[j], true);
                     const unsigned a2 = mma::pair_of(w8[j], w9[j], false), a3 = mma::pair_of(w8[j], w9[j], true);
                     #pragma unroll
-                    for (int n = 0; n < TILES; n++) mma::Of<TYPE>::step(run.o[n][(c * VPIECES + i) * 4 + j], a0, a1, a2, a3, p[n][0], p[n][1]);
+                    for (int n = 0; n < TILES; n++) mma::Of<TYPE>::step(run.o[n][(c * VALUES + i) * WORDS + j], a0, a1, a2, a3, p[n][0], p[n][1]);
                 }
             }
         }
@@ -256,22 +288,22 @@ struct Kernel {
     // All steps of a share, in one warp.
     static __device__ __forceinline__ void walk(const Args &a, const Share &s, Run &run) {
         const unsigned lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
-        uint4 q[TILES][DIM / (4 * VALUES)];
+        Piece q[TILES][QUERY_PIECES];
         #pragma unroll
         for (int n = 0; n < TILES; n++) {
             const unsigned in_group = s.chunk * HEADS + n * 8 + g;
             const char *row = a.q + ((size_t)s.entry * a.q_row + (size_t)(s.kv_head * a.group + in_group) * a.q_head) * SIZE;
             #pragma unroll
-            for (int i = 0; i < DIM / (4 * VALUES); i++) {
-                const unsigned f = i * 4 * VALUES + t * VALUES;
-                q[n][i] = load_piece(row + f * SIZE, in_group < a.group && f < a.head_dim);
+            for (int i = 0; i < QUERY_PIECES; i++) {
+                const int at = (i * 4 + (int)t) * KEY_PIECE;
+                load_piece<false, KEY_PIECE>(q[n][i], row + at, in_group < a.group, (int)a.head_dim * SIZE - at);
             }
         }
         run.clear();
         // rows of two steps: lanes 0 ... 15 the first one's keys, 16 ... 31 the second one's
         unsigned step = s.begin;
         long long rows = row_of(a, s, step * STEP, lane);
-        uint4 buf[2][8];
+        Buffer buf[2];
         // buffers in turn: all chunks of a step's keys, then all of its values; each is filled again as soon as it has been multiplied
         long long key0 = from_lane(rows, g), key8 = from_lane(rows, g + 8), value[4];
         bool second = false;
@@ -343,71 +375,56 @@ struct Kernel {
                 const float inv = run.sum[n][j] == 0.f ? 0.f : 1.f / run.sum[n][j];
                 if (in_group >= a.group) continue;
                 char *row = out_of(a, s.entry, s.kv_head, in_group);
+                constexpr int PER = 16 / SIZE;
                 #pragma unroll
-                for (int i = 0; i < Run::PIECES; i++) {
-                    const unsigned f = Run::feature(i, g);
-                    float v[Run::PIECE];
+                for (int i = 0; i < Run::PIECES; i++)
                     #pragma unroll
-                    for (int x = 0; x < Run::PIECE; x++) v[x] = run.value(n, i, x, j) * inv;
-                    if (f < a.head_dim) store_piece<TYPE>(row + f * SIZE, v);
-                }
+                    for (int h = 0; h < Run::PIECE; h += PER) {
+                        const unsigned f = Run::feature(i, g) + h;
+                        float v[PER];
+                        #pragma unroll
+                        for (int x = 0; x < PER; x++) v[x] = run.value(n, i, h + x, j) * inv;
+                        if (f < a.head_dim) store_piece<TYPE>(row + f * SIZE, v);
+                    }
             }
     }
     // A shared item's part to the warp's place in shared memory.
-    static __device__ __forceinline__ void keep(float *at, const Run &run) {
+    static __device__ __forceinline__ void keep(float *at, const Run &run, unsigned heads) {
         const unsigned g = threadIdx.x % 32 >> 2, t = threadIdx.x & 3;
         #pragma unroll
         for (int n = 0; n < TILES; n++)
             #pragma unroll
             for (int j = 0; j < 2; j++) {
+                if (n * 8 + 2 * t + j >= heads) continue;
                 float *row = at + (n * 8 + 2 * t + j) * ROW;
                 #pragma unroll
                 for (int i = 0; i < Run::PIECES; i++)
                     #pragma unroll
-                    for (int x = 0; x < Run::PIECE; x += 2)
-                        *reinterpret_cast<float2 *>(row + Run::feature(i, g) + x) = make_float2(run.value(n, i, x, j), run.value(n, i, x + 1, j));
+                    for (int x = 0; x < Run::PIECE; x += 4)
+                        *reinterpret_cast<float4 *>(row + Run::feature(i, g) + x) = make_float4(run.value(n, i, x, j), run.value(n, i, x + 1, j), run.value(n, i, x + 2, j), run.value(n, i, x + 3, j));
                 if (g == 0) *reinterpret_cast<float2 *>(row + DIM) = make_float2(run.max[n][j], run.sum[n][j]);
             }
     }
 };
 
-// Value f of head r from `count` partial results, `stride` floats apart, joined in order; the maximum and the sum too.
-template <int ROW, int DIM>
-__device__ __forceinline__ float join(const float *first, size_t stride, unsigned count, int r, int f, float &max, float &sum) {
-    first += r * ROW;
-    max = -INFINITY;
-    for (unsigned i = 0; i < count; i++) max = fmaxf(max, first[i * stride + DIM]);
-    const float ref = max == -INFINITY ? 0.f : max;
-    float v = 0.f;
-    sum = 0.f;
-    #pragma unroll 4
-    for (unsigned i = 0; i < count; i++) {
-        const float *p = first + i * stride;
-        const float w = mma::exp2_fast(p[DIM] - ref);
-        sum = fmaf(w, p[DIM + 1], sum);
-        v = fmaf(w, p[f], v);
-    }
-    return v;
-}
-
-template <int TYPE, int DIM, int HEADS, int CTAS>
-__global__ void __launch_bounds__(256, CTAS) decode_kernel(const Args a) {
-    typedef Kernel<TYPE, DIM, HEADS> K;
+template <int TYPE, int DIM, int HEADS, bool WIDE>
+__global__ void __launch_bounds__(threads_of(TYPE, DIM, HEADS), ctas_of(TYPE, DIM)) decode_kernel(const Args a) {
+    typedef Kernel<TYPE, DIM, HEADS, WIDE> K;
     typedef typename K::Run Run;
-    extern __shared__ float kept[];             // [warp][2][HEADS][ROW]
-    __shared__ Line line;
+    extern __shared__ __align__(16) float kept[];             // [warp][2][HEADS][ROW]
+    __shared__ Line<K::THREADS> line;
     __shared__ int item_of[K::WARPS * 2], whole_of[K::WARPS * 2];      // of the kept parts: the item (-1: none); bit 0: has its begin, bit 1: its end
     const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const unsigned each = (a.entries + 255) / 256, items = a.kv_heads * a.chunks;
-    measure<256>(a, each, line);
-    const unsigned long long all = line.before[256];
+    const unsigned each = (a.entries + K::THREADS - 1) / K::THREADS, items = a.kv_heads * a.chunks;
+    measure<K::THREADS>(a, each, line);
+    const unsigned long long all = line.before[K::THREADS];
     if (threadIdx.x < K::WARPS * 2) item_of[threadIdx.x] = -1;
     // sequences without tokens
     for (unsigned e = blockIdx.x; e < a.entries; e += gridDim.x) {
         const int slot = slot_of(a, e);
         if (attn::sequence_length(a.at, slot) != 0) continue;
-        for (unsigned i = threadIdx.x; i < a.kv_heads * a.group * a.head_dim; i += 256)
+        for (unsigned i = threadIdx.x; i < a.kv_heads * a.group * a.head_dim; i += K::THREADS)
             store_value<TYPE>(a.out + ((size_t)e * a.out_row + (size_t)(i / a.head_dim) * a.out_head + i % a.head_dim) * K::SIZE, 0.f);
         if (threadIdx.x == 0 && (slot < 0 || (unsigned)slot >= a.at.sequences)) atomicOr(a.at.status, ASPEN_B200_CACHE_BAD_INDEX);
     }
@@ -420,7 +437,7 @@ __global__ void __launch_bounds__(256, CTAS) decode_kernel(const Args a) {
         unsigned long long pos = cta0 + attn::first_step(steps, warp, K::WARPS);
         const unsigned long long end = cta0 + attn::first_step(steps, warp + 1, K::WARPS);
         if (pos < end) {
-            unsigned lo = 0, hi = 256;          // the last thread whose entries begin at pos or before
+            unsigned lo = 0, hi = K::THREADS;   // the last thread whose entries begin at pos or before
             while (hi - lo > 1) { const unsigned mid = (lo + hi) / 2; if (line.before[mid] <= pos) lo = mid; else hi = mid; }
             unsigned e = lo * each;
             unsigned long long base = line.before[lo];
@@ -449,7 +466,7 @@ __global__ void __launch_bounds__(256, CTAS) decode_kernel(const Args a) {
                 else {
                     // the one that began before this warp's share, or the one that goes on behind it
                     const unsigned place = warp * 2 + (s.begin != 0 ? 0 : 1);
-                    K::keep(kept + (size_t)place * HEADS * K::ROW, run);
+                    K::keep(kept + (size_t)place * HEADS * K::ROW, run, min((unsigned)HEADS, a.group - s.chunk * HEADS));
                     if (lane == 0) { item_of[place] = (int)(e * items + item); whole_of[place] = (s.begin == 0 ? 1 : 0) | (s.end == n ? 2 : 0); }
                 }
                 pos += s.end - s.begin;
@@ -470,7 +487,7 @@ __global__ void __launch_bounds__(256, CTAS) decode_kernel(const Args a) {
         const bool begins = whole_of[i] & 1, ends = whole_of[last] & 2;
         const unsigned e = (unsigned)item / items, rest = (unsigned)item % items, kv_head = rest / a.chunks, chunk = rest % a.chunks;
         float *const part = a.part + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * HEADS * K::ROW;
-        for (unsigned x = threadIdx.x; x < HEADS * DIM; x += 256) {
+        for (unsigned x = threadIdx.x; x < min((unsigned)HEADS, a.group - chunk * HEADS) * DIM; x += K::THREADS) {
             const unsigned r = x / DIM, f = x % DIM;
             float max = -INFINITY, sum = 0.f, v = 0.f;
             for (unsigned j = 0; j < count; j++) max = fmaxf(max, kept[(places[j] * HEADS + r) * K::ROW + DIM]);
@@ -502,52 +519,72 @@ __global__ void __launch_bounds__(256, CTAS) decode_kernel(const Args a) {
     }
 }
 
-// Items that several CTAs had a part of: CTA b joins the one that began in CTA b and went on.
+// Items that several CTAs had a part of: block (b, r) joins head r of the one that began in CTA b and went on.
 template <int TYPE, int DIM, int HEADS>
-__global__ void __launch_bounds__(JOINERS) join_kernel(const Args a) {
-    typedef Kernel<TYPE, DIM, HEADS> K;
+__global__ void __launch_bounds__(DIM) join_kernel(const Args a) {
+    typedef Kernel<TYPE, DIM, HEADS, true> K;
+    constexpr unsigned AT_ONCE = DIM;
+    __shared__ float weight[AT_ONCE], maxima[DIM / 32], sums[DIM / 32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int item = a.record[2 * blockIdx.x];
     if (item < 0) return;
-    const unsigned count = (unsigned)a.record[2 * blockIdx.x + 1] - blockIdx.x, items = a.kv_heads * a.chunks;    // CTAs behind this one
-    const unsigned e = (unsigned)item / items, rest = (unsigned)item % items, kv_head = rest / a.chunks, chunk = rest % a.chunks;
+    const unsigned parts = (unsigned)a.record[2 * blockIdx.x + 1] - blockIdx.x + 1, items = a.kv_heads * a.chunks;      // of the CTAs from this one on
+    const unsigned e = (unsigned)item / items, rest = (unsigned)item % items, kv_head = rest / a.chunks, chunk = rest % a.chunks, f = threadIdx.x;
+    const unsigned in_group = chunk * HEADS + blockIdx.y;
+    if (in_group >= a.group) return;
     constexpr size_t SLOT = (size_t)HEADS * K::ROW;
-    const float *const mine = a.part + ((size_t)blockIdx.x * 2 + 1) * SLOT;
-    for (unsigned x = threadIdx.x; x < HEADS * DIM; x += JOINERS) {
-        const unsigned r = x / DIM, f = x % DIM, in_group = chunk * HEADS + r;
-        if (in_group >= a.group || f >= a.head_dim) continue;
-        float m, s;
-        // the others' parts that began before their CTA: every second place from here on
-        const float v = join<K::ROW, DIM>(mine + SLOT, 2 * SLOT, count, r, f, m, s);
-        const float *p = mine + r * K::ROW;
-        const float max = fmaxf(m, p[DIM]), ref = max == -INFINITY ? 0.f : max;
-        const float w0 = mma::exp2_fast(p[DIM] - ref), w1 = mma::exp2_fast(m - ref);
-        const float sum = fmaf(w0, p[DIM + 1], w1 * s), value = fmaf(w0, p[f], w1 * v);
-        store_value<TYPE>(K::out_of(a, e, kv_head, in_group) + f * K::SIZE, sum == 0.f ? 0.f : value / sum);
+    // this CTA's second place, then the first places of the CTAs behind it
+    const float *const first = a.part + ((size_t)blockIdx.x * 2 + 1) * SLOT + blockIdx.y * K::ROW;
+    auto at = [&](unsigned i) { return first + (i ? (2 * (size_t)i - 1) * SLOT : 0); };
+    float max = -INFINITY;
+    for (unsigned i = f; i < parts; i += DIM) max = fmaxf(max, at(i)[DIM]);
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) max = fmaxf(max, __shfl_xor_sync(0xffffffffu, max, o));
+    if (f % 32 == 0) maxima[f / 32] = max;
+    __syncthreads();
+    #pragma unroll
+    for (int i = 0; i < DIM / 32; i++) max = fmaxf(max, maxima[i]);
+    const float ref = max == -INFINITY ? 0.f : max;
+    float v = 0.f, sum = 0.f;
+    for (unsigned i0 = 0; i0 < parts; i0 += AT_ONCE) {
+        __syncthreads();
+        if (i0 + f < parts) {
+            const float *const p = at(i0 + f);
+            const float w = mma::exp2_fast(p[DIM] - ref);
+            weight[f] = w;
+            sum = fmaf(w, p[DIM + 1], sum);
+        }
+        __syncthreads();
+        const unsigned n = min(AT_ONCE, parts - i0);
+        #pragma unroll 8
+        for (unsigned i = 0; i < n; i++) v = fmaf(weight[i], at(i0 + i)[f], v);
     }
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (f % 32 == 0) sums[f / 32] = sum;
+    __syncthreads();
+    sum = 0.f;
+    #pragma unroll
+    for (int i = 0; i < DIM / 32; i++) sum += sums[i];
+    if (f < a.head_dim) store_value<TYPE>(K::out_of(a, e, kv_head, in_group) + f * K::SIZE, sum == 0.f ? 0.f : v / sum);
 }
-
-// Heads of a group that one pass over the keys serves: eight columns of a product, or sixteen (features permitting: the sums of 256 take the registers).
-unsigned heads_of_pass(unsigned group, unsigned dim) { return group <= 8 || dim == 256 ? 8 : 16; }
-unsigned dim_of(unsigned head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
-// CTAs on an SM: registers for that many (three for heads of up to 128 features and 8 heads).
-unsigned ctas_of(unsigned heads, unsigned dim, int type) { return dim == 256 || (heads == 16 && dim == 128) ? 1 : type == ASPEN_B200_FP32 && dim == 128 ? 1 : 2; }
 
 size_t workspace_bytes(unsigned sms, unsigned heads, unsigned dim, int type) {
-    const size_t ctas = (size_t)sms * ctas_of(heads, dim, type);
-    return ctas * 16 + ctas * 2 * heads * (dim + 2) * 4;
+    const size_t ctas = (size_t)sms * ctas_of(type, dim);
+    return ctas * 16 + ctas * 2 * heads * (dim + 4) * 4;
 }
 
-template <int TYPE, int DIM, int HEADS, int CTAS>
+template <int TYPE, int DIM, int HEADS, bool WIDE>
 cudaError_t launch(const Args &a, unsigned sms, cudaStream_t stream) {
-    typedef Kernel<TYPE, DIM, HEADS> K;
-    cudaError_t err = cudaFuncSetAttribute(decode_kernel<TYPE, DIM, HEADS, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, K::SMEM);
+    typedef Kernel<TYPE, DIM, HEADS, WIDE> K;
+    constexpr unsigned CTAS = ctas_of(TYPE, DIM);
+    cudaError_t err = cudaFuncSetAttribute(decode_kernel<TYPE, DIM, HEADS, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, K::SMEM);
     if (err != cudaSuccess) return err;
-    decode_kernel<TYPE, DIM, HEADS, CTAS><<<sms * CTAS, 256, K::SMEM, stream>>>(a);
+    decode_kernel<TYPE, DIM, HEADS, WIDE><<<sms * CTAS, K::THREADS, K::SMEM, stream>>>(a);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms * CTAS);
-    cfg.blockDim = dim3(JOINERS);
+    cfg.gridDim = dim3(sms * CTAS, a.group < HEADS ? a.group : HEADS);
+    cfg.blockDim = dim3(DIM);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -556,12 +593,16 @@ cudaError_t launch(const Args &a, unsigned sms, cudaStream_t stream) {
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, join_kernel<TYPE, DIM, HEADS>, a);
 }
-template <int TYPE>
+template <int TYPE, bool WIDE>
 cudaError_t launch(const Args &a, unsigned heads, unsigned dim, unsigned sms, cudaStream_t stream) {
-    constexpr int WIDE = TYPE == ASPEN_B200_FP32 ? 1 : 2;
-    if (dim == 64) return heads == 8 ? launch<TYPE, 64, 8, 2>(a, sms, stream) : launch<TYPE, 64, 16, 2>(a, sms, stream);
-    if (dim == 128) return heads == 8 ? launch<TYPE, 128, 8, WIDE>(a, sms, stream) : launch<TYPE, 128, 16, 1>(a, sms, stream);
-    return launch<TYPE, 256, 8, 1>(a, sms, stream);
+    if (dim == 64) return heads == 8 ? launch<TYPE, 64, 8, WIDE>(a, sms, stream) : launch<TYPE, 64, 16, WIDE>(a, sms, stream);
+    if (dim == 256) return launch<TYPE, 256, 8, WIDE>(a, sms, stream);
+    if constexpr (TYPE != ASPEN_B200_FP32) if (heads == 16) return launch<TYPE, 128, 16, WIDE>(a, sms, stream);
+    return launch<TYPE, 128, 8, WIDE>(a, sms, stream);
+}
+template <int TYPE>
+cudaError_t launch(const Args &a, bool wide, unsigned heads, unsigned dim, unsigned sms, cudaStream_t stream) {
+    return wide ? launch<TYPE, true>(a, heads, dim, sms, stream) : launch<TYPE, false>(a, heads, dim, sms, stream);
 }
 
 int check_heads(const aspen_b200_cache_t *cache, unsigned entries, unsigned heads, const char *what) {
@@ -580,7 +621,7 @@ extern "C" size_t aspen_b200_attention_decode_workspace(const aspen_b200_cache_t
     const int sms = attn::sm_count(what);
     if (sms < 0) return 0;
     const unsigned dim = dim_of(cache->head_dim);
-    return workspace_bytes((unsigned)sms, heads_of_pass(heads / cache->kv_heads, dim), dim, cache->type);
+    return workspace_bytes((unsigned)sms, heads_of_pass(heads / cache->kv_heads, dim, cache->type), dim, cache->type);
 }
 
 extern "C" int aspen_b200_attention_decode(const aspen_b200_cache_t *cache, unsigned int layer, const aspen_b200_decode_t *d, void *cuda_stream) {
@@ -597,7 +638,7 @@ extern "C" int aspen_b200_attention_decode(const aspen_b200_cache_t *cache, unsi
     if (!d->workspace || reinterpret_cast<uintptr_t>(d->workspace) % 16) { ASPEN_ERR("%s: no workspace, or not on a 16-byte boundary\n", what); return -1; }
     const int sms = attn::sm_count(what);
     if (sms < 0) return sms;
-    const unsigned group = d->heads / cache->kv_heads, dim = dim_of(cache->head_dim), heads = heads_of_pass(group, dim);
+    const unsigned group = d->heads / cache->kv_heads, dim = dim_of(cache->head_dim), heads = heads_of_pass(group, dim, cache->type);
     const size_t need = workspace_bytes((unsigned)sms, heads, dim, cache->type);
     if (d->workspace_bytes < need) { ASPEN_ERR("%s: a workspace of %zu bytes; %zu are needed\n", what, d->workspace_bytes, need); return -1; }
     const attn::Named all[] = {{cache->k, "the cache's k"}, {cache->v, "the cache's v"}, {cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->status, "status"},
@@ -621,15 +662,18 @@ extern "C" int aspen_b200_attention_decode(const aspen_b200_cache_t *cache, unsi
     a.chunks = (group + heads - 1) / heads;
     a.head_dim = cache->head_dim;
     a.scale = d->scale * 1.4426950408889634f;
-    const size_t ctas = (size_t)sms * ctas_of(heads, dim, cache->type);
+    const size_t ctas = (size_t)sms * ctas_of(cache->type, dim);
     a.record = static_cast<int *>(d->workspace);
     a.part = reinterpret_cast<float *>(static_cast<char *>(d->workspace) + ctas * 16);
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    // rows of keys and values on 32-byte boundaries, and whole pieces of 32 bytes in them: one load a piece instead of two
+    const size_t starts = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | (a.at.page_stride | a.at.head_stride | a.at.token_stride | cache->head_dim) * size;
+    const bool wide = starts % 32 == 0;
     cudaError_t err;
     switch (cache->type) {
-        case ASPEN_B200_FP32: err = launch<ASPEN_B200_FP32>(a, heads, dim, (unsigned)sms, stream); break;
-        case ASPEN_B200_BF16: err = launch<ASPEN_B200_BF16>(a, heads, dim, (unsigned)sms, stream); break;
-        default: err = launch<ASPEN_B200_FP16>(a, heads, dim, (unsigned)sms, stream); break;
+        case ASPEN_B200_FP32: err = launch<ASPEN_B200_FP32>(a, wide, heads, dim, (unsigned)sms, stream); break;
+        case ASPEN_B200_BF16: err = launch<ASPEN_B200_BF16>(a, wide, heads, dim, (unsigned)sms, stream); break;
+        default: err = launch<ASPEN_B200_FP16>(a, wide, heads, dim, (unsigned)sms, stream); break;
     }
     if (err != cudaSuccess) { cudaGetLastError(); ASPEN_ERR("%s: %s\n", what, cudaGetErrorString(err)); return -3; }
     return 0;
