@@ -40,23 +40,51 @@ struct Args {
     float *part;                                // [CTAs][2][HEADS][DIM + 4]: what began before the CTA, and what goes on behind it
 };
 
+__device__ __forceinline__ unsigned steps_of(unsigned tokens) { return (tokens + STEP - 1) / STEP; }
+__device__ __forceinline__ int slot_of(const Args &a, unsigned e) { return a.slots ? a.slots[e] : (int)e; }
+
+template <int TYPE>
+__device__ __forceinline__ void store_value(char *at, float v) {
+    if (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float *>(at) = v;
+    else if (TYPE == ASPEN_B200_BF16) *reinterpret_cast<__nv_bfloat16 *>(at) = __float2bfloat16_rn(v);
+    else *reinterpret_cast<__half *>(at) = __float2half_rn(v);
+}
+
 // Steps of all items, and where each thread's entries begin in the line.
 template <int THREADS>
 struct Line {
     unsigned long long before[THREADS + 1];     // [i]: steps of the entries before thread i's; [THREADS]: all
     unsigned long long sums[THREADS / 32];
+    unsigned tokens[THREADS];                   // of each thread's only entry, where there are no more entries than threads
+    int slot[THREADS];
+    __device__ __forceinline__ void entry(const Args &a, unsigned each, unsigned e, int &s, unsigned &n) const {
+        if (each == 1) { s = slot[e]; n = tokens[e]; return; }
+        s = slot_of(a, e);
+        n = attn::sequence_length(a.at, s);
+    }
 };
 
-__device__ __forceinline__ unsigned steps_of(unsigned tokens) { return (tokens + STEP - 1) / STEP; }
-__device__ __forceinline__ int slot_of(const Args &a, unsigned e) { return a.slots ? a.slots[e] : (int)e; }
-
-template <int THREADS>
+// Also the outputs of sequences without tokens: entry e in CTA e.
+template <int TYPE, int THREADS>
 __device__ void measure(const Args &a, unsigned each, Line<THREADS> &line) {
+    constexpr int SIZE = TYPE == ASPEN_B200_FP32 ? 4 : 2;
     const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     unsigned long long mine = 0;
     for (unsigned i = 0; i < each; i++) {
         const unsigned e = threadIdx.x * each + i;
-        if (e < a.entries) mine += steps_of(attn::sequence_length(a.at, slot_of(a, e)));
+        bool empty = false;
+        if (e < a.entries) {
+            const int slot = slot_of(a, e);
+            const unsigned tokens = attn::sequence_length(a.at, slot);
+            mine += steps_of(tokens);
+            empty = tokens == 0 && e % gridDim.x == blockIdx.x;
+            if (each == 1) { line.tokens[threadIdx.x] = tokens; line.slot[threadIdx.x] = slot; }
+            if (empty && (slot < 0 || (unsigned)slot >= a.at.sequences)) atomicOr(a.at.status, ASPEN_B200_CACHE_BAD_INDEX);
+        }
+        for (unsigned left = __ballot_sync(0xffffffffu, empty); left; left &= left - 1) {
+            const size_t row = (size_t)((warp * 32 + __ffs(left) - 1) * each + i) * a.out_row;
+            for (unsigned x = lane; x < a.kv_heads * a.group * a.head_dim; x += 32) store_value<TYPE>(a.out + (row + (size_t)(x / a.head_dim) * a.out_head + x % a.head_dim) * SIZE, 0.f);
+        }
     }
     mine *= a.kv_heads * a.chunks;
     unsigned long long s = mine;
@@ -65,7 +93,8 @@ __device__ void measure(const Args &a, unsigned each, Line<THREADS> &line) {
     if (lane == 31) line.sums[warp] = s;
     __syncthreads();
     unsigned long long base = 0;
-    for (unsigned w = 0; w < warp; w++) base += line.sums[w];
+    #pragma unroll
+    for (unsigned w = 0; w < THREADS / 32; w++) base += w < warp ? line.sums[w] : 0ull;
     line.before[threadIdx.x] = base + s - mine;
     if (threadIdx.x == THREADS - 1) line.before[THREADS] = base + s;
     __syncthreads();
@@ -110,13 +139,6 @@ __device__ __forceinline__ void store_piece(char *at, const float *v) {
         *reinterpret_cast<uint4 *>(at) = make_uint4(T::pack(v[0], v[1]), T::pack(v[2], v[3]), T::pack(v[4], v[5]), T::pack(v[6], v[7]));
     }
 }
-template <int TYPE>
-__device__ __forceinline__ void store_value(char *at, float v) {
-    if (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float *>(at) = v;
-    else if (TYPE == ASPEN_B200_BF16) *reinterpret_cast<__nv_bfloat16 *>(at) = __float2bfloat16_rn(v);
-    else *reinterpret_cast<__half *>(at) = __float2half_rn(v);
-}
-
 __device__ __forceinline__ uint4 load16(const char *p, bool ok) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (ok) asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -411,111 +433,127 @@ template <int TYPE, int DIM, int HEADS, bool WIDE>
 __global__ void __launch_bounds__(threads_of(TYPE, DIM, HEADS), ctas_of(TYPE, DIM)) decode_kernel(const Args a) {
     typedef Kernel<TYPE, DIM, HEADS, WIDE> K;
     typedef typename K::Run Run;
-    extern __shared__ __align__(16) float kept[];             // [warp][2][HEADS][ROW]
+    extern __shared__ __align__(16) float kept[];             // [place][HEADS][ROW]; places: two of each warp, an item that began before its share and one that goes on behind it
+    constexpr unsigned PLACES = K::WARPS * 2;
+    static_assert(PLACES <= 32, "a lane a place");
     __shared__ Line<K::THREADS> line;
-    __shared__ int item_of[K::WARPS * 2], whole_of[K::WARPS * 2];      // of the kept parts: the item (-1: none); bit 0: has its begin, bit 1: its end
+    __shared__ int item_of[PLACES], whole_of[PLACES];         // the item (-1: none); bit 0: the place has its first step, bit 1: its last
+    __shared__ unsigned long long last_of[PLACES];            // the item's last step, in the line
+    __shared__ unsigned same_as[PLACES];                      // the places of the same item, a bit each
+    __shared__ float weight[PLACES][HEADS], total[PLACES][HEADS];
     const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const unsigned each = (a.entries + K::THREADS - 1) / K::THREADS, items = a.kv_heads * a.chunks;
-    measure<K::THREADS>(a, each, line);
+    if (threadIdx.x < PLACES) item_of[threadIdx.x] = -1;
+    if (threadIdx.x == 0) a.record[2 * blockIdx.x] = -1;
+    measure<TYPE, K::THREADS>(a, each, line);
     const unsigned long long all = line.before[K::THREADS];
-    if (threadIdx.x < K::WARPS * 2) item_of[threadIdx.x] = -1;
-    // sequences without tokens
-    for (unsigned e = blockIdx.x; e < a.entries; e += gridDim.x) {
-        const int slot = slot_of(a, e);
-        if (attn::sequence_length(a.at, slot) != 0) continue;
-        for (unsigned i = threadIdx.x; i < a.kv_heads * a.group * a.head_dim; i += K::THREADS)
-            store_value<TYPE>(a.out + ((size_t)e * a.out_row + (size_t)(i / a.head_dim) * a.out_head + i % a.head_dim) * K::SIZE, 0.f);
-        if (threadIdx.x == 0 && (slot < 0 || (unsigned)slot >= a.at.sequences)) atomicOr(a.at.status, ASPEN_B200_CACHE_BAD_INDEX);
-    }
-    __syncthreads();
     // CTAs that get a share: a step for each of their warps at least, so that little is joined where little is to do
     const unsigned ctas = (unsigned)min((unsigned long long)gridDim.x, (all + K::WARPS - 1) / K::WARPS);
-    if (blockIdx.x < ctas) {
-        const unsigned long long cta0 = attn::first_step(all, blockIdx.x, ctas), cta1 = attn::first_step(all, blockIdx.x + 1, ctas);
-        const unsigned long long steps = cta1 - cta0;
-        unsigned long long pos = cta0 + attn::first_step(steps, warp, K::WARPS);
-        const unsigned long long end = cta0 + attn::first_step(steps, warp + 1, K::WARPS);
-        if (pos < end) {
-            unsigned lo = 0, hi = K::THREADS;   // the last thread whose entries begin at pos or before
-            while (hi - lo > 1) { const unsigned mid = (lo + hi) / 2; if (line.before[mid] <= pos) lo = mid; else hi = mid; }
-            unsigned e = lo * each;
-            unsigned long long base = line.before[lo];
-            while (pos < end) {
-                Share s;
-                unsigned n;
-                // bounded by the number of entries: `end` does not lie behind the last one's steps
-                for (;; e++) {
-                    s.slot = slot_of(a, e);
-                    s.tokens = attn::sequence_length(a.at, s.slot);
-                    n = steps_of(s.tokens);
-                    if (base + (unsigned long long)n * items > pos || e + 1 >= a.entries) break;
-                    base += (unsigned long long)n * items;
+    if (blockIdx.x >= ctas) return;
+    const unsigned long long cta0 = attn::first_step(all, blockIdx.x, ctas), cta1 = attn::first_step(all, blockIdx.x + 1, ctas);
+    const unsigned long long steps = cta1 - cta0;
+    unsigned long long pos = cta0 + attn::first_step(steps, warp, K::WARPS);
+    const unsigned long long end = cta0 + attn::first_step(steps, warp + 1, K::WARPS);
+    if (pos < end) {
+        unsigned lo = 0, hi = K::THREADS;       // the last thread whose entries begin at pos or before
+        while (hi - lo > 1) { const unsigned mid = (lo + hi) / 2; if (line.before[mid] <= pos) lo = mid; else hi = mid; }
+        unsigned e = lo * each;
+        unsigned long long base = line.before[lo];
+        while (pos < end) {
+            Share s;
+            unsigned n;
+            // bounded by the number of entries: `end` does not lie behind the last one's steps
+            for (;; e++) {
+                line.entry(a, each, e, s.slot, s.tokens);
+                n = steps_of(s.tokens);
+                if (base + (unsigned long long)n * items > pos || e + 1 >= a.entries) break;
+                base += (unsigned long long)n * items;
+            }
+            const unsigned long long rel = pos - base;
+            if (rel >= (unsigned long long)n * items) break;           // lengths that changed under the call
+            const unsigned item = rel >> 32 ? (unsigned)(rel / n) : (unsigned)rel / n;
+            s.entry = e;
+            s.kv_head = item / a.chunks;
+            s.chunk = item - s.kv_head * a.chunks;
+            s.begin = (unsigned)(rel - (unsigned long long)item * n);
+            s.end = (unsigned)min((unsigned long long)n, s.begin + (end - pos));
+            Run run;
+            K::walk(a, s, run);
+            if (s.begin == 0 && s.end == n) K::finish(a, s, run);
+            else {
+                const unsigned place = warp * 2 + (s.begin != 0 ? 0 : 1);
+                K::keep(kept + (size_t)place * HEADS * K::ROW, run, min((unsigned)HEADS, a.group - s.chunk * HEADS));
+                if (lane == 0) {
+                    item_of[place] = (int)(e * items + item);
+                    whole_of[place] = (s.begin == 0 ? 1 : 0) | (s.end == n ? 2 : 0);
+                    last_of[place] = base + (unsigned long long)(item + 1) * n - 1;
                 }
-                const unsigned long long rel = pos - base;
-                if (rel >= (unsigned long long)n * items) break;           // lengths that changed under the call
-                const unsigned item = (unsigned)(rel / n);
-                s.entry = e;
-                s.kv_head = item / a.chunks;
-                s.chunk = item - s.kv_head * a.chunks;
-                s.begin = (unsigned)(rel - (unsigned long long)item * n);
-                s.end = (unsigned)min((unsigned long long)n, s.begin + (end - pos));
-                Run run;
-                K::walk(a, s, run);
-                if (s.begin == 0 && s.end == n) K::finish(a, s, run);
-                else {
-                    // the one that began before this warp's share, or the one that goes on behind it
-                    const unsigned place = warp * 2 + (s.begin != 0 ? 0 : 1);
-                    K::keep(kept + (size_t)place * HEADS * K::ROW, run, min((unsigned)HEADS, a.group - s.chunk * HEADS));
-                    if (lane == 0) { item_of[place] = (int)(e * items + item); whole_of[place] = (s.begin == 0 ? 1 : 0) | (s.end == n ? 2 : 0); }
-                }
-                pos += s.end - s.begin;
+            }
+            pos += s.end - s.begin;
+        }
+    }
+    __syncthreads();
+    // Items that warps share: which places each has, ...
+    if (warp == 0) {
+        const int item = lane < PLACES ? item_of[lane] : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, item), first = __ffs(same) - 1, last = 31 - __clz(same);
+        const int begins = __shfl_sync(0xffffffffu, lane < PLACES ? whole_of[lane] : 0, first) & 1, ends = __shfl_sync(0xffffffffu, lane < PLACES ? whole_of[lane] : 0, last) & 2;
+        if (lane < PLACES) {
+            // one that has all of it is done here; of one that goes on behind the CTA the joining kernel has to know
+            same_as[lane] = item >= 0 && lane == first ? same : 0u;
+            if (item >= 0 && lane == first) {
+                whole_of[lane] = begins | ends;
+                if (begins && !ends) { a.record[2 * blockIdx.x + 1] = (int)attn::part_of_step(all, last_of[lane], ctas); a.record[2 * blockIdx.x] = item; }
             }
         }
     }
     __syncthreads();
-    // Parts of one item stand next to each other; those of all warps, in order.
-    if (threadIdx.x == 0) a.record[2 * blockIdx.x] = -1;
+    // ... what each part counts, ...
+    for (unsigned x = threadIdx.x; x < PLACES * HEADS; x += K::THREADS) {
+        const unsigned first = x / HEADS, r = x % HEADS;
+        float max = -INFINITY, sum = 0.f;
+        for (unsigned left = same_as[first]; left; left &= left - 1) max = fmaxf(max, kept[((__ffs(left) - 1) * HEADS + r) * K::ROW + DIM]);
+        const float ref = max == -INFINITY ? 0.f : max;
+        for (unsigned left = same_as[first]; left; left &= left - 1) {
+            const unsigned j = __ffs(left) - 1;
+            const float *p = kept + (j * HEADS + r) * K::ROW + DIM;
+            const float w = mma::exp2_fast(p[0] - ref);
+            weight[j][r] = w;
+            sum = fmaf(w, p[1], sum);
+        }
+        total[first][r] = sum;
+        if (same_as[first]) kept[(first * HEADS + r) * K::ROW + DIM + 2] = max;
+    }
     __syncthreads();
-    for (unsigned i = 0; i < K::WARPS * 2;) {
-        const int item = item_of[i];
-        if (item < 0) { i++; continue; }
-        // the parts behind this one that are of the same item (places that are empty lie between them: a warp's second place when its first one goes on)
-        unsigned places[K::WARPS * 2], count = 0, last = i;
-        for (unsigned j = i; j < K::WARPS * 2; j++)
-            if (item_of[j] == item) { places[count++] = j; last = j; }
-        const bool begins = whole_of[i] & 1, ends = whole_of[last] & 2;
-        const unsigned e = (unsigned)item / items, rest = (unsigned)item % items, kv_head = rest / a.chunks, chunk = rest % a.chunks;
+    // ... and their sum: four values a thread.
+    for (unsigned first = 0; first < PLACES; first++) {
+        const unsigned same = same_as[first];
+        if (!same) continue;
+        const bool begins = whole_of[first] & 1, ends = whole_of[first] & 2;
+        const unsigned item = (unsigned)item_of[first], e = item / items, rest = item - e * items, kv_head = rest / a.chunks, chunk = rest - kv_head * a.chunks;
         float *const part = a.part + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * HEADS * K::ROW;
-        for (unsigned x = threadIdx.x; x < min((unsigned)HEADS, a.group - chunk * HEADS) * DIM; x += K::THREADS) {
-            const unsigned r = x / DIM, f = x % DIM;
-            float max = -INFINITY, sum = 0.f, v = 0.f;
-            for (unsigned j = 0; j < count; j++) max = fmaxf(max, kept[(places[j] * HEADS + r) * K::ROW + DIM]);
-            const float ref = max == -INFINITY ? 0.f : max;
-            for (unsigned j = 0; j < count; j++) {
-                const float *p = kept + (places[j] * HEADS + r) * K::ROW;
-                const float w = mma::exp2_fast(p[DIM] - ref);
-                sum = fmaf(w, p[DIM + 1], sum);
-                v = fmaf(w, p[f], v);
+        for (unsigned x = threadIdx.x; x < min((unsigned)HEADS, a.group - chunk * HEADS) * (DIM / 4); x += K::THREADS) {
+            const unsigned r = x / (DIM / 4), f = x % (DIM / 4) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (unsigned left = same; left; left &= left - 1) {
+                const unsigned j = __ffs(left) - 1;
+                const float4 p = *reinterpret_cast<const float4 *>(kept + (j * HEADS + r) * K::ROW + f);
+                const float w = weight[j][r];
+                v.x = fmaf(w, p.x, v.x); v.y = fmaf(w, p.y, v.y); v.z = fmaf(w, p.z, v.z); v.w = fmaf(w, p.w, v.w);
             }
+            const float sum = total[first][r];
             if (begins && ends) {
-                const unsigned in_group = chunk * HEADS + r;
-                if (in_group < a.group && f < a.head_dim) store_value<TYPE>(K::out_of(a, e, kv_head, in_group) + f * K::SIZE, sum == 0.f ? 0.f : v / sum);
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                char *const out = K::out_of(a, e, kv_head, chunk * HEADS + r) + f * K::SIZE;
+                if (f >= a.head_dim) continue;
+                if constexpr (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float4 *>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                else *reinterpret_cast<uint2 *>(out) = make_uint2(mma::Of<TYPE>::pack(v.x * inv, v.y * inv), mma::Of<TYPE>::pack(v.z * inv, v.w * inv));
             } else {
-                part[r * K::ROW + f] = v;
-                if (f == 0) { part[r * K::ROW + DIM] = max; part[r * K::ROW + DIM + 1] = sum; }
+                *reinterpret_cast<float4 *>(part + r * K::ROW + f) = v;
+                if (f == 0) *reinterpret_cast<float2 *>(part + r * K::ROW + DIM) = make_float2(kept[(first * HEADS + r) * K::ROW + DIM + 2], sum);
             }
         }
-        if (begins && !ends && threadIdx.x == 0) {
-            // where the item's last step is
-            const unsigned owner = e / each;
-            unsigned long long base = line.before[owner];
-            for (unsigned j = owner * each; j < e; j++) base += (unsigned long long)steps_of(attn::sequence_length(a.at, slot_of(a, j))) * items;
-            const unsigned n = steps_of(attn::sequence_length(a.at, slot_of(a, e)));
-            a.record[2 * blockIdx.x] = item;
-            a.record[2 * blockIdx.x + 1] = (int)attn::part_of_step(all, base + (unsigned long long)(rest + 1) * n - 1, ctas);
-        }
-        i = last + 1;
     }
 }
 
@@ -536,6 +574,23 @@ __global__ void __launch_bounds__(DIM) join_kernel(const Args a) {
     // this CTA's second place, then the first places of the CTAs behind it
     const float *const first = a.part + ((size_t)blockIdx.x * 2 + 1) * SLOT + blockIdx.y * K::ROW;
     auto at = [&](unsigned i) { return first + (i ? (2 * (size_t)i - 1) * SLOT : 0); };
+    // few parts: all that a thread needs is asked for at once
+    constexpr unsigned FEW = 8;
+    if (parts <= FEW) {
+        float m[FEW], l[FEW], x[FEW], max = -INFINITY, sum = 0.f, v = 0.f;
+        #pragma unroll
+        for (unsigned i = 0; i < FEW; i++) {
+            m[i] = -INFINITY; l[i] = x[i] = 0.f;
+            if (i < parts) { const float *const p = at(i); m[i] = p[DIM]; l[i] = p[DIM + 1]; x[i] = p[f]; }
+        }
+        #pragma unroll
+        for (unsigned i = 0; i < FEW; i++) max = fmaxf(max, m[i]);
+        const float ref = max == -INFINITY ? 0.f : max;
+        #pragma unroll
+        for (unsigned i = 0; i < FEW; i++) { const float w = mma::exp2_fast(m[i] - ref); sum = fmaf(w, l[i], sum); v = fmaf(w, x[i], v); }
+        if (f < a.head_dim) store_value<TYPE>(K::out_of(a, e, kv_head, in_group) + f * K::SIZE, sum == 0.f ? 0.f : v / sum);
+        return;
+    }
     float max = -INFINITY;
     for (unsigned i = f; i < parts; i += DIM) max = fmaxf(max, at(i)[DIM]);
     #pragma unroll
