@@ -40,10 +40,20 @@ ATTN_FN long long token_offset(const Pages &c, int slot, unsigned token) {
     return (long long)((size_t)(unsigned)page * c.page_stride + (size_t)(token - i * c.page_size) * c.token_stride);
 }
 
-// `steps` pieces of work are dealt to `parts` workers in order: part p has those from first(p) to before first(p + 1).
-ATTN_FN unsigned long long first_step(unsigned long long steps, unsigned p, unsigned parts) { return steps / parts * p + steps % parts * p / parts; }
+// `steps` pieces of work are dealt to `parts` workers in order: part p has those from first_step(p) = steps * p / parts to before first_step(p + 1).  (In 32 bits where they
+// do: a 64-bit division takes a GPU some hundred instructions.)
+ATTN_FN unsigned long long first_step(unsigned long long steps, unsigned p, unsigned parts) {
+    if (steps >> 32 == 0 && parts < 65536u) {
+        const unsigned n = (unsigned)steps, each = n / parts;
+        return (unsigned long long)each * p + (n - each * parts) * p / parts;
+    }
+    return steps / parts * p + steps % parts * p / parts;
+}
 // The part that has step x: the least p with x < first_step(p + 1), i.e. with (x + 1) * parts <= steps * (p + 1).
-ATTN_FN unsigned part_of_step(unsigned long long steps, unsigned long long x, unsigned parts) { return (unsigned)(((x + 1) * parts - 1) / steps); }
+ATTN_FN unsigned part_of_step(unsigned long long steps, unsigned long long x, unsigned parts) {
+    const unsigned long long all = (x + 1) * parts - 1;
+    return (all | steps) >> 32 ? (unsigned)(all / steps) : (unsigned)all / (unsigned)steps;
+}
 
 // ---- checks of arguments (attention.cpp) ----
 // 0, or the return value after a message; `what` is the entry point.

@@ -439,8 +439,6 @@ __global__ void __launch_bounds__(threads_of(TYPE, DIM, HEADS), ctas_of(TYPE, DI
     __shared__ Line<K::THREADS> line;
     __shared__ int item_of[PLACES], whole_of[PLACES];         // the item (-1: none); bit 0: the place has its first step, bit 1: its last
     __shared__ unsigned long long last_of[PLACES];            // the item's last step, in the line
-    __shared__ unsigned same_as[PLACES];                      // the places of the same item, a bit each
-    __shared__ float weight[PLACES][HEADS], total[PLACES][HEADS];
     const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const unsigned each = (a.entries + K::THREADS - 1) / K::THREADS, items = a.kv_heads * a.chunks;
@@ -453,11 +451,13 @@ __global__ void __launch_bounds__(threads_of(TYPE, DIM, HEADS), ctas_of(TYPE, DI
     if (blockIdx.x >= ctas) return;
     const unsigned long long cta0 = attn::first_step(all, blockIdx.x, ctas), cta1 = attn::first_step(all, blockIdx.x + 1, ctas);
     const unsigned long long steps = cta1 - cta0;
-    unsigned long long pos = cta0 + attn::first_step(steps, warp, K::WARPS);
-    const unsigned long long end = cta0 + attn::first_step(steps, warp + 1, K::WARPS);
-    if (pos < end) {
-        unsigned lo = 0, hi = K::THREADS;       // the last thread whose entries begin at pos or before
-        while (hi - lo > 1) { const unsigned mid = (lo + hi) / 2; if (line.before[mid] <= pos) lo = mid; else hi = mid; }
+    const unsigned warps = (unsigned)min((unsigned long long)K::WARPS, steps);          // the first ones, if there are fewer steps than warps
+    unsigned long long pos = cta0 + attn::first_step(steps, warp, warps);
+    const unsigned long long end = cta0 + attn::first_step(steps, warp + 1, warps);
+    if (warp < warps) {
+        // the last thread whose entries begin at pos or before: of every WARPS-th one, then of the WARPS behind it
+        const unsigned block = 31 - __clz(__ballot_sync(0xffffffffu, line.before[lane * K::WARPS] <= pos));
+        const unsigned lo = block * K::WARPS + 31 - __clz(__ballot_sync(0xffffffffu, lane < K::WARPS && line.before[block * K::WARPS + lane] <= pos));
         unsigned e = lo * each;
         unsigned long long base = line.before[lo];
         while (pos < end) {
@@ -494,65 +494,52 @@ __global__ void __launch_bounds__(threads_of(TYPE, DIM, HEADS), ctas_of(TYPE, DI
         }
     }
     __syncthreads();
-    // Items that warps share: which places each has, ...
-    if (warp == 0) {
-        const int item = lane < PLACES ? item_of[lane] : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, item), first = __ffs(same) - 1, last = 31 - __clz(same);
-        const int begins = __shfl_sync(0xffffffffu, lane < PLACES ? whole_of[lane] : 0, first) & 1, ends = __shfl_sync(0xffffffffu, lane < PLACES ? whole_of[lane] : 0, last) & 2;
-        if (lane < PLACES) {
-            // one that has all of it is done here; of one that goes on behind the CTA the joining kernel has to know
-            same_as[lane] = item >= 0 && lane == first ? same : 0u;
-            if (item >= 0 && lane == first) {
-                whole_of[lane] = begins | ends;
-                if (begins && !ends) { a.record[2 * blockIdx.x + 1] = (int)attn::part_of_step(all, last_of[lane], ctas); a.record[2 * blockIdx.x] = item; }
-            }
-        }
-    }
-    __syncthreads();
-    // ... what each part counts, ...
-    for (unsigned x = threadIdx.x; x < PLACES * HEADS; x += K::THREADS) {
-        const unsigned first = x / HEADS, r = x % HEADS;
-        float max = -INFINITY, sum = 0.f;
-        for (unsigned left = same_as[first]; left; left &= left - 1) max = fmaxf(max, kept[((__ffs(left) - 1) * HEADS + r) * K::ROW + DIM]);
-        const float ref = max == -INFINITY ? 0.f : max;
-        for (unsigned left = same_as[first]; left; left &= left - 1) {
-            const unsigned j = __ffs(left) - 1;
-            const float *p = kept + (j * HEADS + r) * K::ROW + DIM;
-            const float w = mma::exp2_fast(p[0] - ref);
-            weight[j][r] = w;
-            sum = fmaf(w, p[1], sum);
-        }
-        total[first][r] = sum;
-        if (same_as[first]) kept[(first * HEADS + r) * K::ROW + DIM + 2] = max;
-    }
-    __syncthreads();
-    // ... and their sum: four values a thread.
-    for (unsigned first = 0; first < PLACES; first++) {
-        const unsigned same = same_as[first];
-        if (!same) continue;
-        const bool begins = whole_of[first] & 1, ends = whole_of[first] & 2;
-        const unsigned item = (unsigned)item_of[first], e = item / items, rest = item - e * items, kv_head = rest / a.chunks, chunk = rest - kv_head * a.chunks;
-        float *const part = a.part + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * HEADS * K::ROW;
-        for (unsigned x = threadIdx.x; x < min((unsigned)HEADS, a.group - chunk * HEADS) * (DIM / 4); x += K::THREADS) {
-            const unsigned r = x / (DIM / 4), f = x % (DIM / 4) * 4;
+    // Items that warps share.  One's parts are the place where it begins, or the first of a warp that has some of what began before, and the first places of the warps behind.
+    // A warp joins one head of one item: a lane weighs a part each, then four features.
+    const int place_item = lane < PLACES ? item_of[lane] : -1, place_whole = lane < PLACES ? whole_of[lane] : 0;
+    const unsigned same = __match_any_sync(0xffffffffu, place_item), leaders = __ballot_sync(0xffffffffu, place_item >= 0 && (same & ((1u << lane) - 1u)) == 0);
+    const unsigned rows = min((unsigned)HEADS, a.group);
+    unsigned left = leaders, gone = 0;
+    for (unsigned task = warp; task < __popc(leaders) * rows; task += K::WARPS) {
+        for (; gone < task / rows; gone++) left &= left - 1;
+        const unsigned r = task - gone * rows, first = __ffs(left) - 1, places = __shfl_sync(0xffffffffu, same, first), count = __popc(places);
+        const bool begins = __shfl_sync(0xffffffffu, place_whole, first) & 1, ends = __shfl_sync(0xffffffffu, place_whole, 31 - __clz(places)) & 2;
+        const unsigned item = (unsigned)__shfl_sync(0xffffffffu, place_item, first), e = item / items, rest = item - e * items, kv_head = rest / a.chunks, chunk = rest - kv_head * a.chunks;
+        if (chunk * HEADS + r >= a.group) continue;
+        auto row = [&](unsigned i) { return kept + ((i ? (first / 2 + i) * 2 : first) * HEADS + r) * K::ROW; };
+        const float2 mine = lane < count ? *reinterpret_cast<const float2 *>(row(lane) + DIM) : make_float2(-INFINITY, 0.f);
+        float max = mine.x;
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) max = fmaxf(max, __shfl_xor_sync(0xffffffffu, max, o));
+        const float weight = mma::exp2_fast(mine.x - (max == -INFINITY ? 0.f : max));
+        float sum = weight * mine.y;
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        float *const part = a.part + (((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * HEADS + r) * K::ROW;
+        #pragma unroll
+        for (unsigned f0 = 0; f0 < DIM; f0 += 128) {
+            const unsigned f = f0 + lane * 4;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (unsigned left = same; left; left &= left - 1) {
-                const unsigned j = __ffs(left) - 1;
-                const float4 p = *reinterpret_cast<const float4 *>(kept + (j * HEADS + r) * K::ROW + f);
-                const float w = weight[j][r];
+            #pragma unroll 4
+            for (unsigned i = 0; i < count; i++) {
+                const float w = __shfl_sync(0xffffffffu, weight, i);
+                if (DIM < 128 && f >= DIM) continue;
+                const float4 p = *reinterpret_cast<const float4 *>(row(i) + f);
                 v.x = fmaf(w, p.x, v.x); v.y = fmaf(w, p.y, v.y); v.z = fmaf(w, p.z, v.z); v.w = fmaf(w, p.w, v.w);
             }
-            const float sum = total[first][r];
-            if (begins && ends) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            if (f >= DIM) continue;
+            if (!begins || !ends) *reinterpret_cast<float4 *>(part + f) = v;
+            else if (f < a.head_dim) {
                 char *const out = K::out_of(a, e, kv_head, chunk * HEADS + r) + f * K::SIZE;
-                if (f >= a.head_dim) continue;
                 if constexpr (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float4 *>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                 else *reinterpret_cast<uint2 *>(out) = make_uint2(mma::Of<TYPE>::pack(v.x * inv, v.y * inv), mma::Of<TYPE>::pack(v.z * inv, v.w * inv));
-            } else {
-                *reinterpret_cast<float4 *>(part + r * K::ROW + f) = v;
-                if (f == 0) *reinterpret_cast<float2 *>(part + r * K::ROW + DIM) = make_float2(kept[(first * HEADS + r) * K::ROW + DIM + 2], sum);
             }
+        }
+        if (lane == 0 && (!begins || !ends)) {
+            *reinterpret_cast<float2 *>(part + DIM) = make_float2(max, sum);
+            // the joining kernel has to know of one that goes on behind the CTA
+            if (begins && r == 0) { a.record[2 * blockIdx.x + 1] = (int)attn::part_of_step(all, last_of[first], ctas); a.record[2 * blockIdx.x] = (int)item; }
         }
     }
 }
