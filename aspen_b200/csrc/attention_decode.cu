@@ -11,9 +11,8 @@
 // Cut: all (sequence, key head) items' steps stand in one line that is dealt to CTAs and then to their warps in equal shares, whatever the lengths (they are known on the
 // device only, and a captured call may see others each time).  A warp's whole items are finished in its registers; at most two it shares with its neighbours.  Shares are
 // joined in the CTA through shared memory, and those that cross CTAs by a second kernel, started early, in order of the steps: the same call gives the same bits.
+#include "early_launch.cuh"
 #include "mma_sync.cuh"
-
-#include <cuda_runtime.h>
 
 namespace {
 
@@ -440,7 +439,8 @@ __global__ void __launch_bounds__(threads_of(TYPE, DIM, HEADS), ctas_of(TYPE, DI
     __shared__ int item_of[PLACES], whole_of[PLACES];         // the item (-1: none); bit 0: the place has its first step, bit 1: its last
     __shared__ unsigned long long last_of[PLACES];            // the item's last step, in the line
     const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    attn::let_next_kernel_start();
+    attn::wait_for_previous_kernel();
     const unsigned each = (a.entries + K::THREADS - 1) / K::THREADS, items = a.kv_heads * a.chunks;
     if (threadIdx.x < PLACES) item_of[threadIdx.x] = -1;
     if (threadIdx.x == 0) a.record[2 * blockIdx.x] = -1;
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(DIM) join_kernel(const Args a) {
     typedef Kernel<TYPE, DIM, HEADS, true> K;
     constexpr unsigned AT_ONCE = DIM;
     __shared__ float weight[AT_ONCE], maxima[DIM / 32], sums[DIM / 32];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    attn::wait_for_previous_kernel();
     const int item = a.record[2 * blockIdx.x];
     if (item < 0) return;
     const unsigned parts = (unsigned)a.record[2 * blockIdx.x + 1] - blockIdx.x + 1, items = a.kv_heads * a.chunks;      // of the CTAs from this one on
@@ -622,18 +622,9 @@ cudaError_t launch(const Args &a, unsigned sms, cudaStream_t stream) {
     constexpr unsigned CTAS = ctas_of(TYPE, DIM);
     cudaError_t err = cudaFuncSetAttribute(decode_kernel<TYPE, DIM, HEADS, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, K::SMEM);
     if (err != cudaSuccess) return err;
-    decode_kernel<TYPE, DIM, HEADS, WIDE><<<sms * CTAS, K::THREADS, K::SMEM, stream>>>(a);
-    if ((err = cudaGetLastError()) != cudaSuccess) return err;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms * CTAS, a.group < HEADS ? a.group : HEADS);
-    cfg.blockDim = dim3(DIM);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<TYPE, DIM, HEADS>, a);
+    err = attn::launch_early(decode_kernel<TYPE, DIM, HEADS, WIDE>, sms * CTAS, K::THREADS, K::SMEM, stream, a);
+    if (err != cudaSuccess) return err;
+    return attn::launch_early(join_kernel<TYPE, DIM, HEADS>, dim3(sms * CTAS, a.group < HEADS ? a.group : HEADS), DIM, 0, stream, a);
 }
 template <int TYPE, bool WIDE>
 cudaError_t launch(const Args &a, unsigned heads, unsigned dim, unsigned sms, cudaStream_t stream) {

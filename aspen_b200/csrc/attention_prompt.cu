@@ -6,9 +6,8 @@
 // shared memory for the four warps of a CTA, asked for one tile ahead.  Rows in shared memory are 64 (keys) and 16 bytes (values) longer than a power of two, so that the 16-byte pieces
 // that eight lanes read together lie in different banks.
 #include "attention_tc.cuh"
+#include "early_launch.cuh"
 #include "mma_sync.cuh"
-
-#include <cuda_runtime.h>
 
 namespace {
 
@@ -89,6 +88,7 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
     extern __shared__ __align__(128) char smem[];
     const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane >> 2, t = lane & 3, head = blockIdx.y, kv_head = head / a.group;
     Block b;
+    attn::wait_for_previous_kernel();
     if (!find_block(a, blockIdx.x, R::QUERIES, b)) return;
     const int behind = b.keys - b.queries;                      // query i sees keys up to i + behind
     const int last = min(b.queries, b.first + R::QUERIES) - 1;
@@ -255,8 +255,7 @@ cudaError_t launch_rows(const Args &a, cudaStream_t stream) {
     cudaError_t err = cudaFuncSetAttribute(prompt_rows<TYPE, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM);
     if (err != cudaSuccess) return err;
     const unsigned blocks = a.q_rows / R::QUERIES + (a.sequences < a.q_rows ? a.sequences : a.q_rows);
-    prompt_rows<TYPE, DIM><<<dim3(blocks, a.heads), R::THREADS, R::SMEM, stream>>>(a);
-    return cudaGetLastError();
+    return attn::launch_early(prompt_rows<TYPE, DIM>, dim3(blocks, a.heads), R::THREADS, R::SMEM, stream, a);
 }
 template <int TYPE>
 cudaError_t launch_rows(const Args &a, cudaStream_t stream) {
@@ -326,6 +325,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
         tc::fence_proxy_async_smem();
     }
     if (warp == 9) tc::tmem_alloc(&sh.tmem, 512u);
+    attn::wait_for_previous_kernel();
     Job begin;
     bool found = false;
     if (warp == 10) found = find_job(a, blockIdx.x, kv_heads, begin);       // beside the rest of the beginning
@@ -710,8 +710,7 @@ cudaError_t launch_tiles(const Args &a, const CUtensorMap *maps, cudaStream_t st
     const unsigned long long kv_heads = a.heads / a.group, sequences = a.sequences < a.q_rows ? a.sequences : a.q_rows;
     const unsigned long long jobs = ((a.q_rows / fused::TILE + sequences) * a.group + sequences) / 2 * kv_heads;       // at most
     if (jobs > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-    prompt_tiles<TYPE, DIM><<<(unsigned)jobs, fused::THREADS, fused::Shape<DIM>::SMEM, stream>>>(maps[0], maps[1], maps[2], a, (unsigned)kv_heads);
-    return cudaGetLastError();
+    return attn::launch_early(prompt_tiles<TYPE, DIM>, (unsigned)jobs, fused::THREADS, fused::Shape<DIM>::SMEM, stream, maps[0], maps[1], maps[2], a, (unsigned)kv_heads);
 }
 // False: not a call for these kernels.
 bool try_tiles(const Args &a, int type, cudaStream_t stream, cudaError_t *err) {

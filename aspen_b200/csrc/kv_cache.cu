@@ -5,15 +5,17 @@
 //
 // extend, fork and compact begin with ONE CTA of 1024 threads that checks everything before it changes anything and picks pages in a fixed order: the state
 // is small (4 bytes a page; 65 536 pages are 64 loads a thread) and a grid would need two more launches for its sums.  What moves data is a second kernel over all
-// SMs that starts while the first one runs and waits for its end on the device (programmatic launch; a launch behind the first one's end costs some 2 us more).
+// SMs that starts while the first one runs and waits for its end on the device (early_launch.cuh).
 // Pages are copied with 16-byte loads, eight of a thread in flight; bound by memory.
 #include "attention.h"
-
-#include <cuda_runtime.h>
+#include "early_launch.cuh"
 
 namespace {
 
 using attn::Pages;
+using attn::launch_early;
+using attn::let_next_kernel_start;
+using attn::wait_for_previous_kernel;
 
 constexpr unsigned BOOK = 1024;                // threads of the CTA that keeps the books
 constexpr unsigned MOST_PAGES = 1u << 21;      // for one entry of an extend: sums over the CTA's threads stay below 2^32
@@ -50,9 +52,6 @@ Space space_of(const aspen_b200_cache_t &c, unsigned entries, void *workspace) {
     w.mark = w.to + list;
     return w;
 }
-
-__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Sum over the threads before this one; `all` is that over all of them.  For the whole CTA of BOOK threads.
 __device__ __forceinline__ unsigned before_me(unsigned v, unsigned &all, unsigned *sums) {
@@ -97,6 +96,7 @@ __global__ void __launch_bounds__(BOOK) extend_kernel(const Pool pool, const Spa
     __shared__ unsigned sums[32];
     __shared__ int refused;
     const unsigned page = pool.at.page_size;
+    wait_for_previous_kernel();
     if (threadIdx.x == 0) refused = 0;
     if (slots)
         for (unsigned i = threadIdx.x; i < pool.at.sequences; i += BOOK) w.mark[i] = 0;
@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(BOOK) fork_kernel(const Pool pool, const Space
     __shared__ int refused;
     const unsigned page = pool.at.page_size;
     let_next_kernel_start();
+    wait_for_previous_kernel();
     if (threadIdx.x == 0) refused = 0;
     for (unsigned i = threadIdx.x; i < pool.at.sequences; i += BOOK) w.mark[i] = 0;
     __syncthreads();
@@ -282,6 +283,7 @@ __global__ void __launch_bounds__(COPY) fork_copy_kernel(const Pool pool, const 
 
 __global__ void __launch_bounds__(COPY) free_kernel(const Pool pool, const int *slots) {
     __shared__ unsigned length;
+    wait_for_previous_kernel();
     const int slot = slots[blockIdx.x];
     if (slot < 0 || (unsigned)slot >= pool.at.sequences) {
         if (threadIdx.x == 0) atomicOr(pool.at.status, ASPEN_B200_CACHE_BAD_INDEX);
@@ -311,6 +313,7 @@ __global__ void __launch_bounds__(BOOK) compact_kernel(const Pool pool, const Sp
     __shared__ unsigned sums[32];
     const unsigned pages = pool.at.pages;
     let_next_kernel_start();
+    wait_for_previous_kernel();
     unsigned mine = 0, live;
     for (unsigned p0 = threadIdx.x; p0 < pages; p0 += BOOK * SCAN) {
         #pragma unroll
@@ -372,6 +375,7 @@ __global__ void __launch_bounds__(COPY) compact_copy_kernel(const Pool pool, con
     }
 }
 __global__ void __launch_bounds__(COPY) copy_kernel(const Pool pool, const Plane plane, const int *from, const int *to, unsigned count) {
+    wait_for_previous_kernel();
     const ListPair pair{from, to, pool.at.page_size, pool.at.pages};
     for (unsigned i = blockIdx.x * COPY + threadIdx.x; i < count; i += gridDim.x * COPY) {
         int a, b;
@@ -392,6 +396,7 @@ struct New {
 };
 __global__ void __launch_bounds__(COPY) append_kernel(const Pages at /* strides in vectors */, const New n) {
     const unsigned lane = threadIdx.x % 32, r = blockIdx.x * (COPY / 32) + threadIdx.x / 32;
+    wait_for_previous_kernel();
     if (r >= n.rows) return;
     unsigned e = r;
     int begin = (int)r, end = (int)r + 1;
@@ -442,26 +447,11 @@ Plane plane_of(const aspen_b200_cache_t &c) {
     return p;
 }
 
-int done(const char *what) {
-    const cudaError_t err = cudaGetLastError();
+int done(cudaError_t err, const char *what) {
     if (err == cudaSuccess) return 0;
+    cudaGetLastError();
     ASPEN_ERR("%s: %s\n", what, cudaGetErrorString(err));
     return -3;
-}
-
-// A kernel that may start before the one in front of it in the stream has ended, and waits for it itself.
-template <typename... P, typename... A>
-void launch_behind(void (*kernel)(P...), unsigned grid, unsigned threads, cudaStream_t stream, A... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 int check_space(const aspen_b200_cache_t *c, unsigned entries, const void *workspace, size_t bytes, const char *what) {
@@ -493,8 +483,7 @@ extern "C" int aspen_b200_cache_extend(const aspen_b200_cache_t *cache, const in
     const attn::Named all[] = {{cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->refs, "refs"}, {cache->status, "status"},
                                {slots, "slots"}, {starts, "starts"}, {workspace, "workspace"}};
     if ((rc = attn::check_device(all, 7, what))) return rc;
-    extend_kernel<<<1, BOOK, 0, static_cast<cudaStream_t>(cuda_stream)>>>(pool_of(*cache), space_of(*cache, entries, workspace), slots, starts, entries);
-    return done(what);
+    return done(launch_early(extend_kernel, 1, BOOK, 0, static_cast<cudaStream_t>(cuda_stream), pool_of(*cache), space_of(*cache, entries, workspace), slots, starts, entries), what);
 }
 
 extern "C" int aspen_b200_cache_append(const aspen_b200_cache_t *cache, unsigned int layer, const aspen_b200_append_t *a, void *cuda_stream) {
@@ -532,8 +521,7 @@ extern "C" int aspen_b200_cache_append(const aspen_b200_cache_t *cache, unsigned
     n.rows = a->rows;
     n.heads = cache->kv_heads;
     n.vectors = p.row;
-    append_kernel<<<(a->rows + COPY / 32 - 1) / (COPY / 32), COPY, 0, static_cast<cudaStream_t>(cuda_stream)>>>(at, n);
-    return done(what);
+    return done(launch_early(append_kernel, (a->rows + COPY / 32 - 1) / (COPY / 32), COPY, 0, static_cast<cudaStream_t>(cuda_stream), at, n), what);
 }
 
 extern "C" int aspen_b200_cache_fork(const aspen_b200_cache_t *cache, const int *from, const int *to, unsigned int entries, void *workspace, size_t workspace_bytes,
@@ -552,10 +540,8 @@ extern "C" int aspen_b200_cache_fork(const aspen_b200_cache_t *cache, const int 
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     const Pool pool = pool_of(*cache);
     const Space w = space_of(*cache, entries, workspace);
-    fork_kernel<<<1, BOOK, 0, stream>>>(pool, w, from, to, entries);
-    if ((rc = done(what))) return rc;
-    launch_behind(fork_copy_kernel, (unsigned)sms * 4, COPY, stream, pool, w, plane_of(*cache), from, to, entries);
-    return done(what);
+    if ((rc = done(launch_early(fork_kernel, 1, BOOK, 0, stream, pool, w, from, to, entries), what))) return rc;
+    return done(launch_early(fork_copy_kernel, (unsigned)sms * 4, COPY, 0, stream, pool, w, plane_of(*cache), from, to, entries), what);
 }
 
 extern "C" int aspen_b200_cache_free(const aspen_b200_cache_t *cache, const int *slots, unsigned int entries, void *cuda_stream) {
@@ -566,8 +552,7 @@ extern "C" int aspen_b200_cache_free(const aspen_b200_cache_t *cache, const int 
     if (!slots) { ASPEN_ERR("%s: no list of sequences\n", what); return -1; }
     const attn::Named all[] = {{cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->refs, "refs"}, {cache->status, "status"}, {slots, "slots"}};
     if ((rc = attn::check_device(all, 5, what))) return rc;
-    free_kernel<<<entries, COPY, 0, static_cast<cudaStream_t>(cuda_stream)>>>(pool_of(*cache), slots);
-    return done(what);
+    return done(launch_early(free_kernel, entries, COPY, 0, static_cast<cudaStream_t>(cuda_stream), pool_of(*cache), slots), what);
 }
 
 extern "C" int aspen_b200_cache_compact(const aspen_b200_cache_t *cache, void *workspace, size_t workspace_bytes, void *cuda_stream) {
@@ -582,10 +567,8 @@ extern "C" int aspen_b200_cache_compact(const aspen_b200_cache_t *cache, void *w
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     const Pool pool = pool_of(*cache);
     const Space w = space_of(*cache, 0, workspace);
-    compact_kernel<<<1, BOOK, 0, stream>>>(pool, w);
-    if ((rc = done(what))) return rc;
-    launch_behind(compact_copy_kernel, (unsigned)sms * 4, COPY, stream, pool, w, plane_of(*cache));
-    return done(what);
+    if ((rc = done(launch_early(compact_kernel, 1, BOOK, 0, stream, pool, w), what))) return rc;
+    return done(launch_early(compact_copy_kernel, (unsigned)sms * 4, COPY, 0, stream, pool, w, plane_of(*cache)), what);
 }
 
 extern "C" int aspen_b200_cache_copy(const aspen_b200_cache_t *cache, const int *from, const int *to, unsigned int count, void *cuda_stream) {
@@ -598,6 +581,5 @@ extern "C" int aspen_b200_cache_copy(const aspen_b200_cache_t *cache, const int 
     if ((rc = attn::check_device(all, 5, what))) return rc;
     const int sms = attn::sm_count(what);
     if (sms < 0) return sms;
-    copy_kernel<<<(unsigned)sms * 4, COPY, 0, static_cast<cudaStream_t>(cuda_stream)>>>(pool_of(*cache), plane_of(*cache), from, to, count);
-    return done(what);
+    return done(launch_early(copy_kernel, (unsigned)sms * 4, COPY, 0, static_cast<cudaStream_t>(cuda_stream), pool_of(*cache), plane_of(*cache), from, to, count), what);
 }
