@@ -31,6 +31,7 @@ int check_cache(const aspen_b200_cache_t *c, const char *what, bool pool) {
     if (!c->layers || !c->pages || !c->page_size || !c->kv_heads || !c->sequences || !c->max_pages) { ASPEN_ERR("%s: a size of the cache is 0\n", what); return -1; }
     const int bad = check_type(c->type, c->head_dim, what);
     if (bad) return bad;
+    if (c->layers > 1024) { ASPEN_ERR("%s: %u layers; 1024 are possible\n", what, c->layers); return -2; }
     if (c->pages > 0x7fffffffu || c->sequences > 0x7fffffffu || (unsigned long long)c->max_pages * c->page_size > 0x7fffffffull) {
         ASPEN_ERR("%s: pages, sequences and the tokens of a sequence must be below 2^31\n", what);
         return -2;

@@ -6,7 +6,7 @@
 // extend, fork and compact begin with ONE CTA of 1024 threads that checks everything before it changes anything and picks pages in a fixed order: the state
 // is small (4 bytes a page; 65 536 pages are 64 loads a thread) and a grid would need two more launches for its sums.  What moves data is a second kernel over all
 // SMs that starts while the first one runs and waits for its end on the device (early_launch.cuh).
-// Pages are copied with 16-byte loads, eight of a thread in flight; bound by memory.
+// Pages are copied with 16-byte loads, two of each of an SM's 2048 threads in flight (four: compaction of 32 sequences 66 us instead of 62, where 50 are the bytes); bound by memory.
 #include "attention.h"
 #include "early_launch.cuh"
 
@@ -19,7 +19,7 @@ using attn::wait_for_previous_kernel;
 
 constexpr unsigned BOOK = 1024;                // threads of the CTA that keeps the books
 constexpr unsigned MOST_PAGES = 1u << 21;      // for one entry of an extend: sums over the CTA's threads stay below 2^32
-constexpr unsigned COPY = 256, IN_FLIGHT = 8;  // threads of a copying CTA, 16-byte loads in flight of each
+constexpr unsigned COPY = 256, IN_FLIGHT = 2, COPY_CTAS = 8;        // threads of a copying CTA, 16-byte loads in flight of each, CTAs on an SM
 
 struct Pool {
     Pages at;
@@ -207,45 +207,39 @@ struct Plane {
     bool dense;                         // a page of a layer is contiguous
 };
 
-// Vectors first ... of the first `tokens` tokens of a page, one each `step`, from one page to another.
+// Vectors `first`, first + step, ... (IN_FLIGHT of them, those below `end`) of the first `tokens` tokens of a page, from one page to another.
 __device__ __forceinline__ void copy_plane(const Plane &p, const uint4 *src, uint4 *dst, unsigned tokens, unsigned first, unsigned end, unsigned step) {
+    const bool dense = p.dense && tokens == p.page_size;
     const unsigned per = tokens * p.row;
-    for (unsigned i0 = first; i0 < end; i0 += step * IN_FLIGHT) {
-        uint4 v[IN_FLIGHT];
-        size_t at[IN_FLIGHT];
-        #pragma unroll
-        for (unsigned j = 0; j < IN_FLIGHT; j++) {
-            const unsigned i = i0 + j * step;
-            if (p.dense && tokens == p.page_size) at[j] = i;
-            else {
-                const unsigned h = i / per, r = i - h * per, t = r / p.row;
-                at[j] = h * p.head + t * p.token + (r - t * p.row);
-            }
-            if (i < end) v[j] = __ldcs(src + at[j]);
-        }
-        #pragma unroll
-        for (unsigned j = 0; j < IN_FLIGHT; j++)
-            if (i0 + j * step < end) __stcs(dst + at[j], v[j]);
-    }
+    uint4 v[IN_FLIGHT];
+    auto at = [&](unsigned i) -> size_t {
+        if (dense) return i;
+        const unsigned h = i / per, r = i - h * per, t = r / p.row;
+        return h * p.head + t * p.token + (r - t * p.row);
+    };
+    #pragma unroll
+    for (unsigned j = 0; j < IN_FLIGHT; j++) if (first + j * step < end) v[j] = __ldcs(src + at(first + j * step));
+    #pragma unroll
+    for (unsigned j = 0; j < IN_FLIGHT; j++) if (first + j * step < end) __stcs(dst + at(first + j * step), v[j]);
 }
 
-// Copies pages of all layers: CTA by CTA, pieces of COPY * IN_FLIGHT vectors.
+// Copies pages of all layers: worker by worker of `workers`, pieces of COPY * IN_FLIGHT vectors.
 // Pair: bool operator()(unsigned i, int &from, int &to, unsigned &tokens).
 template <typename Pair>
-__device__ __forceinline__ void copy_pages(const Plane &p, unsigned count, const Pair &pair) {
+__device__ __forceinline__ void copy_pages(const Plane &p, unsigned count, const Pair &pair, unsigned worker, unsigned workers) {
     constexpr unsigned PIECE = COPY * IN_FLIGHT;
-    const unsigned whole = p.heads * p.page_size * p.row, pieces = (whole + PIECE - 1) / PIECE;
-    const unsigned long long units = (unsigned long long)count * pieces * p.layers * 2;
-    for (unsigned long long u = blockIdx.x; u < units; u += gridDim.x) {
-        const unsigned piece = (unsigned)(u % pieces);
-        const unsigned long long r = u / pieces;
-        const unsigned kv = (unsigned)(r & 1), layer = (unsigned)((r >> 1) % p.layers), i = (unsigned)((r >> 1) / p.layers);
+    const unsigned whole = p.heads * p.page_size * p.row, pieces = (whole + PIECE - 1) / PIECE, each = pieces * p.layers * 2;        // of a pair of pages
+    const unsigned pairs_on = workers / each, rest_on = workers - pairs_on * each;
+    unsigned i = worker / each, rest = worker - i * each;
+    for (; i < count; i += pairs_on, rest += rest_on) {
+        if (rest >= each) { rest -= each; if (++i >= count) break; }
+        const unsigned plane = rest / pieces, piece = rest - plane * pieces, kv = plane & 1u, layer = plane >> 1;
         int a, b;
         unsigned tokens;
         if (!pair(i, a, b, tokens)) continue;
         const unsigned vectors = p.heads * tokens * p.row, first = piece * PIECE, end = min(vectors, first + PIECE);
         if (first >= vectors) continue;
-        uint4 *const base = p.base[kv] + layer * p.layer;
+        uint4 *const base = (kv ? p.base[1] : p.base[0]) + layer * p.layer;
         copy_plane(p, base + (size_t)a * p.page, base + (size_t)b * p.page, tokens, first + threadIdx.x, end, COPY);
     }
 }
@@ -261,11 +255,13 @@ struct ForkPair {
         return true;
     }
 };
-__global__ void __launch_bounds__(COPY) fork_copy_kernel(const Pool pool, const Space w, const Plane plane, const int *from, const int *to, unsigned entries) {
+__global__ void __launch_bounds__(COPY, COPY_CTAS) fork_copy_kernel(const Pool pool, const Space w, const Plane plane, const int *from, const int *to, unsigned entries) {
     wait_for_previous_kernel();
     if (!w.head[OK]) return;
-    const unsigned max_pages = pool.at.max_pages, page = pool.at.page_size, strips = (max_pages + COPY - 1) / COPY;
-    for (unsigned long long u = blockIdx.x; u < (unsigned long long)entries * strips; u += gridDim.x) {
+    const unsigned max_pages = pool.at.max_pages, page = pool.at.page_size, strips = (max_pages + COPY - 1) / COPY, half = gridDim.x / 2;
+    // half of the CTAs copy tokens, the others rows of the table
+    if (blockIdx.x < half) { copy_pages(plane, entries, ForkPair{w, page}, blockIdx.x, half); return; }
+    for (unsigned long long u = blockIdx.x - half; u < (unsigned long long)entries * strips; u += gridDim.x - half) {
         const unsigned e = (unsigned)(u / strips), i = (unsigned)(u % strips) * COPY + threadIdx.x;
         if (i >= max_pages) continue;
         const unsigned len = (unsigned)w.length[e], full = len / page;
@@ -278,7 +274,6 @@ __global__ void __launch_bounds__(COPY) fork_copy_kernel(const Pool pool, const 
         pool.table[(size_t)to[e] * max_pages + i] = p;
         if (i == 0) pool.lengths[to[e]] = (int)len;
     }
-    copy_pages(plane, entries, ForkPair{w, page});
 }
 
 __global__ void __launch_bounds__(COPY) free_kernel(const Pool pool, const int *slots) {
@@ -363,18 +358,18 @@ struct ListPair {
         return a >= 0 && (unsigned)a < pages && b >= 0 && (unsigned)b < pages;
     }
 };
-__global__ void __launch_bounds__(COPY) compact_copy_kernel(const Pool pool, const Space w, const Plane plane) {
+__global__ void __launch_bounds__(COPY, COPY_CTAS) compact_copy_kernel(const Pool pool, const Space w, const Plane plane) {
     wait_for_previous_kernel();
     const unsigned live = (unsigned)w.head[LIVE], count = (unsigned)w.head[COUNT];
     if (!count) return;
-    copy_pages(plane, count, ListPair{w.from, w.to, pool.at.page_size, pool.at.pages});
+    copy_pages(plane, count, ListPair{w.from, w.to, pool.at.page_size, pool.at.pages}, blockIdx.x, gridDim.x);
     const unsigned long long n = (unsigned long long)pool.at.sequences * pool.at.max_pages;
     for (unsigned long long i = (unsigned long long)blockIdx.x * COPY + threadIdx.x; i < n; i += (unsigned long long)gridDim.x * COPY) {
         const int p = pool.table[i];
         if (p >= 0 && (unsigned)p >= live && (unsigned)p < pool.at.pages && w.mark[p] != p) pool.table[i] = w.mark[p];
     }
 }
-__global__ void __launch_bounds__(COPY) copy_kernel(const Pool pool, const Plane plane, const int *from, const int *to, unsigned count) {
+__global__ void __launch_bounds__(COPY, COPY_CTAS) copy_kernel(const Pool pool, const Plane plane, const int *from, const int *to, unsigned count) {
     wait_for_previous_kernel();
     const ListPair pair{from, to, pool.at.page_size, pool.at.pages};
     for (unsigned i = blockIdx.x * COPY + threadIdx.x; i < count; i += gridDim.x * COPY) {
@@ -382,7 +377,7 @@ __global__ void __launch_bounds__(COPY) copy_kernel(const Pool pool, const Plane
         unsigned tokens;
         if (!pair(i, a, b, tokens)) atomicOr(pool.at.status, ASPEN_B200_CACHE_BAD_INDEX);
     }
-    copy_pages(plane, count, pair);
+    copy_pages(plane, count, pair, blockIdx.x, gridDim.x);
 }
 
 // Append: a warp writes the keys and values of one new token.
@@ -541,7 +536,7 @@ extern "C" int aspen_b200_cache_fork(const aspen_b200_cache_t *cache, const int 
     const Pool pool = pool_of(*cache);
     const Space w = space_of(*cache, entries, workspace);
     if ((rc = done(launch_early(fork_kernel, 1, BOOK, 0, stream, pool, w, from, to, entries), what))) return rc;
-    return done(launch_early(fork_copy_kernel, (unsigned)sms * 4, COPY, 0, stream, pool, w, plane_of(*cache), from, to, entries), what);
+    return done(launch_early(fork_copy_kernel, (unsigned)sms * COPY_CTAS, COPY, 0, stream, pool, w, plane_of(*cache), from, to, entries), what);
 }
 
 extern "C" int aspen_b200_cache_free(const aspen_b200_cache_t *cache, const int *slots, unsigned int entries, void *cuda_stream) {
@@ -568,7 +563,7 @@ extern "C" int aspen_b200_cache_compact(const aspen_b200_cache_t *cache, void *w
     const Pool pool = pool_of(*cache);
     const Space w = space_of(*cache, 0, workspace);
     if ((rc = done(launch_early(compact_kernel, 1, BOOK, 0, stream, pool, w), what))) return rc;
-    return done(launch_early(compact_copy_kernel, (unsigned)sms * 4, COPY, 0, stream, pool, w, plane_of(*cache)), what);
+    return done(launch_early(compact_copy_kernel, (unsigned)sms * COPY_CTAS, COPY, 0, stream, pool, w, plane_of(*cache)), what);
 }
 
 extern "C" int aspen_b200_cache_copy(const aspen_b200_cache_t *cache, const int *from, const int *to, unsigned int count, void *cuda_stream) {
@@ -581,5 +576,5 @@ extern "C" int aspen_b200_cache_copy(const aspen_b200_cache_t *cache, const int 
     if ((rc = attn::check_device(all, 5, what))) return rc;
     const int sms = attn::sm_count(what);
     if (sms < 0) return sms;
-    return done(launch_early(copy_kernel, (unsigned)sms * 4, COPY, 0, static_cast<cudaStream_t>(cuda_stream), pool_of(*cache), plane_of(*cache), from, to, count), what);
+    return done(launch_early(copy_kernel, (unsigned)sms * COPY_CTAS, COPY, 0, static_cast<cudaStream_t>(cuda_stream), pool_of(*cache), plane_of(*cache), from, to, count), what);
 }

@@ -312,7 +312,7 @@ typedef struct {
 } aspen_b200_prompt_t;
 int aspen_b200_attention_prompt(const aspen_b200_prompt_t *prompt, void *cuda_stream);
 
-/* A cache of the keys and values of up to `sequences` sequences, in pages of page_size tokens that they take from one pool.  A program fills the description once,
+/* A cache of the keys and values of up to `sequences` sequences, in pages of page_size tokens that they take from one pool; up to 1024 layers.  A program fills the description once,
  * sets page_table to -1 and lengths, refs and *status to 0, and from then on leaves them to the calls below.
  *     k, v         [layers][pages][kv_heads][page_size][head_dim], or with other strides
  *     page_table   [sequences][max_pages]: token t of sequence s is row t % page_size of page page_table[s][t / page_size], in every layer

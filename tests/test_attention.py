@@ -158,7 +158,7 @@ def good_cache(**change):
 BAD_CACHES = [(dict(type=3), -1), (dict(type=-1), -1), (dict(head_dim=0), -1), (dict(head_dim=12), -1), (dict(head_dim=264), -1), (dict(page_size=0), -1),
               (dict(pages=0), -1), (dict(layers=0), -1), (dict(kv_heads=0), -1), (dict(sequences=0), -1), (dict(max_pages=0), -1), (dict(k=0), -1), (dict(v=0), -1),
               (dict(k=4104), -1), (dict(page_table=0), -1), (dict(lengths=0), -1), (dict(status=0), -1), (dict(token_stride=65), -1), (dict(head_stride=4), -1),
-              (dict(page_stride=1001), -1), (dict(layer_stride=4), -1), (dict(page_size=2**20, max_pages=2**12), -2), (dict(pages=2**31), -2),
+              (dict(page_stride=1001), -1), (dict(layer_stride=4), -1), (dict(page_size=2**20, max_pages=2**12), -2), (dict(pages=2**31), -2), (dict(layers=1025), -2),
               (dict(token_stride=2**30), -2), (dict(page_stride=2**31), -2)]
 
 
