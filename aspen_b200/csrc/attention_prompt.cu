@@ -7,6 +7,7 @@
 // that eight lanes read together lie in different banks.
 #include "attention_tc.cuh"
 #include "early_launch.cuh"
+#include "gemm_split.cuh"
 #include "mma_sync.cuh"
 
 namespace {
@@ -299,6 +300,35 @@ struct Walk {
     }
 };
 
+// The warp that finds the work: the CTA's own first (`begin`, if there is such a job), then that of others that have not begun.
+__device__ __forceinline__ void deal(fused::Shared &sh, const Args &a, unsigned kv_heads, fused::Job begin, bool found) {
+    using namespace fused;
+    const unsigned lane = threadIdx.x % 32;
+    bool ok = true;
+    unsigned index, slot = 0, lap = 0, asked = 0, wanted = 0;
+    while (true) {
+        if (found) {
+            ok = warp_wait(&sh.job_empty[slot], (lap & 1u) ^ 1u, &sh.gave_up);
+            if (ok && lane == 0) { sh.jobs[slot] = begin; tc::mbar_arrive(&sh.job_full[slot]); }
+            __syncwarp();
+            if (++slot == JOBS) { slot = 0; lap++; }
+            if (begin.both() > 0) ok = ok && warp_wait(&sh.wanted, wanted++ & 1u, &sh.gave_up, whole_job(begin.both()));
+            if (!ok) break;
+        }
+        if (lane == 0) ask_for_work(&sh);
+        __syncwarp();
+        ok = warp_wait(&sh.answered, asked++ & 1u, &sh.gave_up);
+        if (!ok) break;
+        const bool more = given_work(&sh, index);
+        tc::fence_proxy_async_smem();          // the answer has been read before the next one is written
+        __syncwarp();
+        if (!more) break;
+        found = find_job(a, index, kv_heads, begin);
+    }
+    if (warp_wait(&sh.job_empty[slot], (lap & 1u) ^ 1u, &sh.gave_up) && lane == 0) { sh.jobs[slot].live = 0; tc::mbar_arrive(&sh.job_full[slot]); }
+    __syncwarp();
+}
+
 template <int TYPE, int DIM>
 __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                                                                    const Args a, unsigned kv_heads) {
@@ -348,7 +378,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                 if (first < 0) continue;
                 float factor = 0.f;
                 if (steps > 0) {
-                    ok = ok && warp_wait(&sh.l_full[w], done >> w & 1u, gave_up) && warp_wait(&sh.o_done[w], done >> w & 1u, gave_up);
+                    ok = ok && warp_wait(&sh.l_full[w], done >> w & 1u, gave_up, whole_job(steps)) && warp_wait(&sh.o_done[w], done >> w & 1u, gave_up);
                     done ^= 1u << w;
                     tc::tc_fence_after();
                     factor = sh.factor[w][row];
@@ -388,28 +418,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         bool ok = true;
         if (warp == 10) {
-            unsigned index, slot = 0, lap = 0, asked = 0, wanted = 0;
-            while (true) {
-                if (found) {
-                    ok = warp_wait(&sh.job_empty[slot], (lap & 1u) ^ 1u, gave_up);
-                    if (ok && lane == 0) { sh.jobs[slot] = begin; tc::mbar_arrive(&sh.job_full[slot]); }
-                    __syncwarp();
-                    if (++slot == JOBS) { slot = 0; lap++; }
-                    if (begin.both() > 0) ok = ok && warp_wait(&sh.wanted, wanted++ & 1u, gave_up);
-                    if (!ok) break;
-                }
-                if (lane == 0) ask_for_work(&sh);
-                __syncwarp();
-                ok = warp_wait(&sh.answered, asked++ & 1u, gave_up);
-                if (!ok) break;
-                const bool more = given_work(&sh, index);
-                tc::fence_proxy_async_smem();          // the answer has been read before the next one is written
-                __syncwarp();
-                if (!more) break;
-                found = find_job(a, index, kv_heads, begin);
-            }
-            if (warp_wait(&sh.job_empty[slot], (lap & 1u) ^ 1u, gave_up) && lane == 0) { sh.jobs[slot].live = 0; tc::mbar_arrive(&sh.job_full[slot]); }
-            __syncwarp();
+            deal(sh, a, kv_heads, begin, found);
         } else if (warp == 8) {
             unsigned stage = 0, lap = 0, q_uses[2] = {0, 0};
             for (Walk walk{&sh}; ok && walk.next(); walk.done()) {
@@ -685,6 +694,333 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
     }
 }
 
+// ---- fp32 on tcgen05: operands of three bf16 parts each (attention_tc.cuh) ----
+
+__global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, unsigned kv_heads) {
+    using namespace fused;
+    typedef Parts H;
+    extern __shared__ char raw[];
+    const unsigned base = (tc::smem_u32(raw) + 1023u) & ~1023u;
+    char *const smem = raw + (base - tc::smem_u32(raw));
+    const unsigned q_at = base, k_at = base + 6 * H::BYTES, v_at = k_at + 3 * H::BYTES;
+    __shared__ __align__(16) Shared sh;
+    const unsigned warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;
+    unsigned *const gave_up = &sh.gave_up;
+    if (threadIdx.x == 0) {
+        sh.gave_up = 0u;
+        tc::mbar_init(&sh.answered, 1u); tc::mbar_init(&sh.wanted, 1u);
+        for (unsigned i = 0; i < JOBS; i++) { tc::mbar_init(&sh.job_full[i], 1u); tc::mbar_init(&sh.job_empty[i], 13u); }
+        for (int w = 0; w < 2; w++) {
+            tc::mbar_init(&sh.q_full[0][w], 128u); tc::mbar_init(&sh.q_empty[0][w], 1u);
+            tc::mbar_init(&sh.s_full[w], 1u); tc::mbar_init(&sh.o_full[w], 1u); tc::mbar_init(&sh.p_full[w][0], 4u);
+        }
+        tc::mbar_init(&sh.k_full[0], 128u); tc::mbar_init(&sh.k_empty[0], 1u); tc::mbar_init(&sh.v_full[0], 128u); tc::mbar_init(&sh.v_empty[0], 1u);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tc::fence_proxy_async_smem();
+    }
+    if (warp == 9) tc::tmem_alloc(&sh.tmem, 512u);
+    attn::wait_for_previous_kernel();
+    Job begin;
+    bool found = false;
+    if (warp == 10) found = find_job(a, blockIdx.x, kv_heads, begin);       // beside the rest of the beginning
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const unsigned tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+    // Registers: 128 x (2 x 168 + 64 + 112) = 512 x 128, what the launch holds
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        // Splits queries, keys and values: a thread eight features of every 16th row.
+        const unsigned t = threadIdx.x & 127u, row0 = t >> 3, piece = t & 7u;
+        unsigned q_uses[2] = {0, 0}, uses = 0;
+        bool ok = true;
+        auto stage = [&](const char *from, size_t stride, int rows, unsigned to, unsigned long long *empty, unsigned parity, unsigned long long *full) {
+            float4 v[8][2];
+            #pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int r = (int)row0 + 16 * i;
+                const bool in = r < rows && piece * 8 < a.head_dim;
+                const char *const p = from + (in ? (size_t)r * stride + piece * 8 : 0) * 4;
+                v[i][0] = in ? __ldg(reinterpret_cast<const float4 *>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[i][1] = in ? __ldg(reinterpret_cast<const float4 *>(p) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            if (!warp_wait(empty, parity, gave_up)) { ok = false; return; }
+            #pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const unsigned r = row0 + 16 * i;
+                split::Pair x[4] = {split::pack(v[i][0].x, v[i][0].y), split::pack(v[i][0].z, v[i][0].w), split::pack(v[i][1].x, v[i][1].y), split::pack(v[i][1].z, v[i][1].w)};
+                char *const at = smem + (to - base) + r * 128 + ((piece ^ (r & 7u)) << 4);
+                *reinterpret_cast<uint4 *>(at) = make_uint4(split::take_part<0>(x[0]), split::take_part<0>(x[1]), split::take_part<0>(x[2]), split::take_part<0>(x[3]));
+                *reinterpret_cast<uint4 *>(at + H::BYTES) = make_uint4(split::take_part<1>(x[0]), split::take_part<1>(x[1]), split::take_part<1>(x[2]), split::take_part<1>(x[3]));
+                *reinterpret_cast<uint4 *>(at + 2 * H::BYTES) = make_uint4(split::take_part<2>(x[0]), split::take_part<2>(x[1]), split::take_part<2>(x[2]), split::take_part<2>(x[3]));
+            }
+            tc::fence_proxy_async_smem();
+            tc::mbar_arrive(full);
+        };
+        for (Walk walk{&sh}; ok && walk.next(); walk.done()) {
+            const Job &job = walk.job();
+            const int steps = job.both();
+            #pragma unroll 1
+            for (int w = 0; w < 2 && ok; w++) {
+                if (job.steps[w] == 0) continue;
+                stage(a.q + ((size_t)(job.q0 + job.first[w]) * a.q_row + job.head[w] * a.q_head) * 4, a.q_row, job.queries - job.first[w], q_at + w * 3 * H::BYTES, &sh.q_empty[0][w],
+                      (q_uses[w] & 1u) ^ 1u, &sh.q_full[0][w]);
+                q_uses[w]++;
+            }
+            #pragma unroll 1
+            for (int i = 0; i < 2 * steps && ok; i++) {
+                const int key = i / 2 * (int)TILE;
+                if (i & 1) stage(a.v + ((size_t)(job.k0 + key) * a.v_row + job.kv_head * a.v_head) * 4, a.v_row, job.keys - key, v_at, &sh.v_empty[0], (uses & 1u) ^ 1u, &sh.v_full[0]);
+                else stage(a.k + ((size_t)(job.k0 + key) * a.k_row + job.kv_head * a.k_head) * 4, a.k_row, job.keys - key, k_at, &sh.k_empty[0], (uses & 1u) ^ 1u, &sh.k_full[0]);
+                uses += i & 1;
+            }
+        }
+        __syncwarp();
+        tc::tc_fence_before();
+        __syncthreads();
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        bool ok = true;
+        if (warp == 10) deal(sh, a, kv_heads, begin, found);
+        else if (warp == 9) {
+            constexpr unsigned IDESC = 1u << 4 | 1u << 7 | 1u << 10 | (128u >> 4) << 24;               // sums fp32, operands bf16, 128 rows
+            constexpr unsigned IDESC_S = IDESC | (128u >> 3) << 17, IDESC_O = IDESC | (64u >> 3) << 17 | 1u << 16;        // the second operand of PV: features contiguous
+            unsigned k_uses = 0, v_uses = 0, q_uses[2] = {0, 0}, done[2] = {0, 0};
+            Walk walk{&sh};
+            int steps[2], next[2] = {0, 0};
+            bool live = true, begun = false;          // begun: the next job's first scores have been asked for
+            auto look = [&]() {
+                next[0] = next[1] = 0;
+                live = walk.next();
+                if (!live) return;
+                const Job &job = walk.job();
+                next[0] = tc::uniform(job.steps[0]);
+                next[1] = tc::uniform(job.steps[1]);
+                walk.done();
+            };
+            // Six of the nine products of parts, smallest first: what the sums cut off then is small.
+            auto scores = [&](int w, bool first, bool last) {
+                if (first) ok = ok && warp_wait(&sh.q_full[0][w], q_uses[w] & 1u, gave_up);
+                if (last) q_uses[w]++;
+                if (!ok) return;
+                tc::tc_fence_after();
+                const unsigned q = q_at + w * 3 * H::BYTES, d = tmem + w * 256;
+                if (tc::elect_one()) {
+                    constexpr unsigned char order[6][2] = {{2, 0}, {1, 1}, {0, 2}, {1, 0}, {0, 1}, {0, 0}};
+                    #pragma unroll
+                    for (int p = 0; p < 6; p++) {
+                        const unsigned x = tc::umma_desc_low(q + order[p][0] * H::BYTES), y = tc::umma_desc_low(k_at + order[p][1] * H::BYTES);
+                        #pragma unroll
+                        for (int k = 0; k < 4; k++) mma_ss(d, x + k * 2, y + k * 2, IDESC_S, p + k);
+                    }
+                    tc::tc_commit(&sh.s_full[w]);
+                    if (last) tc::tc_commit(&sh.q_empty[0][w]);
+                }
+                __syncwarp();
+            };
+            auto values = [&](int w) {
+                const unsigned d = tmem + w * 256;
+                if (tc::elect_one()) {
+                    constexpr unsigned char order[6][2] = {{2, 0}, {1, 1}, {0, 2}, {1, 0}, {0, 1}, {0, 0}};
+                    #pragma unroll
+                    for (int p = 0; p < 6; p++) {
+                        const unsigned x = d + (order[p][0] == 2 ? 128 : order[p][0] * 16), apart = order[p][0] == 2 ? 16 : 32, y = (v_at + order[p][1] * H::BYTES) >> 4;
+                        #pragma unroll
+                        for (int k = 0; k < 8; k++) mma_ts(d + H::O, x + k / 2 * apart + k % 2 * 8, y + k * 128, IDESC_O, p + k);
+                    }
+                    tc::tc_commit(&sh.o_full[w]);
+                }
+                __syncwarp();
+            };
+            auto release = [&](unsigned long long *bar) { if (tc::elect_one()) tc::tc_commit(bar); __syncwarp(); };
+            for (look(); ok && live;) {
+                if (!next[0] && !next[1]) { look(); continue; }
+                if (!begun) {
+                    ok = warp_wait(&sh.k_full[0], k_uses++ & 1u, gave_up);
+                    #pragma unroll 1
+                    for (int w = 0; w < 2; w++) if (next[w]) scores(w, true, next[w] == 1);
+                    if (!ok) break;
+                    release(&sh.k_empty[0]);
+                }
+                steps[0] = next[0]; steps[1] = next[1];
+                const int all = max(steps[0], steps[1]);
+                #pragma unroll 1
+                for (int j = 0; j < all; j++) {
+                    // the scores to ask for now: the next step's, or the next job's first ones
+                    const bool turn = j + 1 == all;
+                    if (j == max(0, all - 3) && lane == 0) tc::mbar_arrive(&sh.wanted);
+                    if (turn) look();
+                    const int then = turn ? 0 : j + 1, until[2] = {turn ? next[0] : steps[0], turn ? next[1] : steps[1]};
+                    const bool more = then < until[0] || then < until[1];
+                    begun = turn && more;
+                    ok = warp_wait(&sh.v_full[0], v_uses++ & 1u, gave_up);
+                    bool keys = false;
+                    #pragma unroll 1
+                    for (int w = 0; w < 2; w++) {
+                        if (ok && j < steps[w]) {
+                            ok = warp_wait(&sh.p_full[w][0], done[w]++ & 1u, gave_up);
+                            if (!ok) break;
+                            tc::tc_fence_after();
+                            values(w);
+                        }
+                        if (ok && then < until[w]) {
+                            if (!keys) ok = warp_wait(&sh.k_full[0], k_uses++ & 1u, gave_up);
+                            keys = true;
+                            scores(w, turn, then + 1 == until[w]);
+                        }
+                    }
+                    if (!ok) break;
+                    release(&sh.v_empty[0]);
+                    if (more) release(&sh.k_empty[0]);
+                }
+            }
+        }
+        __syncwarp();
+        tc::tc_fence_before();
+        __syncthreads();
+        if (warp == 9) {
+            if (sh.gave_up) {
+                // MMAs may still be in flight; they take microseconds
+                unsigned long long t0, now;
+                asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+                do { __nanosleep(1000); asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now)); } while (now - t0 < 2000000ull);
+            }
+            tc::tc_fence_after();
+            tc::tmem_dealloc(tmem, 512u);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        const int w = (int)(warp >> 2);
+        const unsigned row = (warp & 3u) * 32u + lane, s_at = tmem + ((warp & 3u) << 21) + w * 256;
+        float4 *const turn = reinterpret_cast<float4 *>(smem + 12 * H::BYTES + warp * 4096);
+        const Pair scale2 = pair(a.scale, a.scale);
+        unsigned done = 0;
+        bool ok = true;
+        for (Walk walk{&sh}; walk.next(); walk.done()) {
+            const Job &job = walk.job();
+            const int first = job.first[w], steps = tc::uniform(job.steps[w]);
+            if (first < 0) continue;
+            const int query = first + (int)row;
+            const int seen = a.masked ? min(job.keys, query + job.behind() + 1) : job.keys;              // first key that the row does not see
+            const int least_seen = __shfl_sync(0xffffffffu, seen, 0), most_seen = __shfl_sync(0xffffffffu, seen, 31);       // of the warp's rows
+            float max = -INFINITY, sum = 0.f, down = 0.f;
+            Pair o[32];
+            #pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = 0ull;
+            // scores of 32 keys; those that are not seen are -inf
+            auto load = [&](float *s, int key) {
+                ld32(s_at + (key & 127), s);
+                ld_done32(s);
+                if (least_seen < key + 32) {
+                    const int left = seen - key;
+                    #pragma unroll
+                    for (int i = 0; i < 32; i++) s[i] = i < left ? s[i] : -INFINITY;
+                }
+            };
+            // the last product, relative to the maximum of its step, to the sums
+            auto add = [&]() {
+                ok = ok && warp_wait(&sh.o_full[w], (done & 1u) ^ 1u, gave_up);
+                tc::tc_fence_after();
+                const Pair down2 = pair(down, down);
+                #pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float v[32];
+                    ld32(s_at + H::O + h * 32, v);
+                    ld_done32(v);
+                    #pragma unroll
+                    for (int i = 0; i < 16; i++) o[h * 16 + i] = fma2(o[h * 16 + i], down2, pair(v[2 * i], v[2 * i + 1]));
+                }
+            };
+            #pragma unroll 1
+            for (int j = 0; j < steps && ok; j++) {
+                ok = warp_wait(&sh.s_full[w], done & 1u, gave_up);
+                if (!ok) break;
+                tc::tc_fence_after();
+                const int key0 = j * (int)TILE, key1 = min(key0 + (int)TILE, most_seen);
+                float m0 = -INFINITY, m1 = -INFINITY;
+                #pragma unroll 1
+                for (int key = key0; key < key1; key += 32) {
+                    float s[32];
+                    load(s, key);
+                    #pragma unroll
+                    for (int i = 0; i < 32; i += 4) { m0 = max3(m0, s[i], s[i + 1]); m1 = max3(m1, s[i + 2], s[i + 3]); }
+                }
+                // a NaN stays the maximum, and so it becomes if a score is infinite: then all weights of the row are NaN
+                float top = max3(max, m0, m1);
+                if (top == INFINITY) top = NAN;
+                const float ref = top == -INFINITY ? 0.f : -top * a.scale, next_down = top == -INFINITY ? 1.f : mma::exp2_fast((max - top) * a.scale);
+                const Pair ref2 = pair(ref, ref);
+                max = top;
+                sum *= next_down;
+                Pair part[2] = {0ull, 0ull};
+                #pragma unroll 1
+                for (int key = key0; key < key0 + (int)TILE; key += 32) {
+                    unsigned p[3][16];
+                    if (most_seen > key) {
+                        float s[32];
+                        load(s, key);
+                        #pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const Pair x = fma2(pair(s[2 * i], s[2 * i + 1]), scale2, ref2);
+                            float y0, y1;
+                            unpair(x, y0, y1);
+                            Pair y = pair(mma::exp2_fast(y0), mma::exp2_fast(y1));
+                            part[i & 1] = add2(part[i & 1], y);
+                            p[0][i] = split::take_part<0>(y);
+                            p[1][i] = split::take_part<1>(y);
+                            p[2][i] = split::take_part<2>(y);
+                        }
+                    } else {
+                        #pragma unroll
+                        for (int i = 0; i < 16; i++) p[0][i] = p[1][i] = p[2][i] = 0u;
+                    }
+                    // two parts in the place of their scores
+                    st16(s_at + (key & 127), p[0]);
+                    st16(s_at + (key & 127) + 16, p[1]);
+                    st16(s_at + 128 + (key & 127) / 2, p[2]);
+                }
+                float x0, x1;
+                unpair(add2(part[0], part[1]), x0, x1);
+                sum += x0 + x1;
+                if (j > 0) add();
+                down = next_down;
+                st_done();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sh.p_full[w][0]);
+                done++;
+            }
+            if (steps > 0) add();
+            tc::tc_fence_before();
+            const float inv = !ok ? NAN : sum == 0.f ? 0.f : 1.f / sum;
+            char *const out = a.out + ((size_t)(job.q0 + first) * a.out_row + job.head[w] * a.out_head) * 4;
+            const int left = job.queries - first;
+            // 32 features at a time: a thread has its row's, and stores 16 bytes each of four rows
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                __syncwarp();
+                #pragma unroll
+                for (unsigned x = 0; x < 8; x++) {
+                    float4 y;
+                    unpair(o[h * 16 + 2 * x], y.x, y.y);
+                    unpair(o[h * 16 + 2 * x + 1], y.z, y.w);
+                    turn[lane * 8 + (x ^ (lane & 7u))] = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+                }
+                __syncwarp();
+                const unsigned f = h * 32 + (lane & 7u) * 4;
+                #pragma unroll
+                for (unsigned x = 0; x < 8; x++) {
+                    const unsigned r = x * 4 + (lane >> 3), q = (warp & 3u) * 32 + r;
+                    if ((int)q < left && f < a.head_dim) *reinterpret_cast<float4 *>(out + (q * a.out_row + f) * 4) = turn[r * 8 + ((lane & 7u) ^ (r & 7u))];
+                }
+            }
+        }
+        __syncwarp();
+        tc::tc_fence_before();
+        __syncthreads();
+    }
+}
+
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeFn encode_fn() {
@@ -703,18 +1039,32 @@ bool encode(CUtensorMap *map, int type, const char *p, unsigned dim, unsigned he
                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Jobs of a call, at most.
+unsigned long long jobs_of(const Args &a) {
+    const unsigned long long kv_heads = a.heads / a.group, sequences = a.sequences < a.q_rows ? a.sequences : a.q_rows;
+    return ((a.q_rows / fused::TILE + sequences) * a.group + sequences) / 2 * kv_heads;
+}
+cudaError_t launch_parts(const Args &a, cudaStream_t stream) {
+    cudaError_t err = cudaFuncSetAttribute(prompt_parts, cudaFuncAttributeMaxDynamicSharedMemorySize, fused::Parts::SMEM);
+    if (err != cudaSuccess) return err;
+    return attn::launch_early(prompt_parts, (unsigned)jobs_of(a), fused::THREADS, fused::Parts::SMEM, stream, a, a.heads / a.group);
+}
 template <int TYPE, int DIM>
 cudaError_t launch_tiles(const Args &a, const CUtensorMap *maps, cudaStream_t stream) {
     cudaError_t err = cudaFuncSetAttribute(prompt_tiles<TYPE, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, fused::Shape<DIM>::SMEM);
     if (err != cudaSuccess) return err;
-    const unsigned long long kv_heads = a.heads / a.group, sequences = a.sequences < a.q_rows ? a.sequences : a.q_rows;
-    const unsigned long long jobs = ((a.q_rows / fused::TILE + sequences) * a.group + sequences) / 2 * kv_heads;       // at most
-    if (jobs > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-    return attn::launch_early(prompt_tiles<TYPE, DIM>, (unsigned)jobs, fused::THREADS, fused::Shape<DIM>::SMEM, stream, maps[0], maps[1], maps[2], a, (unsigned)kv_heads);
+    return attn::launch_early(prompt_tiles<TYPE, DIM>, (unsigned)jobs_of(a), fused::THREADS, fused::Shape<DIM>::SMEM, stream, maps[0], maps[1], maps[2], a, a.heads / a.group);
 }
 // False: not a call for these kernels.
 bool try_tiles(const Args &a, int type, cudaStream_t stream, cudaError_t *err) {
-    if (type == ASPEN_B200_FP32 || a.head_dim > 128 || !a.kv_rows || !(a.scale > 0.f) || !encode_fn()) return false;      // a row's largest score is its largest product only for a scale above 0
+    // a row's largest score is its largest product only for a scale above 0
+    if (!a.kv_rows || !(a.scale > 0.f) || jobs_of(a) > 0x7fffffffull) return false;
+    if (type == ASPEN_B200_FP32) {
+        if (a.head_dim > 64) return false;
+        *err = launch_parts(a, stream);
+        return true;
+    }
+    if (a.head_dim > 128 || !encode_fn()) return false;
     const unsigned kv_heads = a.heads / a.group;
     CUtensorMap maps[3];
     if (!encode(&maps[0], type, a.q, a.head_dim, a.heads, a.q_rows, a.q_head, a.q_row) || !encode(&maps[1], type, a.k, a.head_dim, kv_heads, a.kv_rows, a.k_head, a.k_row) ||

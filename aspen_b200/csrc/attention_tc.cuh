@@ -25,7 +25,7 @@
 //
 // Values behind the end of a sequence are another one's, or nobody's: the MMA warp sets them to zero in shared memory, since 0 x NaN would reach every row.
 //
-// Every wait is bounded (2 s) and is for another role of the CTA; if one runs out all roles leave, TMEM is freed and the rows of out that were in work become NaN.
+// Every wait is bounded (2 s, or 2 s and 100 us a step) and is for another role of the CTA; if one runs out all roles leave, TMEM is freed and the rows of out that were in work become NaN.
 #pragma once
 #include "tiles_tc.cuh"
 
@@ -45,6 +45,13 @@ struct Shape {
     static constexpr int SMEM = 2 * QUERIES * BYTES + 2 * STAGES * BYTES + OUT_BYTES + 1024;
     static constexpr bool OWN_P = DIM == 64;
     static constexpr unsigned S = 0, O = 256, P = OWN_P ? 384 : 0, P_APART = OWN_P ? 64 : 128;      // TMEM columns
+};
+
+// fp32, heads of up to 64 features: every operand as three bf16 parts, six of the nine products.
+struct Parts {
+    static constexpr int BYTES = TILE * 128;                        // a part of a tile: 128 rows of 64 features
+    static constexpr int SMEM = 12 * BYTES + 8 * 4096 + 1024;       // two tiles of queries, keys, values; outputs being turned round
+    static constexpr unsigned O = 192;                              // TMEM columns of a tile: scores 128 (then two parts of the weights), the third part 64, a product 64
 };
 
 // A CTA's work: two tiles of queries of one sequence and one head of keys.
@@ -83,7 +90,7 @@ __device__ __forceinline__ bool given_work(Shared *sh, unsigned &index) {
     return yes != 0u;
 }
 
-__device__ __forceinline__ bool wait(unsigned long long *bar, unsigned parity, unsigned *gave_up) {
+__device__ __forceinline__ bool wait(unsigned long long *bar, unsigned parity, unsigned *gave_up, unsigned long long limit) {
     #pragma unroll 1
     for (unsigned spin = 0; spin < 4096u; spin++)
         if (tc::mbar_try_wait(bar, parity)) return true;
@@ -95,12 +102,16 @@ __device__ __forceinline__ bool wait(unsigned long long *bar, unsigned parity, u
         if ((spin & 255u) == 0u) {
             asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
             if (*(volatile unsigned *)gave_up != 0u) return false;
-            if (now - t0 > LIMIT_NS) { atomicExch(gave_up, 1u); return false; }
+            if (now - t0 > limit) { atomicExch(gave_up, 1u); return false; }
         }
     }
 }
 // A warp's lanes wait, and give up, together.
-__device__ __forceinline__ bool warp_wait(unsigned long long *bar, unsigned parity, unsigned *gave_up) { return __all_sync(0xffffffffu, wait(bar, parity, gave_up)); }
+__device__ __forceinline__ bool warp_wait(unsigned long long *bar, unsigned parity, unsigned *gave_up, unsigned long long limit = LIMIT_NS) {
+    return __all_sync(0xffffffffu, wait(bar, parity, gave_up, limit));
+}
+// For something that comes at the end of a job: 100 us a step more.
+__device__ __forceinline__ unsigned long long whole_job(int steps) { return LIMIT_NS + 100000ull * (unsigned)steps; }
 
 // Both operands in shared memory, K-major, 128-byte swizzle; or A in TMEM and B with features contiguous (MN-major): 64 features of a row side by side, the next 64
 // CHUNK_BYTES on, eight keys 1024 bytes.
