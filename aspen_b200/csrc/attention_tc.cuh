@@ -52,6 +52,9 @@ struct Parts {
     static constexpr int BYTES = TILE * 128;                        // a part of a tile: 128 rows of 64 features
     static constexpr int SMEM = 12 * BYTES + 8 * 4096 + 1024;       // two tiles of queries, keys, values; outputs being turned round
     static constexpr unsigned O = 192;                              // TMEM columns of a tile: scores 128 (then two parts of the weights), the third part 64, a product 64
+    // the parts of product p: 2 0, 1 1, 0 2, 1 0, 0 1, 0 0
+    static __device__ __forceinline__ unsigned first(int p) { return 0x001012u >> (4 * p) & 15u; }
+    static __device__ __forceinline__ unsigned second(int p) { return 0x010210u >> (4 * p) & 15u; }
 };
 
 // A CTA's work: two tiles of queries of one sequence and one head of keys.
