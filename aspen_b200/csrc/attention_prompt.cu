@@ -8,6 +8,7 @@
 #include "attention_tc.cuh"
 #include "early_launch.cuh"
 #include "gemm_split.cuh"
+#include "index_div.h"
 #include "mma_sync.cuh"
 
 namespace {
@@ -16,8 +17,11 @@ struct Args {
     const char *q, *k, *v;
     char *out;
     const int *q_starts, *kv_starts;
-    size_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;      // in elements
+    unsigned q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;    // in elements, below 2^29
     unsigned sequences, q_rows, kv_rows, heads, group, head_dim;
+    unsigned part;                      // of 2^16 that is one over the group, rounded up: r / group = r * part >> 16 for r and group up to 128
+    unsigned block;                     // 128 / group
+    Divisor by_block;
     int masked;
     float scale;                        // with log2(e)
 };
@@ -149,9 +153,13 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
             for (int n = 0; n < KT; n++) {
                 const uint4 w = *reinterpret_cast<const uint4 *>(ks + (n * 8 + g) * R::KPITCH + f);
                 if constexpr (TYPE == ASPEN_B200_FP32) {
+                    // sums of 16 features are added outside: the tensor cores cut off what they add to a sum
                     const unsigned a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w}, b0[2] = {w.x, w.y}, b1[2] = {w.z, w.w};
-                    mma::tf32x3(s[n], a0, b0);
-                    mma::tf32x3(s[n], a1, b1);
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma::tf32x3(part, a0, b0);
+                    mma::tf32x3(part, a1, b1);
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++) s[n][j] += part[j];
                 } else {
                     mma::Of<TYPE>::step(s[n], x.x, y.x, x.y, y.y, w.x, w.y);
                     mma::Of<TYPE>::step(s[n], x.z, y.z, x.w, y.w, w.z, w.w);
@@ -191,16 +199,21 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
         }
         if constexpr (TYPE == ASPEN_B200_FP32) {
             #pragma unroll
-            for (int n = 0; n < KT; n++) {
-                const unsigned p[4] = {__float_as_uint(s[n][0]), __float_as_uint(s[n][2]), __float_as_uint(s[n][1]), __float_as_uint(s[n][3])};
-                const char *const row = vs + (n * 8 + 2 * t) * R::VPITCH;
+            for (int i = 0; i < R::VPIECES; i++) {
+                float part[4][4];
                 #pragma unroll
-                for (int i = 0; i < R::VPIECES; i++) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(row + (i * 32 + g * 4) * SIZE), y = *reinterpret_cast<const uint4 *>(row + R::VPITCH + (i * 32 + g * 4) * SIZE);
+                for (int j = 0; j < 16; j++) part[j / 4][j % 4] = 0.f;
+                #pragma unroll
+                for (int n = 0; n < KT; n++) {
+                    const unsigned p[4] = {__float_as_uint(s[n][0]), __float_as_uint(s[n][2]), __float_as_uint(s[n][1]), __float_as_uint(s[n][3])};
+                    const char *const row = vs + (n * 8 + 2 * t) * R::VPITCH + (i * 32 + g * 4) * SIZE;
+                    const uint4 x = *reinterpret_cast<const uint4 *>(row), y = *reinterpret_cast<const uint4 *>(row + R::VPITCH);
                     const unsigned w0[4] = {x.x, x.y, x.z, x.w}, w1[4] = {y.x, y.y, y.z, y.w};
                     #pragma unroll
-                    for (int j = 0; j < 4; j++) { const unsigned w[2] = {w0[j], w1[j]}; mma::tf32x3(o[i * 4 + j], p, w); }
+                    for (int j = 0; j < 4; j++) { const unsigned w[2] = {w0[j], w1[j]}; mma::tf32x3(part[j], p, w); }
                 }
+                #pragma unroll
+                for (int j = 0; j < 16; j++) o[i * 4 + j / 4][j % 4] += part[j / 4][j % 4];
             }
         } else {
             typedef mma::Of<TYPE> T;
@@ -265,67 +278,76 @@ cudaError_t launch_rows(const Args &a, cudaStream_t stream) {
 
 // ---- tcgen05 (attention_tc.cuh) ----
 
-// As find_piece, in another order: the last piece of the sequence that has most, ..., the first pieces of all sequences.  With a mask the keys of a piece go by its number, so heavy work
-// comes first, whatever sequence it is of, and light work fills the ends (8 prompts of 512 tokens: 7 tiles on the busiest SM instead of 10).  For up to 128 sequences, four a lane.
-constexpr unsigned LEVELLED = 128;
-template <typename Pieces>
-__device__ __forceinline__ int find_levelled(const Args &a, unsigned index, const Pieces &pieces, int &q_first, int &queries, int &k_first, int &keys) {
-    const unsigned lane = threadIdx.x % 32;
-    unsigned n[4], most = 0;
-    #pragma unroll
-    for (unsigned k = 0; k < 4; k++) {
-        const unsigned s = lane * 4 + k;
-        n[k] = s < a.sequences ? pieces((unsigned)max(0, clamped(a.q_starts, s + 1, a.q_rows) - clamped(a.q_starts, s, a.q_rows))) : 0u;
-        most = max(most, n[k]);
+// Finds the jobs of a call: job `index` is two neighbouring tiles of a sequence and a head of keys.  With a mask the keys of a tile go by its number, so pairs of tiles are counted not
+// sequence by sequence but from the highest number down: heavy work comes first, whatever sequence it is of, and light work fills the ends (8 prompts of 512 tokens: 7 tiles on the busiest
+// SM instead of 10).  For up to 128 sequences, whose numbers of pairs a warp keeps, four a lane.
+struct Finder {
+    unsigned n[4], most;
+    bool levelled;
+    static __device__ __forceinline__ unsigned pairs(const Args &a, unsigned queries) { return (div_by(queries + a.block - 1, a.by_block) + 1) / 2; }
+    __device__ __forceinline__ Finder(const Args &a) : most(0), levelled(a.masked && a.sequences <= 128) {
+        if (!levelled) return;
+        #pragma unroll
+        for (unsigned k = 0; k < 4; k++) {
+            const unsigned s = threadIdx.x % 32 * 4 + k;
+            n[k] = s < a.sequences ? pairs(a, (unsigned)max(0, clamped(a.q_starts, s + 1, a.q_rows) - clamped(a.q_starts, s, a.q_rows))) : 0u;
+            most = max(most, n[k]);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
     }
-    // pieces numbered `level` and above
-    auto from = [&](unsigned level) {
+    // pairs numbered `level` and above
+    __device__ __forceinline__ unsigned from(unsigned level) const {
         unsigned x = 0;
         #pragma unroll
         for (unsigned k = 0; k < 4; k++) x += n[k] > level ? n[k] - level : 0u;
         return __reduce_add_sync(0xffffffffu, x);
-    };
-    if (index >= from(0)) return -1;
-    unsigned lo = 0, hi = __reduce_max_sync(0xffffffffu, most);         // the largest level that `index` is behind: from(lo) > index >= from(hi)
-    while (hi - lo > 1) { const unsigned mid = (lo + hi) / 2; if (from(mid) > index) lo = mid; else hi = mid; }
-    const unsigned rank = index - from(lo + 1);
-    unsigned mine = 0;
-    #pragma unroll
-    for (unsigned k = 0; k < 4; k++) mine += n[k] > lo;
-    unsigned sum = mine;
-    #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const unsigned u = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= (unsigned)o) sum += u; }
-    const int at = __ffs(__ballot_sync(0xffffffffu, sum > rank)) - 1;
-    unsigned left = rank - (sum - mine), which = 0;
-    #pragma unroll
-    for (unsigned k = 0; k < 4; k++) if (n[k] > lo) { if (left == 0) which = k; left--; }
-    const unsigned s = at * 4 + __shfl_sync(0xffffffffu, which, at);
-    q_first = clamped(a.q_starts, s, a.q_rows);
-    queries = clamped(a.q_starts, s + 1, a.q_rows) - q_first;
-    k_first = clamped(a.kv_starts, s, a.kv_rows);
-    keys = max(0, clamped(a.kv_starts, s + 1, a.kv_rows) - k_first);
-    return (int)lo;
-}
-
-// Tiles of a head of keys in a sequence: block by block of 128 queries, the heads of the group side by side; a job is two neighbours.
-__device__ __forceinline__ bool find_job(const Args &a, unsigned index, unsigned kv_heads, fused::Job &job) {
-    const unsigned group = a.group;
-    const auto pairs = [=](unsigned queries) { return ((queries + fused::TILE - 1) / fused::TILE * group + 1) / 2; };
-    const int pair = a.masked && a.sequences <= LEVELLED ? find_levelled(a, index / kv_heads, pairs, job.q0, job.queries, job.k0, job.keys)
-                                                         : find_piece(a, index / kv_heads, pairs, job.q0, job.queries, job.k0, job.keys);
-    if (pair < 0) return false;
-    job.kv_head = (int)(index % kv_heads);
-    #pragma unroll
-    for (int w = 0; w < 2; w++) {
-        const unsigned tile = (unsigned)pair * 2 + w, block = tile / group;
-        job.head[w] = job.kv_head * (int)group + (int)(tile - block * group);
-        job.first[w] = (int)(block * fused::TILE);
-        const bool there = job.first[w] < job.queries;
-        job.steps[w] = there ? (job.end(w, a.masked) + (int)fused::TILE - 1) / (int)fused::TILE : 0;
-        if (!there) job.first[w] = -1;
     }
-    job.live = 1;
-    return true;
+    // The pair's number in its sequence, -1: there is none.
+    __device__ __forceinline__ int by_level(const Args &a, unsigned index, fused::Job &job) const {
+        if (index >= from(0)) return -1;
+        const unsigned lane = threadIdx.x % 32;
+        unsigned lo = 0, hi = most;             // the largest level that `index` is behind: from(lo) > index >= from(hi)
+        while (hi - lo > 1) { const unsigned mid = (lo + hi) / 2; if (from(mid) > index) lo = mid; else hi = mid; }
+        const unsigned rank = index - from(lo + 1);
+        unsigned mine = 0;
+        #pragma unroll
+        for (unsigned k = 0; k < 4; k++) mine += n[k] > lo;
+        unsigned sum = mine;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const unsigned u = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= (unsigned)o) sum += u; }
+        const int at = __ffs(__ballot_sync(0xffffffffu, sum > rank)) - 1;
+        unsigned left = rank - (sum - mine), which = 0;
+        #pragma unroll
+        for (unsigned k = 0; k < 4; k++) if (n[k] > lo) { if (left == 0) which = k; left--; }
+        const unsigned s = at * 4 + __shfl_sync(0xffffffffu, which, at);
+        job.q0 = clamped(a.q_starts, s, a.q_rows);
+        job.queries = clamped(a.q_starts, s + 1, a.q_rows) - job.q0;
+        job.k0 = clamped(a.kv_starts, s, a.kv_rows);
+        job.keys = max(0, clamped(a.kv_starts, s + 1, a.kv_rows) - job.k0);
+        return (int)lo;
+    }
+    __device__ __forceinline__ bool find(const Args &a, unsigned index, unsigned kv_heads, fused::Job &job) const {
+        const unsigned number = index / kv_heads;
+        const int pair = levelled ? by_level(a, number, job) : find_piece(a, number, [&](unsigned queries) { return pairs(a, queries); }, job.q0, job.queries, job.k0, job.keys);
+        if (pair < 0) return false;
+        job.kv_head = (int)(index - number * kv_heads);
+        job.block = (int)a.block;
+        #pragma unroll
+        for (int w = 0; w < 2; w++) {
+            job.first[w] = (pair * 2 + w) * (int)a.block;
+            const bool there = job.first[w] < job.queries;
+            job.steps[w] = there ? (job.end(w, a.masked) + (int)fused::TILE - 1) / (int)fused::TILE : 0;
+            if (!there) job.first[w] = -1;
+        }
+        job.live = 1;
+        return true;
+    }
+};
+// Where row r of a tile is in a matrix of rows and heads, in elements; -1: nowhere.
+__device__ __forceinline__ long long row_at(const Args &a, const fused::Job &job, int first, unsigned r, unsigned row_stride, unsigned head_stride) {
+    const unsigned q = r * a.part >> 16, h = r - q * a.group, query = (unsigned)first + q;
+    if (q >= a.block || (int)query >= job.queries) return -1;
+    return (long long)((unsigned long long)((unsigned)job.q0 + query) * row_stride + (unsigned long long)((unsigned)job.kv_head * a.group + h) * head_stride);
 }
 
 // A role's walk through the jobs.
@@ -344,11 +366,13 @@ struct Walk {
     }
 };
 
-// The warp that finds the work: the CTA's own first (`begin`, if there is such a job), then that of others that have not begun.
-__device__ __forceinline__ void deal(fused::Shared &sh, const Args &a, unsigned kv_heads, fused::Job begin, bool found) {
+// The warp that finds the work: the CTA's own first, then that of others that have not begun.
+__device__ __forceinline__ void deal(fused::Shared &sh, const Args &a, unsigned kv_heads) {
     using namespace fused;
     const unsigned lane = threadIdx.x % 32;
-    bool ok = true;
+    const Finder finder(a);
+    Job begin;
+    bool ok = true, found = finder.find(a, blockIdx.x, kv_heads, begin);
     unsigned index, slot = 0, lap = 0, asked = 0, wanted = 0;
     while (true) {
         if (found) {
@@ -367,7 +391,7 @@ __device__ __forceinline__ void deal(fused::Shared &sh, const Args &a, unsigned 
         tc::fence_proxy_async_smem();          // the answer has been read before the next one is written
         __syncwarp();
         if (!more) break;
-        found = find_job(a, index, kv_heads, begin);
+        found = finder.find(a, index, kv_heads, begin);
     }
     if (warp_wait(&sh.job_empty[slot], (lap & 1u) ^ 1u, &sh.gave_up) && lane == 0) { sh.jobs[slot].live = 0; tc::mbar_arrive(&sh.job_full[slot]); }
     __syncwarp();
@@ -400,16 +424,13 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
     }
     if (warp == 9) tc::tmem_alloc(&sh.tmem, 512u);
     attn::wait_for_previous_kernel();
-    Job begin;
-    bool found = false;
-    if (warp == 10) found = find_job(a, blockIdx.x, kv_heads, begin);       // beside the rest of the beginning
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
-    // Registers: 128 x (2 x 200 + 40 + 72) = 512 x 128, what the launch holds
+    // Registers: 128 x (2 x 192 + 40 + 88) = 512 x 128, what the launch holds
     if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const unsigned quarter = warp & 3u, row = quarter * 32u + lane, lanes = tmem + (quarter << 21);
         uint4 *const turn = reinterpret_cast<uint4 *>(smem + (2 * H::QUERIES + 2 * H::STAGES) * H::BYTES + quarter * 2048);
         unsigned done = 0;                             // a bit for each tile: the parity of its jobs
@@ -420,6 +441,9 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
             for (int w = 0; w < 2; w++) {
                 const int first = job.first[w], steps = job.steps[w];
                 if (first < 0) continue;
+                long long at[4];                       // the rows that the thread stores
+                #pragma unroll
+                for (unsigned x = 0; x < 4; x++) at[x] = row_at(a, job, first, quarter * 32 + x * 8 + (lane >> 2), a.out_row, a.out_head);
                 float factor = 0.f;
                 if (steps > 0) {
                     ok = ok && warp_wait(&sh.l_full[w], done >> w & 1u, gave_up, whole_job(steps)) && warp_wait(&sh.o_done[w], done >> w & 1u, gave_up);
@@ -427,8 +451,6 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                     tc::tc_fence_after();
                     factor = sh.factor[w][row];
                 }
-                char *const out = a.out + ((size_t)(job.q0 + first) * a.out_row + job.head[w] * a.out_head) * 2;
-                const int left = job.queries - first;
                 // 32 features at a time: a thread has its row's, and stores 16 bytes each of eight rows
                 #pragma unroll 1
                 for (int i = 0; i < DIM; i += 32) {
@@ -449,8 +471,8 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                     const unsigned f = i + (lane & 3u) * 8;
                     #pragma unroll
                     for (unsigned x = 0; x < 4; x++) {
-                        const unsigned r = x * 8 + (lane >> 2), q = quarter * 32 + r;
-                        if ((int)q < left && f < a.head_dim) *reinterpret_cast<uint4 *>(out + (q * a.out_row + f) * 2) = turn[r * 4 + ((lane & 3u) ^ (r >> 1 & 3u))];
+                        const unsigned r = x * 8 + (lane >> 2);
+                        if (at[x] >= 0 && f < a.head_dim) *reinterpret_cast<uint4 *>(a.out + (at[x] + f) * 2) = turn[r * 4 + ((lane & 3u) ^ (r >> 1 & 3u))];
                     }
                 }
             }
@@ -462,7 +484,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         bool ok = true;
         if (warp == 10) {
-            deal(sh, a, kv_heads, begin, found);
+            deal(sh, a, kv_heads);
         } else if (warp == 8) {
             unsigned stage = 0, lap = 0, q_uses[2] = {0, 0};
             for (Walk walk{&sh}; ok && walk.next(); walk.done()) {
@@ -485,10 +507,10 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                             ok = warp_wait(&sh.q_empty[b][w], (use & 1u) ^ 1u, gave_up);
                             q_uses[w]++;
                             if (ok && tc::elect_one()) {
-                                tc::mbar_arrive_expect_tx(&sh.q_full[b][w], H::BYTES);
+                                tc::mbar_arrive_expect_tx(&sh.q_full[b][w], H::CHUNKS * a.group * a.block * 128u);
                                 #pragma unroll
                                 for (int c = 0; c < H::CHUNKS; c++)
-                                    tc::tma_load_3d(q_at + (b * 2 + w) * H::BYTES + c * H::CHUNK_BYTES, &q_map, c * 64, job.head[w], job.q0 + job.first[w], &sh.q_full[b][w]);
+                                    tc::tma_load_3d(q_at + (b * 2 + w) * H::BYTES + c * H::CHUNK_BYTES, &q_map, c * 64, kv_head * (int)a.group, job.q0 + job.first[w], &sh.q_full[b][w]);
                             }
                             __syncwarp();
                         }
@@ -634,7 +656,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
             tc::tmem_dealloc(tmem, 512u);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int w = (int)(warp >> 2);
         const unsigned row = (warp & 3u) * 32u + lane, lanes = tmem + ((warp & 3u) << 21), s_at = lanes + H::S + w * 128, p_at = lanes + H::P + w * H::P_APART, o_at = lanes + H::O + w * DIM;
         const Pair scale2 = pair(a.scale, a.scale);
@@ -644,7 +666,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
             const Job &job = walk.job();
             const int first = job.first[w], steps = tc::uniform(job.steps[w]);
             if (first < 0 || steps == 0) continue;
-            const int query = first + (int)row;
+            const int query = first + (int)(row * a.part >> 16);
             const int seen = a.masked ? min(job.keys, query + job.behind() + 1) : job.keys;              // first key that the row does not see
             const int least_seen = __shfl_sync(0xffffffffu, seen, 0), most_seen = __shfl_sync(0xffffffffu, seen, 31);       // of the warp's rows
             float max = -INFINITY, sum = 0.f;
@@ -764,9 +786,6 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
     }
     if (warp == 9) tc::tmem_alloc(&sh.tmem, 512u);
     attn::wait_for_previous_kernel();
-    Job begin;
-    bool found = false;
-    if (warp == 10) found = find_job(a, blockIdx.x, kv_heads, begin);       // beside the rest of the beginning
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -778,45 +797,58 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
         const unsigned t = threadIdx.x & 127u, row0 = t >> 3, piece = t & 7u;
         unsigned q_uses[2] = {0, 0}, uses = 0;
         bool ok = true;
-        auto stage = [&](const char *from, size_t stride, int rows, unsigned to, unsigned long long *empty, unsigned parity, unsigned long long *full) {
-            float4 v[8][2];
-            #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int r = (int)row0 + 16 * i;
-                const bool in = r < rows && piece * 8 < a.head_dim;
-                const char *const p = from + (in ? (size_t)r * stride + piece * 8 : 0) * 4;
-                v[i][0] = in ? __ldg(reinterpret_cast<const float4 *>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                v[i][1] = in ? __ldg(reinterpret_cast<const float4 *>(p) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            if (!warp_wait(empty, parity, gave_up)) { ok = false; return; }
-            #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const unsigned r = row0 + 16 * i;
-                split::Pair x[4] = {split::pack(v[i][0].x, v[i][0].y), split::pack(v[i][0].z, v[i][0].w), split::pack(v[i][1].x, v[i][1].y), split::pack(v[i][1].z, v[i][1].w)};
-                char *const at = smem + (to - base) + r * 128 + ((piece ^ (r & 7u)) << 4);
-                *reinterpret_cast<uint4 *>(at) = make_uint4(split::take_part<0>(x[0]), split::take_part<0>(x[1]), split::take_part<0>(x[2]), split::take_part<0>(x[3]));
-                *reinterpret_cast<uint4 *>(at + H::BYTES) = make_uint4(split::take_part<1>(x[0]), split::take_part<1>(x[1]), split::take_part<1>(x[2]), split::take_part<1>(x[3]));
-                *reinterpret_cast<uint4 *>(at + 2 * H::BYTES) = make_uint4(split::take_part<2>(x[0]), split::take_part<2>(x[1]), split::take_part<2>(x[2]), split::take_part<2>(x[3]));
-            }
-            tc::fence_proxy_async_smem();
-            tc::mbar_arrive(full);
-        };
         for (Walk walk{&sh}; ok && walk.next(); walk.done()) {
             const Job &job = walk.job();
-            const int steps = job.both();
+            const int items = 2 * job.both();
+            // the queries of both tiles, then keys and values of each step; one place for all of them in the code
             #pragma unroll 1
-            for (int w = 0; w < 2 && ok; w++) {
-                if (job.steps[w] == 0) continue;
-                stage(a.q + ((size_t)(job.q0 + job.first[w]) * a.q_row + job.head[w] * a.q_head) * 4, a.q_row, job.queries - job.first[w], q_at + w * 3 * H::BYTES, &sh.q_empty[0][w],
-                      (q_uses[w] & 1u) ^ 1u, &sh.q_full[0][w]);
-                q_uses[w]++;
-            }
-            #pragma unroll 1
-            for (int i = 0; i < 2 * steps && ok; i++) {
-                const int key = i / 2 * (int)TILE;
-                if (i & 1) stage(a.v + ((size_t)(job.k0 + key) * a.v_row + job.kv_head * a.v_head) * 4, a.v_row, job.keys - key, v_at, &sh.v_empty[0], (uses & 1u) ^ 1u, &sh.v_full[0]);
-                else stage(a.k + ((size_t)(job.k0 + key) * a.k_row + job.kv_head * a.k_head) * 4, a.k_row, job.keys - key, k_at, &sh.k_empty[0], (uses & 1u) ^ 1u, &sh.k_full[0]);
-                uses += i & 1;
+            for (int i = items ? -2 : 0; i < items && ok; i++) {
+                const int w = i + 2, key = i / 2 * (int)TILE;
+                const bool value = i & 1;
+                unsigned to;
+                unsigned long long *empty, *full;
+                unsigned parity;
+                long long at[8];                       // of the thread's pieces, in elements; -1: zeros
+                if (i < 0) {
+                    if (job.steps[w] == 0) continue;
+                    #pragma unroll
+                    for (int x = 0; x < 8; x++) at[x] = row_at(a, job, job.first[w], row0 + 16 * x, a.q_row, a.q_head);
+                    to = q_at + w * 3 * H::BYTES;
+                    empty = &sh.q_empty[0][w]; full = &sh.q_full[0][w];
+                    parity = (q_uses[w]++ & 1u) ^ 1u;
+                } else {
+                    #pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        const int r = key + (int)row0 + 16 * x;
+                        at[x] = r < job.keys ? (long long)((unsigned long long)(unsigned)(job.k0 + r) * (value ? a.v_row : a.k_row) + (unsigned long long)(unsigned)job.kv_head * (value ? a.v_head : a.k_head)) : -1;
+                    }
+                    to = value ? v_at : k_at;
+                    empty = value ? &sh.v_empty[0] : &sh.k_empty[0]; full = value ? &sh.v_full[0] : &sh.k_full[0];
+                    parity = (uses & 1u) ^ 1u;
+                    uses += value;
+                }
+                const float *const from = reinterpret_cast<const float *>(i < 0 ? a.q : value ? a.v : a.k) + piece * 8;
+                float4 v[8][2];
+                #pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    const bool in = at[x] >= 0 && piece * 8 < a.head_dim;
+                    const float4 *const p = reinterpret_cast<const float4 *>(from + (in ? at[x] : 0));
+                    v[x][0] = in ? __ldg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    v[x][1] = in ? __ldg(p + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                ok = warp_wait(empty, parity, gave_up);
+                if (!ok) break;
+                #pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    const unsigned r = row0 + 16 * x;
+                    split::Pair y[4] = {split::pack(v[x][0].x, v[x][0].y), split::pack(v[x][0].z, v[x][0].w), split::pack(v[x][1].x, v[x][1].y), split::pack(v[x][1].z, v[x][1].w)};
+                    char *const put = smem + (to - base) + r * 128 + ((piece ^ (r & 7u)) << 4);
+                    *reinterpret_cast<uint4 *>(put) = make_uint4(split::take_part<0>(y[0]), split::take_part<0>(y[1]), split::take_part<0>(y[2]), split::take_part<0>(y[3]));
+                    *reinterpret_cast<uint4 *>(put + H::BYTES) = make_uint4(split::take_part<1>(y[0]), split::take_part<1>(y[1]), split::take_part<1>(y[2]), split::take_part<1>(y[3]));
+                    *reinterpret_cast<uint4 *>(put + 2 * H::BYTES) = make_uint4(split::take_part<2>(y[0]), split::take_part<2>(y[1]), split::take_part<2>(y[2]), split::take_part<2>(y[3]));
+                }
+                tc::fence_proxy_async_smem();
+                tc::mbar_arrive(full);
             }
         }
         __syncwarp();
@@ -825,7 +857,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
     } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         bool ok = true;
-        if (warp == 10) deal(sh, a, kv_heads, begin, found);
+        if (warp == 10) deal(sh, a, kv_heads);
         else if (warp == 9) {
             constexpr unsigned IDESC = 1u << 4 | 1u << 7 | 1u << 10 | (128u >> 4) << 24;               // sums fp32, operands bf16, 128 rows
             constexpr unsigned IDESC_S = IDESC | (128u >> 3) << 17, IDESC_O = IDESC | (64u >> 3) << 17 | 1u << 16;        // the second operand of PV: features contiguous
@@ -942,7 +974,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
             const Job &job = walk.job();
             const int first = job.first[w], steps = tc::uniform(job.steps[w]);
             if (first < 0) continue;
-            const int query = first + (int)row;
+            const int query = first + (int)(row * a.part >> 16);
             const int seen = a.masked ? min(job.keys, query + job.behind() + 1) : job.keys;              // first key that the row does not see
             const int least_seen = __shfl_sync(0xffffffffu, seen, 0), most_seen = __shfl_sync(0xffffffffu, seen, 31);       // of the warp's rows
             float max = -INFINITY, sum = 0.f, down = 0.f;
@@ -1032,11 +1064,12 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
                 if (lane == 0) tc::mbar_arrive(&sh.p_full[w][0]);
                 done++;
             }
+            long long at[8];                           // the rows that the thread stores
+            #pragma unroll
+            for (unsigned x = 0; x < 8; x++) at[x] = row_at(a, job, first, (warp & 3u) * 32 + x * 4 + (lane >> 3), a.out_row, a.out_head);
             if (steps > 0) add();
             tc::tc_fence_before();
             const float inv = !ok ? NAN : sum == 0.f ? 0.f : 1.f / sum;
-            char *const out = a.out + ((size_t)(job.q0 + first) * a.out_row + job.head[w] * a.out_head) * 4;
-            const int left = job.queries - first;
             // 32 features at a time: a thread has its row's, and stores 16 bytes each of four rows
             #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -1052,8 +1085,8 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
                 const unsigned f = h * 32 + (lane & 7u) * 4;
                 #pragma unroll
                 for (unsigned x = 0; x < 8; x++) {
-                    const unsigned r = x * 4 + (lane >> 3), q = (warp & 3u) * 32 + r;
-                    if ((int)q < left && f < a.head_dim) *reinterpret_cast<float4 *>(out + (q * a.out_row + f) * 4) = turn[r * 8 + ((lane & 7u) ^ (r & 7u))];
+                    const unsigned r = x * 4 + (lane >> 3);
+                    if (at[x] >= 0 && f < a.head_dim) *reinterpret_cast<float4 *>(a.out + (at[x] + f) * 4) = turn[r * 8 + ((lane & 7u) ^ (r & 7u))];
                 }
             }
         }
@@ -1073,10 +1106,10 @@ EncodeFn encode_fn() {
     }();
     return fn;
 }
-// (feature, head, row) of a 16-bit matrix, boxes of 64 features of 128 rows; zeros outside.
-bool encode(CUtensorMap *map, int type, const char *p, unsigned dim, unsigned heads, unsigned rows, size_t head, size_t row) {
+// (feature, head, row) of a 16-bit matrix, boxes of 64 features of some heads of some rows; zeros outside.
+bool encode(CUtensorMap *map, int type, const char *p, unsigned dim, unsigned heads, unsigned rows, size_t head, size_t row, unsigned box_heads) {
     const cuuint64_t dims[3] = {dim, heads, rows}, strides[2] = {head * 2, row * 2};
-    const cuuint32_t box[3] = {64, 1, fused::TILE}, one[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {64, box_heads, fused::TILE / box_heads}, one[3] = {1, 1, 1};
     return encode_fn()(map, type == ASPEN_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<char *>(p), dims, strides, box, one,
                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1084,7 +1117,7 @@ bool encode(CUtensorMap *map, int type, const char *p, unsigned dim, unsigned he
 // Jobs of a call, at most.
 unsigned long long jobs_of(const Args &a) {
     const unsigned long long kv_heads = a.heads / a.group, sequences = a.sequences < a.q_rows ? a.sequences : a.q_rows;
-    return ((a.q_rows / fused::TILE + sequences) * a.group + sequences) / 2 * kv_heads;
+    return (a.q_rows / a.block + 2 * sequences) / 2 * kv_heads;
 }
 cudaError_t launch_parts(const Args &a, cudaStream_t stream) {
     cudaError_t err = cudaFuncSetAttribute(prompt_parts, cudaFuncAttributeMaxDynamicSharedMemorySize, fused::Parts::SMEM);
@@ -1100,7 +1133,7 @@ cudaError_t launch_tiles(const Args &a, const CUtensorMap *maps, cudaStream_t st
 // False: not a call for these kernels.
 bool try_tiles(const Args &a, int type, cudaStream_t stream, cudaError_t *err) {
     // a row's largest score is its largest product only for a scale above 0
-    if (!a.kv_rows || !(a.scale > 0.f) || jobs_of(a) > 0x7fffffffull) return false;
+    if (!a.kv_rows || !(a.scale > 0.f) || a.group > fused::TILE || jobs_of(a) > 0x7fffffffull) return false;
     if (type == ASPEN_B200_FP32) {
         if (a.head_dim > 64) return false;
         *err = launch_parts(a, stream);
@@ -1109,8 +1142,8 @@ bool try_tiles(const Args &a, int type, cudaStream_t stream, cudaError_t *err) {
     if (a.head_dim > 128 || !encode_fn()) return false;
     const unsigned kv_heads = a.heads / a.group;
     CUtensorMap maps[3];
-    if (!encode(&maps[0], type, a.q, a.head_dim, a.heads, a.q_rows, a.q_head, a.q_row) || !encode(&maps[1], type, a.k, a.head_dim, kv_heads, a.kv_rows, a.k_head, a.k_row) ||
-        !encode(&maps[2], type, a.v, a.head_dim, kv_heads, a.kv_rows, a.v_head, a.v_row)) return false;
+    if (!encode(&maps[0], type, a.q, a.head_dim, a.heads, a.q_rows, a.q_head, a.q_row, a.group) || !encode(&maps[1], type, a.k, a.head_dim, kv_heads, a.kv_rows, a.k_head, a.k_row, 1) ||
+        !encode(&maps[2], type, a.v, a.head_dim, kv_heads, a.kv_rows, a.v_head, a.v_row, 1)) return false;
     if (a.head_dim <= 64) *err = type == ASPEN_B200_BF16 ? launch_tiles<ASPEN_B200_BF16, 64>(a, maps, stream) : launch_tiles<ASPEN_B200_FP16, 64>(a, maps, stream);
     else *err = type == ASPEN_B200_BF16 ? launch_tiles<ASPEN_B200_BF16, 128>(a, maps, stream) : launch_tiles<ASPEN_B200_FP16, 128>(a, maps, stream);
     return true;
@@ -1143,19 +1176,22 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     a.q_starts = p->q_starts;
     a.kv_starts = p->kv_starts;
     const size_t q_row = (size_t)p->heads * p->head_dim, kv_row = (size_t)p->kv_heads * p->head_dim;
-    a.q_row = attn::packed(p->q_row_stride, q_row);
-    a.q_head = attn::packed(p->q_head_stride, p->head_dim);
-    a.k_row = attn::packed(p->k_row_stride, kv_row);
-    a.k_head = attn::packed(p->k_head_stride, p->head_dim);
-    a.v_row = attn::packed(p->v_row_stride, kv_row);
-    a.v_head = attn::packed(p->v_head_stride, p->head_dim);
-    a.out_row = attn::packed(p->out_row_stride, q_row);
-    a.out_head = attn::packed(p->out_head_stride, p->head_dim);
+    a.q_row = (unsigned)attn::packed(p->q_row_stride, q_row);
+    a.q_head = (unsigned)attn::packed(p->q_head_stride, p->head_dim);
+    a.k_row = (unsigned)attn::packed(p->k_row_stride, kv_row);
+    a.k_head = (unsigned)attn::packed(p->k_head_stride, p->head_dim);
+    a.v_row = (unsigned)attn::packed(p->v_row_stride, kv_row);
+    a.v_head = (unsigned)attn::packed(p->v_head_stride, p->head_dim);
+    a.out_row = (unsigned)attn::packed(p->out_row_stride, q_row);
+    a.out_head = (unsigned)attn::packed(p->out_head_stride, p->head_dim);
     a.sequences = p->sequences;
     a.q_rows = p->q_rows;
     a.kv_rows = p->kv_rows;
     a.heads = p->heads;
     a.group = p->heads / p->kv_heads;
+    a.part = (65536 + a.group - 1) / a.group;
+    a.block = a.group > fused::TILE ? 0 : fused::TILE / a.group;
+    a.by_block = make_divisor(a.block);
     a.head_dim = p->head_dim;
     a.masked = p->masked != 0;
     a.scale = p->scale * 1.4426950408889634f;

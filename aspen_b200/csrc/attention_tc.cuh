@@ -1,9 +1,10 @@
 // Attention over whole prompts on tcgen05, 16-bit types, heads of up to 128 features.
 //
-// A CTA takes two tiles of 128 queries that see the same head of keys (two heads of a group, or two blocks of a head's queries) and walks their keys, 128 a step:
-//     S [128 queries x 128 keys] = Q K^T     both operands in shared memory, K-major, scores in TMEM
-//     P = exp2(S - max)                      a thread a query: its row of scores from TMEM to registers, weights back to TMEM as 16-bit pairs
-//     O [128 queries x features] += P V      P from TMEM, V as it lies in memory (features contiguous: the MN-major operand), sums in TMEM
+// A CTA takes two tiles of 128 rows that see the same head of keys and walks their keys, 128 a step.  A row is a query with one of the heads of the group: 128 / group queries to a
+// tile, so that short prompts fill it, too.
+//     S [128 rows x 128 keys] = Q K^T     both operands in shared memory, K-major, scores in TMEM
+//     P = exp2(S - max)                      a thread a row: its scores from TMEM to registers, weights back to TMEM as 16-bit pairs
+//     O [128 rows x features] += P V         P from TMEM, V as it lies in memory (features contiguous: the MN-major operand), sums in TMEM
 // The maximum is followed loosely: O and the sum are scaled again only when a row's maximum has grown by more than 2^8 (weights up to 256 are as exact as weights up to 1), so the
 // sums in TMEM are hardly ever read before the end.
 //
@@ -57,15 +58,15 @@ struct Parts {
     static __device__ __forceinline__ unsigned second(int p) { return 0x010210u >> (4 * p) & 15u; }
 };
 
-// A CTA's work: two tiles of queries of one sequence and one head of keys.
+// A CTA's work: two tiles of one sequence and one head of keys.  A tile is `block` queries with all heads of the group: row r is query first + r / group, head r % group.
 struct Job {
     int q0, queries, k0, keys;
-    int kv_head, head[2];
+    int kv_head, block;
     int first[2], steps[2];                        // first query of a tile, -1: no such tile; steps of 128 keys
     int live;                                      // 0: there are no more
     __device__ __forceinline__ int both() const { return max(steps[0], steps[1]); }
     __device__ __forceinline__ int behind() const { return keys - queries; }
-    __device__ __forceinline__ int end(int w, int masked) const { return masked ? max(0, min(keys, min(queries, first[w] + (int)TILE) + behind())) : keys; }
+    __device__ __forceinline__ int end(int w, int masked) const { return masked ? max(0, min(keys, min(queries, first[w] + block) + behind())) : keys; }
 };
 constexpr unsigned JOBS = 2;                       // the one in work and the next
 

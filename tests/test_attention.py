@@ -413,7 +413,7 @@ def seen_by(n, m, masked):
 PROMPTS = [  # heads, kv_heads, dim, lengths of queries, lengths of keys
     (1, 1, 8, [1], [1]), (12, 12, 64, [37], [37]), (4, 2, 64, [1, 64, 65, 0, 128, 200], [1, 64, 65, 0, 128, 200]), (8, 2, 128, [130, 3, 257], [130, 3, 257]),
     (7, 1, 80, [100, 1], [300, 129]), (4, 4, 96, [5, 70, 3], [0, 20, 64]), (2, 1, 256, [90, 33], [90, 33]), (3, 3, 32, [511], [511]), (6, 2, 128, [129, 1, 1], [1000, 127, 128]),
-    (2, 2, 64, [300], [1100])]
+    (2, 2, 64, [300], [1100]), (24, 2, 64, [70, 9], [75, 200]), (128, 1, 64, [3, 1], [200, 5]), (130, 1, 64, [2], [70]), (48, 1, 128, [4, 130], [4, 130])]
 
 
 @pytest.mark.gpu
