@@ -35,35 +35,37 @@ __device__ __forceinline__ int clamped(const int *starts, unsigned i, unsigned r
 
 // Piece `index` of all sequences, `pieces(queries)` of one, counted from the first sequence; a sequence's last one first, because with a mask it has most keys.
 // Every warp finds it for itself, 32 sequences a turn.  Returns the piece's number in its sequence, -1: there are not so many.
+struct Place { unsigned sequence = 0; unsigned long long before = 0; };       // where a search ended: at 32 sequences, and the pieces before them
 template <typename Pieces>
-__device__ __forceinline__ int find_piece(const Args &a, unsigned index, const Pieces &pieces, int &q_first, int &queries, int &k_first, int &keys) {
+__device__ __forceinline__ int find_piece(const Args &a, unsigned index, Place &from, const Pieces &pieces, int &q_first, int &queries, int &k_first, int &keys) {
     const unsigned lane = threadIdx.x % 32;
-    unsigned long long before = 0;
-    for (unsigned s0 = 0; s0 < a.sequences; s0 += 32) {
-        const unsigned s = s0 + lane;
+    if (index < from.before) from = Place();
+    for (; from.sequence < a.sequences; from.sequence += 32) {
+        const unsigned s = from.sequence + lane;
         int q0 = 0, q1 = 0;
         if (s < a.sequences) { q0 = clamped(a.q_starts, s, a.q_rows); q1 = max(q0, clamped(a.q_starts, s + 1, a.q_rows)); }
         const unsigned n = pieces((unsigned)(q1 - q0));
         unsigned long long sum = n;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const unsigned long long u = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= (unsigned)o) sum += u; }
-        const unsigned here = __ballot_sync(0xffffffffu, before + sum > index);
+        const unsigned here = __ballot_sync(0xffffffffu, from.before + sum > index);
         if (here) {
             const int at = __ffs(here) - 1;
-            const unsigned rank = (unsigned)(before + sum - 1 - index);           // of lane `at`: n - 1 for the first index of its sequence, 0 for the last
+            const unsigned rank = (unsigned)(from.before + sum - 1 - index);      // of lane `at`: n - 1 for the first index of its sequence, 0 for the last
             q_first = __shfl_sync(0xffffffffu, q0, at);
             queries = __shfl_sync(0xffffffffu, q1, at) - q_first;
-            const unsigned mine = s0 + at;
+            const unsigned mine = from.sequence + at;
             k_first = clamped(a.kv_starts, mine, a.kv_rows);
             keys = max(0, clamped(a.kv_starts, mine + 1, a.kv_rows) - k_first);
             return (int)__shfl_sync(0xffffffffu, rank, at);
         }
-        before += __shfl_sync(0xffffffffu, sum, 31);
+        from.before += __shfl_sync(0xffffffffu, sum, 31);
     }
     return -1;
 }
 __device__ __forceinline__ bool find_block(const Args &a, unsigned index, unsigned size, Block &b) {
-    const int i = find_piece(a, index, [=](unsigned queries) { return (queries + size - 1) / size; }, b.q0, b.queries, b.k0, b.keys);
+    Place from;
+    const int i = find_piece(a, index, from, [=](unsigned queries) { return (queries + size - 1) / size; }, b.q0, b.queries, b.k0, b.keys);
     b.first = i * (int)size;
     return i >= 0;
 }
@@ -284,6 +286,7 @@ cudaError_t launch_rows(const Args &a, cudaStream_t stream) {
 struct Finder {
     unsigned n[4], most;
     bool levelled;
+    Place place;
     static __device__ __forceinline__ unsigned pairs(const Args &a, unsigned queries) { return (div_by(queries + a.block - 1, a.by_block) + 1) / 2; }
     __device__ __forceinline__ Finder(const Args &a) : most(0), levelled(a.masked && a.sequences <= 128) {
         if (!levelled) return;
@@ -326,9 +329,9 @@ struct Finder {
         job.keys = max(0, clamped(a.kv_starts, s + 1, a.kv_rows) - job.k0);
         return (int)lo;
     }
-    __device__ __forceinline__ bool find(const Args &a, unsigned index, unsigned kv_heads, fused::Job &job) const {
+    __device__ __forceinline__ bool find(const Args &a, unsigned index, unsigned kv_heads, fused::Job &job) {
         const unsigned number = index / kv_heads;
-        const int pair = levelled ? by_level(a, number, job) : find_piece(a, number, [&](unsigned queries) { return pairs(a, queries); }, job.q0, job.queries, job.k0, job.keys);
+        const int pair = levelled ? by_level(a, number, job) : find_piece(a, number, place, [&](unsigned queries) { return pairs(a, queries); }, job.q0, job.queries, job.k0, job.keys);
         if (pair < 0) return false;
         job.kv_head = (int)(index - number * kv_heads);
         job.block = (int)a.block;
@@ -370,7 +373,7 @@ struct Walk {
 __device__ __forceinline__ void deal(fused::Shared &sh, const Args &a, unsigned kv_heads) {
     using namespace fused;
     const unsigned lane = threadIdx.x % 32;
-    const Finder finder(a);
+    Finder finder(a);
     Job begin;
     bool ok = true, found = finder.find(a, blockIdx.x, kv_heads, begin);
     unsigned index, slot = 0, lap = 0, asked = 0, wanted = 0;
@@ -1134,6 +1137,10 @@ cudaError_t launch_tiles(const Args &a, const CUtensorMap *maps, cudaStream_t st
 bool try_tiles(const Args &a, int type, cudaStream_t stream, cudaError_t *err) {
     // a row's largest score is its largest product only for a scale above 0
     if (!a.kv_rows || !(a.scale > 0.f) || a.group > fused::TILE || jobs_of(a) > 0x7fffffffull) return false;
+    // Short sequences, going by the mean: a job of one step takes 4 us (fp32 5), and a block of prompt_rows 1.2 (3), several at once on an SM.  12 heads of 64, bf16 and fp32, 32 prompts of 60
+    // tokens 10.5 and 14.5 us (in tiles 14 and 22), of 100 tokens 12 and 35 (14 and 28).  Where one sequence of a few is long and the others short, the blocks take up to three times as long,
+    // of 4096 rows at most.
+    if (a.group <= 2 && a.q_rows <= 4096 && a.q_rows <= 64ull * a.sequences && a.kv_rows <= 64ull * a.sequences) return false;
     if (type == ASPEN_B200_FP32) {
         if (a.head_dim > 64) return false;
         *err = launch_parts(a, stream);
