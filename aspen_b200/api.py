@@ -24,7 +24,7 @@ LDATA_FIELDS = ("type", "act", "H", "W", "stride", "tile_h", "tile_w", "num_nins
                 "parent0", "parent1", "mem_size")
 # ASPEN_B200_TYPE, ASPEN_B200_CACHE_* (include/aspen_b200.h)
 FP32, BF16, FP16 = range(3)
-CACHE_BAD_INDEX, CACHE_NO_PAGES, CACHE_TOO_LONG = 1, 2, 4
+CACHE_BAD_INDEX, CACHE_NO_PAGES, CACHE_TOO_LONG, CACHE_REFUSED = 1, 2, 4, 8
 
 NINST_FIELDS = ("pos_h", "pos_w", "tile_h", "tile_w", "num_parents", "num_children", "num_input_pos")
 

@@ -65,8 +65,8 @@ int check_device(const Named *list, unsigned n, const char *what) {
         cudaPointerAttributes a;
         err = cudaPointerGetAttributes(&a, list[i].p);
         if (err != cudaSuccess) break;
-        if (a.type == cudaMemoryTypeUnregistered || !a.devicePointer) { ASPEN_ERR("%s: %s is not memory that the GPU can read\n", what, list[i].name); return -1; }
-        if (a.type == cudaMemoryTypeDevice && a.device != dev) {
+        if (a.type != cudaMemoryTypeDevice) { ASPEN_ERR("%s: %s is not device memory\n", what, list[i].name); return -1; }
+        if (a.device != dev) {
             ASPEN_ERR("%s: %s is memory of device %d, the current one is %d\n", what, list[i].name, a.device, dev);
             return -1;
         }

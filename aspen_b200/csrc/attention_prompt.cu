@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
     const int last = min(b.queries, b.first + R::QUERIES) - 1;
     const int end = a.masked ? min(b.keys, last + behind + 1) : b.keys;
     const int row0 = b.first + (int)warp * 16 + (int)g, row8 = row0 + 8;
-    const char *const k = a.k + ((size_t)b.k0 * a.k_row + kv_head * a.k_head) * SIZE, *const v = a.v + ((size_t)b.k0 * a.v_row + kv_head * a.v_head) * SIZE;
+    const char *const k = a.k + ((size_t)b.k0 * a.k_row + (size_t)kv_head * a.k_head) * SIZE, *const v = a.v + ((size_t)b.k0 * a.v_row + (size_t)kv_head * a.v_head) * SIZE;
     auto fetch = [&](int tile, int stage) {
         char *const at = smem + stage * R::STAGE;
         constexpr int PER_ROW = R::BYTES / 16;
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
     const int tiles = end > 0 ? (end + R::KEYS - 1) / R::KEYS : 0;
     if (tiles > 0) fetch(0, 0);
     // queries, rows g and g + 8 of the warp's 16
-    const char *const q = a.q + (size_t)b.q0 * a.q_row * SIZE + head * a.q_head * SIZE;
+    const char *const q = a.q + ((size_t)b.q0 * a.q_row + (size_t)head * a.q_head) * SIZE;
     char *const own = smem + 2 * R::STAGE + warp * 16 * R::KPITCH;
     uint4 held[R::HELD ? R::PIECES * 2 : 1];
     #pragma unroll
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
         const int row = h ? row8 : row0;
         if (row >= b.queries) continue;
         const float inv = sum[h] == 0.f ? 0.f : 1.f / sum[h];
-        char *const out = a.out + ((size_t)(b.q0 + row) * a.out_row + head * a.out_head) * SIZE;
+        char *const out = a.out + ((size_t)(b.q0 + row) * a.out_row + (size_t)head * a.out_head) * SIZE;
         // column n = 2 t + c of tile j holds the value j of piece n
         constexpr int PER = TYPE == ASPEN_B200_FP32 ? 4 : 8;
         #pragma unroll

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(BOOK) extend_kernel(const Pool pool, const Spa
         __syncthreads();
     }
     if (refused) {
-        if (threadIdx.x == 0) atomicOr(pool.at.status, refused);
+        if (threadIdx.x == 0) atomicOr(pool.at.status, refused | ASPEN_B200_CACHE_REFUSED);
         return;
     }
     for (unsigned i = threadIdx.x; i < total; i += BOOK) {
@@ -392,7 +392,8 @@ struct New {
 __global__ void __launch_bounds__(COPY) append_kernel(const Pages at /* strides in vectors */, const New n) {
     const unsigned lane = threadIdx.x % 32, r = blockIdx.x * (COPY / 32) + threadIdx.x / 32;
     wait_for_previous_kernel();
-    if (r >= n.rows) return;
+    // behind an extend that was refused the last places of a sequence are not the new tokens'
+    if (r >= n.rows || *reinterpret_cast<volatile int *>(at.status) & ASPEN_B200_CACHE_REFUSED) return;
     unsigned e = r;
     int begin = (int)r, end = (int)r + 1;
     if (n.starts) {

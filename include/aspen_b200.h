@@ -285,6 +285,7 @@ int aspen_b200_matmul_noalloc(const float *x_dev, const float *w_dev, const floa
  * What follows from device memory (lengths, indices) is therefore checked on the device: nothing out of range is read or written, and the cache's status word
  * says that it happened.  Calls on several streams may run at once if they share no memory that one of them writes; each needs a workspace of its own
  * while it runs, and so does a captured graph.
+ * While the resident kernel of a dse group in service mode has the SMs, they wait for it as any kernel does.
  * Return values: 0, -1 bad arguments, -2 too large, -3 CUDA error or no sm_100 device (see aspen_b200_last_error); on failure nothing is enqueued but where
  * a CUDA launch itself fails.
  *
@@ -329,6 +330,7 @@ typedef struct {
 #define ASPEN_B200_CACHE_BAD_INDEX 1    /* a sequence or page that does not exist, named twice where it must not be, or a fork onto one that is not empty */
 #define ASPEN_B200_CACHE_NO_PAGES 2     /* the pool has too few free pages, or one sequence asked for more than 2^21 at once */
 #define ASPEN_B200_CACHE_TOO_LONG 4     /* a sequence would need more than max_pages pages */
+#define ASPEN_B200_CACHE_REFUSED 8      /* an extend has changed nothing; until this bit is cleared, append writes nothing */
 
 /* Bytes of workspace of extend, fork (entries: how many are given) and compact (0); 0 on bad arguments. */
 size_t aspen_b200_cache_workspace(const aspen_b200_cache_t *cache, unsigned int entries);

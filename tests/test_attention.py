@@ -243,6 +243,9 @@ def test_host_memory_is_refused():
     host, dev = torch.zeros(1 << 16, dtype=torch.uint8), torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
     p = (host.data_ptr() + 15) // 16 * 16
     L, d = api.lib(), dev.data_ptr()
+    pinned = torch.zeros(1 << 12, dtype=torch.uint8, pin_memory=True)
+    assert L.aspen_b200_attention_prompt(C.byref(api.PromptArgs(type=api.FP16, heads=1, kv_heads=1, head_dim=8, scale=1.0, sequences=1, q_rows=1, kv_rows=1, q_starts=d, kv_starts=d,
+                                                               q=pinned.data_ptr(), k=d, v=d, out=d + 4096)), None) == -1
     good = dict(type=api.FP16, heads=1, kv_heads=1, head_dim=8, scale=1.0, sequences=1, q_rows=1, kv_rows=1, q_starts=d, kv_starts=d, q=d, k=d, v=d, out=d + 4096)
     for name in ("q", "k", "v", "out", "q_starts", "kv_starts"):
         assert L.aspen_b200_attention_prompt(C.byref(api.PromptArgs(**{**good, name: p})), None) == -1, name
@@ -508,6 +511,73 @@ def test_scores_far_apart_and_equal_ones(kind):
     check(got, want, away, size, kind)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30])
+def test_any_finite_scale(scale, kind):
+    rng = np.random.default_rng(23)
+    n = 150
+    q, k, v = (rounded(rng.standard_normal((n, 2, 64)), kind) for _ in range(3))
+    got = prompt(*(to_device(a, kind) for a in (q, k, v)), [0, n], [0, n], kind, True, scale)
+    want, away, size = attend(q, k, v, scale, seen_by(n, n, True))
+    check(got, want, away, size, kind)
+    pool = Pool(kind, 2, 64, 16, 12, 1, 11)
+    pool.fill([n], rng)
+    want, away, size = decode_want(pool, q[:1], [0], [n], scale)
+    check(decode(pool, to_device(q[:1], kind), 2, scale=scale), want, away, size, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 256])
+def test_heads_more_than_32_bits_of_elements_apart(dim):
+    """Keys, values and outputs with one head behind the other, 2^29 - 64 elements apart: head 9 lies behind 2^32."""
+    import torch
+    rng = np.random.default_rng(24)
+    n, heads, apart, kind = 100, 10, 2 ** 29 - 64, api.BF16
+    q, k = (rounded(rng.standard_normal((n, heads, dim)), kind) for _ in range(2))
+    flat = torch.zeros((heads - 1) * apart + n * dim, dtype=torch.bfloat16, device="cuda")
+    out = torch.zeros_like(flat)
+    for h in range(heads):
+        flat[h * apart:h * apart + n * dim] = to_device(k[:, h], kind).reshape(-1)
+    dq, starts = to_device(q, kind), ints([0, n])
+    api.attention_prompt(api.PromptArgs(type=kind, heads=heads, kv_heads=heads, head_dim=dim, masked=1, scale=0.1, sequences=1, q_rows=n, kv_rows=n, q_starts=starts.data_ptr(),
+                                        kv_starts=starts.data_ptr(), q=dq.data_ptr(), k=flat.data_ptr(), v=flat.data_ptr(), out=out.data_ptr(), k_row_stride=dim, k_head_stride=apart,
+                                        v_row_stride=dim, v_head_stride=apart, out_row_stride=dim, out_head_stride=apart))
+    torch.cuda.synchronize()
+    want, away, size = attend(q, k, k, 0.1, seen_by(n, n, True))
+    got = torch.stack([out[h * apart:h * apart + n * dim].view(n, dim) for h in range(heads)], 1)
+    check(got, want, away, size, kind)
+    del flat, out
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dim", [(api.FP32, 64), (api.FP32, 128), (api.BF16, 64), (api.FP16, 128)], ids=str)
+def test_a_captured_prompt_follows_the_starts(kind, dim):
+    """Captured once on a stream of its own, replayed with other sequences in the same rows."""
+    import torch
+    rng = np.random.default_rng(25)
+    n, heads, kv = 400, 4, 2
+    q, k, v = (rounded(rng.standard_normal((n, h, dim)), kind) for h in (heads, kv, kv))
+    dq, dk, dv = (to_device(a, kind) for a in (q, k, v))
+    out, starts = torch.full_like(dq, math.nan), ints([0] * 6)
+    args = api.PromptArgs(type=kind, heads=heads, kv_heads=kv, head_dim=dim, masked=1, scale=0.2, sequences=5, q_rows=n, kv_rows=n, q_starts=starts.data_ptr(), kv_starts=starts.data_ptr(),
+                          q=dq.data_ptr(), k=dk.data_ptr(), v=dv.data_ptr(), out=out.data_ptr())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        api.attention_prompt(args, torch.cuda.current_stream().cuda_stream)
+    for ends in ([400, 400, 400, 400, 400], [1, 130, 131, 131, 390], [0, 0, 0, 0, 257]):
+        out.fill_(math.nan)
+        starts.copy_(ints([0] + ends))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip([0] + ends, ends):
+            want, away, size = attend(q[a:b], k[a:b], v[a:b], 0.2, seen_by(b - a, b - a, True))
+            check(out[a:b], want, away, size, kind)
+        assert out[ends[-1]:].isnan().all()
+
+
 # ---- the pool's books --------------------------------------------------------------------------------------------------------
 
 class Books:
@@ -535,7 +605,7 @@ class Books:
         free = self.free_pages()
         if not why and need > len(free):
             why = api.CACHE_NO_PAGES
-        self.status |= why
+        self.status |= why | (api.CACHE_REFUSED if why else 0)
         if why:
             return
         for s, n in zip(slots, counts):
@@ -682,6 +752,29 @@ def test_append_leaves_out_rows_that_have_no_place():
     want[0, 0, 0, 0], want[0, 0, 0, 1], want[0, 3, 0, 3] = one, one, one
     np.testing.assert_array_equal(got, want)
     assert pool.status.item() == api.CACHE_BAD_INDEX
+
+
+@pytest.mark.gpu
+def test_append_behind_a_refused_extend_writes_nothing():
+    """The last places of the sequence are old tokens' then."""
+    import torch
+    pool = Pool(api.BF16, 1, 16, 4, 2, 2, 3)
+    pool.fill([7], np.random.default_rng(22))
+    before, starts, slots = bits(pool.k), ints([0, 2]), ints([0])
+    k = torch.ones(2, 1, 16, dtype=torch.bfloat16, device="cuda")
+    rows = api.AppendArgs(k=k.data_ptr(), v=k.data_ptr(), slots=slots.data_ptr(), starts=starts.data_ptr(), entries=1, rows=2)
+    pool.cache.extend(slots.data_ptr(), starts.data_ptr(), 1, *pool.space(1))
+    pool.cache.append(0, rows)
+    torch.cuda.synchronize()
+    assert pool.status.item() == api.CACHE_NO_PAGES | api.CACHE_REFUSED and pool.lengths[0].item() == 7
+    np.testing.assert_array_equal(bits(pool.k), before)
+    pool.status.zero_()
+    one = ints([0, 1])
+    pool.cache.extend(slots.data_ptr(), one.data_ptr(), 1, *pool.space(1))
+    pool.cache.append(0, api.AppendArgs(k=k.data_ptr(), v=k.data_ptr(), slots=slots.data_ptr(), starts=one.data_ptr(), entries=1, rows=1))
+    torch.cuda.synchronize()
+    page = pool.table[0, 1].item()
+    assert pool.status.item() == 0 and (pool.k[0, page, 0, 3] == 1).all()
 
 
 @pytest.mark.gpu
