@@ -765,6 +765,33 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
 
 // ---- fp32 on tcgen05: operands of three bf16 parts each (attention_tc.cuh) ----
 
+// A tile of 128 rows of up to 64 features by 128 threads, a thread eight features of every 16th row: read, and written as three parts.
+template <typename At>
+__device__ __forceinline__ void read_tile(const float *from, unsigned features, unsigned t, float4 (&v)[8][2], const At &place) {
+    const unsigned f = (t & 7u) * 8;
+    #pragma unroll
+    for (int x = 0; x < 8; x++) {
+        const long long at = place((t >> 3) + 16 * x);         // in elements; -1: zeros
+        const bool in = at >= 0 && f < features;
+        const float4 *const p = reinterpret_cast<const float4 *>(from + (in ? at + f : 0));
+        v[x][0] = in ? __ldg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[x][1] = in ? __ldg(p + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+}
+__device__ __forceinline__ void split_tile(const float4 (&v)[8][2], char *to, unsigned t) {
+    constexpr int BYTES = fused::Parts::BYTES;
+    #pragma unroll
+    for (int x = 0; x < 8; x++) {
+        const unsigned r = (t >> 3) + 16 * x;
+        split::Pair y[4] = {split::pack(v[x][0].x, v[x][0].y), split::pack(v[x][0].z, v[x][0].w), split::pack(v[x][1].x, v[x][1].y), split::pack(v[x][1].z, v[x][1].w)};
+        char *const put = to + r * 128 + (((t ^ r) & 7u) << 4);
+        *reinterpret_cast<uint4 *>(put) = make_uint4(split::take_part<0>(y[0]), split::take_part<0>(y[1]), split::take_part<0>(y[2]), split::take_part<0>(y[3]));
+        *reinterpret_cast<uint4 *>(put + BYTES) = make_uint4(split::take_part<1>(y[0]), split::take_part<1>(y[1]), split::take_part<1>(y[2]), split::take_part<1>(y[3]));
+        *reinterpret_cast<uint4 *>(put + 2 * BYTES) = make_uint4(split::take_part<2>(y[0]), split::take_part<2>(y[1]), split::take_part<2>(y[2]), split::take_part<2>(y[3]));
+    }
+    tc::fence_proxy_async_smem();
+}
+
 __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, unsigned kv_heads) {
     using namespace fused;
     typedef Parts H;
@@ -780,7 +807,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
         tc::mbar_init(&sh.answered, 1u); tc::mbar_init(&sh.wanted, 1u);
         for (unsigned i = 0; i < JOBS; i++) { tc::mbar_init(&sh.job_full[i], 1u); tc::mbar_init(&sh.job_empty[i], 13u); }
         for (int w = 0; w < 2; w++) {
-            tc::mbar_init(&sh.q_full[0][w], 128u); tc::mbar_init(&sh.q_empty[0][w], 1u);
+            tc::mbar_init(&sh.q_full[0][w], 128u);
             tc::mbar_init(&sh.s_full[w], 1u); tc::mbar_init(&sh.o_full[w], 1u); tc::mbar_init(&sh.p_full[w][0], 4u);
         }
         tc::mbar_init(&sh.k_full[0], 128u); tc::mbar_init(&sh.k_empty[0], 1u); tc::mbar_init(&sh.v_full[0], 128u); tc::mbar_init(&sh.v_empty[0], 1u);
@@ -796,62 +823,27 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
     // Registers: 128 x (2 x 168 + 64 + 112) = 512 x 128, what the launch holds
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-        // Splits queries, keys and values: a thread eight features of every 16th row.
-        const unsigned t = threadIdx.x & 127u, row0 = t >> 3, piece = t & 7u;
-        unsigned q_uses[2] = {0, 0}, uses = 0;
+        // Splits keys and values.
+        const unsigned t = threadIdx.x & 127u;
+        unsigned uses = 0;
         bool ok = true;
         for (Walk walk{&sh}; ok && walk.next(); walk.done()) {
             const Job &job = walk.job();
             const int items = 2 * job.both();
-            // the queries of both tiles, then keys and values of each step; one place for all of them in the code
             #pragma unroll 1
-            for (int i = items ? -2 : 0; i < items && ok; i++) {
-                const int w = i + 2, key = i / 2 * (int)TILE;
+            for (int i = 0; i < items && ok; i++) {
                 const bool value = i & 1;
-                unsigned to;
-                unsigned long long *empty, *full;
-                unsigned parity;
-                long long at[8];                       // of the thread's pieces, in elements; -1: zeros
-                if (i < 0) {
-                    if (job.steps[w] == 0) continue;
-                    #pragma unroll
-                    for (int x = 0; x < 8; x++) at[x] = row_at(a, job, job.first[w], row0 + 16 * x, a.q_row, a.q_head);
-                    to = q_at + w * 3 * H::BYTES;
-                    empty = &sh.q_empty[0][w]; full = &sh.q_full[0][w];
-                    parity = (q_uses[w]++ & 1u) ^ 1u;
-                } else {
-                    #pragma unroll
-                    for (int x = 0; x < 8; x++) {
-                        const int r = key + (int)row0 + 16 * x;
-                        at[x] = r < job.keys ? (long long)((unsigned long long)(unsigned)(job.k0 + r) * (value ? a.v_row : a.k_row) + (unsigned long long)(unsigned)job.kv_head * (value ? a.v_head : a.k_head)) : -1;
-                    }
-                    to = value ? v_at : k_at;
-                    empty = value ? &sh.v_empty[0] : &sh.k_empty[0]; full = value ? &sh.v_full[0] : &sh.k_full[0];
-                    parity = (uses & 1u) ^ 1u;
-                    uses += value;
-                }
-                const float *const from = reinterpret_cast<const float *>(i < 0 ? a.q : value ? a.v : a.k) + piece * 8;
+                const int key = i / 2 * (int)TILE;
                 float4 v[8][2];
-                #pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    const bool in = at[x] >= 0 && piece * 8 < a.head_dim;
-                    const float4 *const p = reinterpret_cast<const float4 *>(from + (in ? at[x] : 0));
-                    v[x][0] = in ? __ldg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    v[x][1] = in ? __ldg(p + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-                ok = warp_wait(empty, parity, gave_up);
+                read_tile(reinterpret_cast<const float *>(value ? a.v : a.k), a.head_dim, t, v, [&](unsigned row) {
+                    const int r = key + (int)row;
+                    return r < job.keys ? (long long)((unsigned long long)(unsigned)(job.k0 + r) * (value ? a.v_row : a.k_row) + (unsigned long long)(unsigned)job.kv_head * (value ? a.v_head : a.k_head)) : -1ll;
+                });
+                ok = warp_wait(value ? &sh.v_empty[0] : &sh.k_empty[0], (uses & 1u) ^ 1u, gave_up);
                 if (!ok) break;
-                #pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    const unsigned r = row0 + 16 * x;
-                    split::Pair y[4] = {split::pack(v[x][0].x, v[x][0].y), split::pack(v[x][0].z, v[x][0].w), split::pack(v[x][1].x, v[x][1].y), split::pack(v[x][1].z, v[x][1].w)};
-                    char *const put = smem + (to - base) + r * 128 + ((piece ^ (r & 7u)) << 4);
-                    *reinterpret_cast<uint4 *>(put) = make_uint4(split::take_part<0>(y[0]), split::take_part<0>(y[1]), split::take_part<0>(y[2]), split::take_part<0>(y[3]));
-                    *reinterpret_cast<uint4 *>(put + H::BYTES) = make_uint4(split::take_part<1>(y[0]), split::take_part<1>(y[1]), split::take_part<1>(y[2]), split::take_part<1>(y[3]));
-                    *reinterpret_cast<uint4 *>(put + 2 * H::BYTES) = make_uint4(split::take_part<2>(y[0]), split::take_part<2>(y[1]), split::take_part<2>(y[2]), split::take_part<2>(y[3]));
-                }
-                tc::fence_proxy_async_smem();
-                tc::mbar_arrive(full);
+                uses += value;
+                split_tile(v, smem + ((value ? v_at : k_at) - base), t);
+                tc::mbar_arrive(value ? &sh.v_full[0] : &sh.k_full[0]);
             }
         }
         __syncwarp();
@@ -878,9 +870,8 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
                 walk.done();
             };
             // Six of the nine products of parts, smallest first: what the sums cut off then is small.  In a loop: the code of all of them is more than is fetched in time.
-            auto scores = [&](int w, bool first, bool last) {
-                if (first) ok = ok && warp_wait(&sh.q_full[0][w], q_uses[w] & 1u, gave_up);
-                if (last) q_uses[w]++;
+            auto scores = [&](int w, bool first) {
+                if (first) ok = ok && warp_wait(&sh.q_full[0][w], q_uses[w]++ & 1u, gave_up);
                 if (!ok) return;
                 tc::tc_fence_after();
                 const unsigned q = q_at + w * 3 * H::BYTES, d = tmem + w * 256;
@@ -892,7 +883,6 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
                         for (int k = 0; k < 4; k++) mma_ss(d, x + k * 2, y + k * 2, IDESC_S, p + k);
                     }
                     tc::tc_commit(&sh.s_full[w]);
-                    if (last) tc::tc_commit(&sh.q_empty[0][w]);
                 }
                 __syncwarp();
             };
@@ -915,7 +905,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
                 if (!begun) {
                     ok = warp_wait(&sh.k_full[0], k_uses++ & 1u, gave_up);
                     #pragma unroll 1
-                    for (int w = 0; w < 2; w++) if (next[w]) scores(w, true, next[w] == 1);
+                    for (int w = 0; w < 2; w++) if (next[w]) scores(w, true);
                     if (!ok) break;
                     release(&sh.k_empty[0]);
                 }
@@ -932,22 +922,25 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
                     begun = turn && more;
                     ok = warp_wait(&sh.v_full[0], v_uses++ & 1u, gave_up);
                     bool keys = false;
+                    // the next job's first scores wait for its queries, which are split when these tiles' outputs have been written
                     #pragma unroll 1
-                    for (int w = 0; w < 2; w++) {
-                        if (ok && j < steps[w]) {
+                    for (int i = 0; i < 4 && ok; i++) {
+                        const int w = turn ? i & 1 : i >> 1;
+                        if (turn && i == 2) release(&sh.v_empty[0]);
+                        if (!(turn ? i >> 1 : i & 1)) {
+                            if (j >= steps[w]) continue;
                             ok = warp_wait(&sh.p_full[w][0], done[w]++ & 1u, gave_up);
                             if (!ok) break;
                             tc::tc_fence_after();
                             values(w);
-                        }
-                        if (ok && then < until[w]) {
+                        } else if (then < until[w]) {
                             if (!keys) ok = warp_wait(&sh.k_full[0], k_uses++ & 1u, gave_up);
                             keys = true;
-                            scores(w, turn, then + 1 == until[w]);
+                            scores(w, turn);
                         }
                     }
                     if (!ok) break;
-                    release(&sh.v_empty[0]);
+                    if (!turn) release(&sh.v_empty[0]);
                     if (more) release(&sh.k_empty[0]);
                 }
             }
@@ -977,6 +970,14 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
             const Job &job = walk.job();
             const int first = job.first[w], steps = tc::uniform(job.steps[w]);
             if (first < 0) continue;
+            if (steps) {
+                // the tile's queries; the scores that were multiplied with the last ones have been read
+                const unsigned t = threadIdx.x & 127u;
+                float4 v[8][2];
+                read_tile(reinterpret_cast<const float *>(a.q), a.head_dim, t, v, [&](unsigned r) { return row_at(a, job, first, r, a.q_row, a.q_head); });
+                split_tile(v, smem + (q_at - base) + w * 3 * H::BYTES, t);
+                tc::mbar_arrive(&sh.q_full[0][w]);
+            }
             const int query = first + (int)(row * a.part >> 16);
             const int seen = a.masked ? min(job.keys, query + job.behind() + 1) : job.keys;              // first key that the row does not see
             const int least_seen = __shfl_sync(0xffffffffu, seen, 0), most_seen = __shfl_sync(0xffffffffu, seen, 31);       // of the warp's rows
