@@ -765,31 +765,18 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
 
 // ---- fp32 on tcgen05: operands of three bf16 parts each (attention_tc.cuh) ----
 
-// A tile of 128 rows of up to 64 features by 128 threads, a thread eight features of every 16th row: read, and written as three parts.
-template <typename At>
-__device__ __forceinline__ void read_tile(const float *from, unsigned features, unsigned t, float4 (&v)[8][2], const At &place) {
-    const unsigned f = (t & 7u) * 8;
-    #pragma unroll
-    for (int x = 0; x < 8; x++) {
-        const long long at = place((t >> 3) + 16 * x);         // in elements; -1: zeros
-        const bool in = at >= 0 && f < features;
-        const float4 *const p = reinterpret_cast<const float4 *>(from + (in ? at + f : 0));
-        v[x][0] = in ? __ldg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-        v[x][1] = in ? __ldg(p + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-}
-__device__ __forceinline__ void split_tile(const float4 (&v)[8][2], char *to, unsigned t) {
+// Eight features of a row to the three parts of a tile.
+__device__ __forceinline__ void split_piece(const float4 (&v)[2], char *put) {
     constexpr int BYTES = fused::Parts::BYTES;
-    #pragma unroll
-    for (int x = 0; x < 8; x++) {
-        const unsigned r = (t >> 3) + 16 * x;
-        split::Pair y[4] = {split::pack(v[x][0].x, v[x][0].y), split::pack(v[x][0].z, v[x][0].w), split::pack(v[x][1].x, v[x][1].y), split::pack(v[x][1].z, v[x][1].w)};
-        char *const put = to + r * 128 + (((t ^ r) & 7u) << 4);
-        *reinterpret_cast<uint4 *>(put) = make_uint4(split::take_part<0>(y[0]), split::take_part<0>(y[1]), split::take_part<0>(y[2]), split::take_part<0>(y[3]));
-        *reinterpret_cast<uint4 *>(put + BYTES) = make_uint4(split::take_part<1>(y[0]), split::take_part<1>(y[1]), split::take_part<1>(y[2]), split::take_part<1>(y[3]));
-        *reinterpret_cast<uint4 *>(put + 2 * BYTES) = make_uint4(split::take_part<2>(y[0]), split::take_part<2>(y[1]), split::take_part<2>(y[2]), split::take_part<2>(y[3]));
-    }
-    tc::fence_proxy_async_smem();
+    split::Pair y[4] = {split::pack(v[0].x, v[0].y), split::pack(v[0].z, v[0].w), split::pack(v[1].x, v[1].y), split::pack(v[1].z, v[1].w)};
+    *reinterpret_cast<uint4 *>(put) = make_uint4(split::take_part<0>(y[0]), split::take_part<0>(y[1]), split::take_part<0>(y[2]), split::take_part<0>(y[3]));
+    *reinterpret_cast<uint4 *>(put + BYTES) = make_uint4(split::take_part<1>(y[0]), split::take_part<1>(y[1]), split::take_part<1>(y[2]), split::take_part<1>(y[3]));
+    *reinterpret_cast<uint4 *>(put + 2 * BYTES) = make_uint4(split::take_part<2>(y[0]), split::take_part<2>(y[1]), split::take_part<2>(y[2]), split::take_part<2>(y[3]));
+}
+__device__ __forceinline__ void read_piece(float4 (&v)[2], const float *from, bool in) {
+    const float4 *const p = reinterpret_cast<const float4 *>(from);
+    v[0] = in ? __ldg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+    v[1] = in ? __ldg(p + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, unsigned kv_heads) {
@@ -823,27 +810,46 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
     // Registers: 128 x (2 x 168 + 64 + 112) = 512 x 128, what the launch holds
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-        // Splits keys and values.
-        const unsigned t = threadIdx.x & 127u;
+        // Splits keys and values, in turn: a thread eight features of every 16th row.
+        const unsigned t = threadIdx.x & 127u, row0 = t >> 3, piece = t & 7u;
+        const bool wide = piece * 8 < a.head_dim;
+        char *const put = smem + (k_at - base) + row0 * 128 + ((piece ^ (row0 & 7u)) << 4);
         unsigned uses = 0;
         bool ok = true;
         for (Walk walk{&sh}; ok && walk.next(); walk.done()) {
             const Job &job = walk.job();
             const int items = 2 * job.both();
+            float4 v[8][2];
+            const float *from;
+            size_t apart;
+            int left;                                  // keys from the thread's first one on
+            auto place = [&](int i) {
+                const unsigned row = i & 1 ? a.v_row : a.k_row, key = (unsigned)(i / 2) * TILE + row0;
+                from = reinterpret_cast<const float *>(i & 1 ? a.v : a.k) + (size_t)(unsigned)job.kv_head * (i & 1 ? a.v_head : a.k_head) + (size_t)((unsigned)job.k0 + key) * row + piece * 8;
+                apart = (size_t)16 * row;
+                left = wide ? job.keys - (int)key : 0;
+            };
+            if (items) {
+                place(0);
+                #pragma unroll
+                for (int x = 0; x < 8; x++) read_piece(v[x], from + x * apart, 16 * x < left);
+            }
             #pragma unroll 1
-            for (int i = 0; i < items && ok; i++) {
-                const bool value = i & 1;
-                const int key = i / 2 * (int)TILE;
-                float4 v[8][2];
-                read_tile(reinterpret_cast<const float *>(value ? a.v : a.k), a.head_dim, t, v, [&](unsigned row) {
-                    const int r = key + (int)row;
-                    return r < job.keys ? (long long)((unsigned long long)(unsigned)(job.k0 + r) * (value ? a.v_row : a.k_row) + (unsigned long long)(unsigned)job.kv_head * (value ? a.v_head : a.k_head)) : -1ll;
-                });
-                ok = warp_wait(value ? &sh.v_empty[0] : &sh.k_empty[0], (uses & 1u) ^ 1u, gave_up);
+            for (int i = 0; i < items; i++) {
+                ok = warp_wait(i & 1 ? &sh.v_empty[0] : &sh.k_empty[0], (uses & 1u) ^ 1u, gave_up);
                 if (!ok) break;
-                uses += value;
-                split_tile(v, smem + ((value ? v_at : k_at) - base), t);
-                tc::mbar_arrive(value ? &sh.v_full[0] : &sh.k_full[0]);
+                uses += i & 1;
+                char *const to = put + (i & 1 ? 3 * H::BYTES : 0);
+                // each piece of what comes next is asked for as soon as this one's has been taken
+                if (i + 1 < items) place(i + 1);
+                else left = 0;
+                #pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    split_piece(v[x], to + x * 2048);
+                    read_piece(v[x], from + x * apart, 16 * x < left);
+                }
+                tc::fence_proxy_async_smem();
+                tc::mbar_arrive(i & 1 ? &sh.v_full[0] : &sh.k_full[0]);
             }
         }
         __syncwarp();
@@ -926,7 +932,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
                     #pragma unroll 1
                     for (int i = 0; i < 4 && ok; i++) {
                         const int w = turn ? i & 1 : i >> 1;
-                        if (turn && i == 2) release(&sh.v_empty[0]);
+                        if (i == (turn ? 2 : 3)) release(&sh.v_empty[0]);
                         if (!(turn ? i >> 1 : i & 1)) {
                             if (j >= steps[w]) continue;
                             ok = warp_wait(&sh.p_full[w][0], done[w]++ & 1u, gave_up);
@@ -940,7 +946,6 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
                         }
                     }
                     if (!ok) break;
-                    if (!turn) release(&sh.v_empty[0]);
                     if (more) release(&sh.k_empty[0]);
                 }
             }
@@ -972,10 +977,18 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
             if (first < 0) continue;
             if (steps) {
                 // the tile's queries; the scores that were multiplied with the last ones have been read
-                const unsigned t = threadIdx.x & 127u;
+                const unsigned t = threadIdx.x & 127u, row0 = t >> 3, piece = t & 7u;
+                char *const put = smem + (q_at - base) + w * 3 * H::BYTES + row0 * 128 + ((piece ^ (row0 & 7u)) << 4);
                 float4 v[8][2];
-                read_tile(reinterpret_cast<const float *>(a.q), a.head_dim, t, v, [&](unsigned r) { return row_at(a, job, first, r, a.q_row, a.q_head); });
-                split_tile(v, smem + (q_at - base) + w * 3 * H::BYTES, t);
+                #pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    const long long at = row_at(a, job, first, row0 + 16 * x, a.q_row, a.q_head);
+                    const bool in = at >= 0 && piece * 8 < a.head_dim;
+                    read_piece(v[x], reinterpret_cast<const float *>(a.q) + (in ? at + piece * 8 : 0), in);
+                }
+                #pragma unroll
+                for (int x = 0; x < 8; x++) split_piece(v[x], put + x * 2048);
+                tc::fence_proxy_async_smem();
                 tc::mbar_arrive(&sh.q_full[0][w]);
             }
             const int query = first + (int)(row * a.part >> 16);
