@@ -415,13 +415,13 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
     if (threadIdx.x == 0) {
         sh.gave_up = 0u;
         tc::mbar_init(&sh.answered, 1u); tc::mbar_init(&sh.wanted, 1u);
-        for (unsigned i = 0; i < JOBS; i++) { tc::mbar_init(&sh.job_full[i], 1u); tc::mbar_init(&sh.job_empty[i], 14u); }
+        for (unsigned i = 0; i < JOBS; i++) { tc::mbar_init(&sh.job_full[i], 1u); tc::mbar_init(&sh.job_empty[i], 13u + H::MMA_WARPS); }
         for (int w = 0; w < 2; w++) {
             for (int b = 0; b < 2; b++) { tc::mbar_init(&sh.q_full[b][w], 1u); tc::mbar_init(&sh.q_empty[b][w], 1u); }
             tc::mbar_init(&sh.s_full[w], 1u); tc::mbar_init(&sh.o_full[w], 1u); tc::mbar_init(&sh.o_done[w], 1u);
             tc::mbar_init(&sh.s_free[w], 4u); tc::mbar_init(&sh.p_full[w][0], 4u); tc::mbar_init(&sh.p_full[w][1], 4u); tc::mbar_init(&sh.o_free[w], 4u); tc::mbar_init(&sh.l_full[w], 4u);
         }
-        for (int s = 0; s < 4; s++) { tc::mbar_init(&sh.k_full[s], 1u); tc::mbar_init(&sh.k_empty[s], 1u); tc::mbar_init(&sh.v_full[s], 1u); tc::mbar_init(&sh.v_empty[s], 1u); }
+        for (int s = 0; s < 4; s++) { tc::mbar_init(&sh.k_full[s], 1u); tc::mbar_init(&sh.k_empty[s], H::MMA_WARPS); tc::mbar_init(&sh.v_full[s], 1u); tc::mbar_init(&sh.v_empty[s], H::MMA_WARPS); tc::mbar_init(&sh.v_clean[s], 1u); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tc::fence_proxy_async_smem();
     }
@@ -529,33 +529,40 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                 }
                 if (!ok) break;
             }
-        } else if (warp == 9) {
+        } else if (warp == 9 || H::MMA_WARPS == 2) {
             constexpr unsigned FORMAT = TYPE == ASPEN_B200_BF16 ? 1u : 0u;
             constexpr unsigned IDESC = 1u << 4 | FORMAT << 7 | FORMAT << 10 | (128u >> 4) << 24;       // sums fp32, 128 rows
             constexpr unsigned IDESC_S = IDESC | (128u >> 3) << 17, IDESC_O = IDESC | ((unsigned)DIM >> 3) << 17 | 1u << 16;      // the second operand of PV: features contiguous
-            unsigned stage = 0, lap = 0, q_uses[2] = {0, 0}, asked[2] = {0, 0}, done[2] = {0, 0}, outs[2] = {0, 0};
+            constexpr int OWN = 2 / H::MMA_WARPS;     // tiles of this warp, w0 the first
+            const unsigned w0 = warp == 11;
+            unsigned stage = 0, lap = 0, q_uses[OWN], asked[OWN], done[OWN], outs[OWN], cleaned = 0;      // cleaned: a bit for each stage, the parity of its steps that the keys ended in
             Walk walk{&sh};
-            // Steps of the job in work and of the next one.  Only the next is looked for while one is in work: the one behind it takes the place of the one in work.
-            int steps[2], next[2] = {0, 0}, keys = 0, next_keys = 0;
+            // Steps of the own tiles, and of both, of the job in work and of the next one.  Only the next is looked for while one is in work: the one behind it takes the place of the one in work.
+            int steps[OWN], keys, next[OWN], next_all, next_keys = 0;
+            #pragma unroll
+            for (int i = 0; i < OWN; i++) q_uses[i] = asked[i] = done[i] = outs[i] = 0;
             bool live = true, begun = false;          // begun: the next one's first scores have been asked for
             auto look = [&]() {
-                next[0] = next[1] = 0;
+                next_all = 0;
+                #pragma unroll
+                for (int i = 0; i < OWN; i++) next[i] = 0;
                 live = walk.next();
                 if (!live) return;
                 const Job &job = walk.job();
-                next[0] = tc::uniform(job.steps[0]);
-                next[1] = tc::uniform(job.steps[1]);
+                #pragma unroll
+                for (int i = 0; i < OWN; i++) next[i] = tc::uniform(job.steps[w0 + i]);
+                next_all = tc::uniform(job.both());
                 next_keys = tc::uniform(job.keys);
                 walk.done();
             };
-            // scores of tile w over the keys of stage `st`; the job's first or last ones
-            auto scores = [&](int w, unsigned st, bool first, bool last) {
-                const unsigned use = q_uses[w], b = use % H::QUERIES;
+            // scores of an own tile over the keys of the stage; the job's first or last ones
+            auto scores = [&](int i, bool first, bool last) {
+                const unsigned w = w0 + i, use = q_uses[i], b = use % H::QUERIES;
                 if (first) ok = ok && warp_wait(&sh.q_full[b][w], use / H::QUERIES & 1u, gave_up);
                 // a tile's softmax has read its scores before: it has given their weights, or (weights of their own) said so
-                if (H::OWN_P) ok = ok && warp_wait(&sh.s_free[w], (asked[w] & 1u) ^ 1u, gave_up);
-                asked[w]++;
-                if (last) q_uses[w]++;
+                if (H::OWN_P) ok = ok && warp_wait(&sh.s_free[w], (asked[i] & 1u) ^ 1u, gave_up);
+                asked[i]++;
+                if (last) q_uses[i]++;
                 if (!ok) return;
                 tc::tc_fence_after();
                 const unsigned q = q_at + (b * 2 + w) * H::BYTES;
@@ -564,14 +571,14 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                     for (int c = 0; c < H::CHUNKS; c++)
                         #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            mma_ss(tmem + H::S + w * 128, tc::umma_desc_low(q + c * H::CHUNK_BYTES + k * 32), tc::umma_desc_low(k_at + st * H::BYTES + c * H::CHUNK_BYTES + k * 32), IDESC_S, c + k);
+                            mma_ss(tmem + H::S + w * 128, tc::umma_desc_low(q + c * H::CHUNK_BYTES + k * 32), tc::umma_desc_low(k_at + stage * H::BYTES + c * H::CHUNK_BYTES + k * 32), IDESC_S, c + k);
                     tc::tc_commit(&sh.s_full[w]);
                     if (last) tc::tc_commit(&sh.q_empty[b][w]);
                 }
                 __syncwarp();
             };
             // keys 16 from ... of the step
-            auto values = [&](int w, unsigned st, bool first, bool last, int from, int to) {
+            auto values = [&](unsigned w, unsigned st, bool first, bool last, int from, int to) {
                 if (tc::elect_one()) {
                     #pragma unroll
                     for (int k = from; k < to; k++)
@@ -582,62 +589,70 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
             };
             auto release = [&](unsigned long long *bar) { if (tc::elect_one()) tc::tc_commit(bar); __syncwarp(); };
             for (look(); ok && live;) {
-                if (!next[0] && !next[1]) { look(); continue; }
+                if (!next_all) { look(); continue; }
                 if (!begun) {
                     ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
                     #pragma unroll
-                    for (int w = 0; w < 2; w++) if (next[w]) scores(w, stage, true, next[w] == 1);
+                    for (int i = 0; i < OWN; i++) if (next[i]) scores(i, true, next[i] == 1);
                     if (!ok) break;
                     release(&sh.k_empty[stage]);
                 }
-                begun = false;
-                steps[0] = next[0]; steps[1] = next[1]; keys = next_keys;
-                const int all = max(steps[0], steps[1]);
+                #pragma unroll
+                for (int i = 0; i < OWN; i++) steps[i] = next[i];
+                const int all = next_all;
+                keys = next_keys;
                 for (int j = 0; j < all; j++) {
                     const unsigned here = stage, at = lap;
                     if (++stage == H::STAGES) { stage = 0; lap++; }
                     // the scores to ask for now: the next step's, or the next job's first ones
                     const bool turn = j + 1 == all;
-                    if (j == max(0, all - 3) && lane == 0) tc::mbar_arrive(&sh.wanted);
+                    if (w0 == 0 && j == max(0, all - 3) && lane == 0) tc::mbar_arrive(&sh.wanted);
                     if (turn) look();
-                    const int then = turn ? 0 : j + 1, until0 = turn ? next[0] : steps[0], until1 = turn ? next[1] : steps[1];
-                    const bool more = then < until0 || then < until1;
-                    begun = turn && more;
+                    begun = turn && next_all > 0;
+                    const bool more = begun || !turn;
+                    const int then = turn ? 0 : j + 1;
                     if (more) ok = warp_wait(&sh.k_full[stage], lap & 1u, gave_up);
                     if (!ok) break;
                     if (H::OWN_P && more) {
                         #pragma unroll
-                        for (int w = 0; w < 2; w++) { const int until = w ? until1 : until0; if (then < until) scores(w, stage, turn, then + 1 == until); }
+                        for (int i = 0; i < OWN; i++) { const int until = turn ? next[i] : steps[i]; if (then < until) scores(i, turn, then + 1 == until); }
                         if (!ok) break;
                         release(&sh.k_empty[stage]);
                     }
                     ok = warp_wait(&sh.v_full[here], at & 1u, gave_up);
                     if (!ok) break;
                     if (keys < (j + 1) * (int)TILE) {
-                        const int from = keys - j * (int)TILE;
-                        char *const v = smem + (v_at - base) + here * H::BYTES;
-                        for (int i = from * 8 + (int)lane; i < (int)TILE * 8; i += 32)
-                            #pragma unroll
-                            for (int c = 0; c < H::CHUNKS; c++) *reinterpret_cast<uint4 *>(v + c * H::CHUNK_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        tc::fence_proxy_async_smem();
-                        __syncwarp();
+                        if (w0 == 0) {
+                            const int from = keys - j * (int)TILE;
+                            char *const v = smem + (v_at - base) + here * H::BYTES;
+                            for (int i = from * 8 + (int)lane; i < (int)TILE * 8; i += 32)
+                                #pragma unroll
+                                for (int c = 0; c < H::CHUNKS; c++) *reinterpret_cast<uint4 *>(v + c * H::CHUNK_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            tc::fence_proxy_async_smem();
+                            __syncwarp();
+                            if (H::MMA_WARPS == 2 && lane == 0) tc::mbar_arrive(&sh.v_clean[here]);
+                        } else {
+                            ok = warp_wait(&sh.v_clean[here], cleaned >> here & 1u, gave_up);
+                            cleaned ^= 1u << here;
+                        }
                     }
                     #pragma unroll
-                    for (int w = 0; w < 2; w++) {
-                        const int until = w ? until1 : until0;
-                        if (ok && j < steps[w]) {
-                            if (j == 0) { ok = warp_wait(&sh.o_free[w], (outs[w] & 1u) ^ 1u, gave_up); outs[w]++; }        // the job before has been written out
-                            ok = ok && warp_wait(&sh.p_full[w][0], done[w] & 1u, gave_up);
+                    for (int i = 0; i < OWN; i++) {
+                        const unsigned w = w0 + i;
+                        const int until = turn ? next[i] : steps[i];
+                        if (ok && j < steps[i]) {
+                            if (j == 0) { ok = warp_wait(&sh.o_free[w], (outs[i] & 1u) ^ 1u, gave_up); outs[i]++; }        // the job before has been written out
+                            ok = ok && warp_wait(&sh.p_full[w][0], done[i] & 1u, gave_up);
                             if (!ok) continue;
                             tc::tc_fence_after();
                             values(w, here, j == 0, false, 0, 6);
-                            ok = warp_wait(&sh.p_full[w][1], done[w] & 1u, gave_up);
+                            ok = warp_wait(&sh.p_full[w][1], done[i] & 1u, gave_up);
                             if (!ok) continue;
-                            done[w]++;
+                            done[i]++;
                             tc::tc_fence_after();
-                            values(w, here, false, j + 1 == steps[w], 6, 8);
+                            values(w, here, false, j + 1 == steps[i], 6, 8);
                         }
-                        if (!H::OWN_P && ok && then < until) scores(w, stage, turn, then + 1 == until);
+                        if (!H::OWN_P && ok && then < until) scores(i, turn, then + 1 == until);
                     }
                     if (!ok) break;
                     release(&sh.v_empty[here]);

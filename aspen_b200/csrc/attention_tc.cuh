@@ -8,7 +8,7 @@
 // The maximum is followed loosely: O and the sum are scaled again only when a row's maximum has grown by more than 2^8 (weights up to 256 are as exact as weights up to 1), so the
 // sums in TMEM are hardly ever read before the end.
 //
-// Warps: 0 - 3 and 4 - 7 the softmax of the two tiles, 8 TMA, 9 MMA, 10 finds the work, 12 - 15 write outputs; nothing but mbarriers connects them, and while one tile's scores are weighed
+// Warps: 0 - 3 and 4 - 7 the softmax of the two tiles, 8 TMA, 9 MMA (with 64 features 9 and 11, a tile each), 10 finds the work, 12 - 15 write outputs; nothing but mbarriers connects them, and while one tile's scores are weighed
 // the other's are multiplied.  The first three quarters of a tile's weights are multiplied while the last one is computed.  TMEM, 512 columns: scores 2 x 128, sums 2 x features, and with 64
 // features weights 2 x 64 of their own, so that the next scores, the next job's too, are there before the weights of these have been multiplied; with 128 the weights take the place of their
 // scores.
@@ -24,7 +24,7 @@
 // Tried and slower: two threads a query (16 warps: registers), a quarter of the exponentials by polynomials in packed multiply-adds (FMA and ALU then take what the exp2 unit gives; their
 // second copy of the code costs instruction fetches), weights from the maximum of the step before with a second try (the same), 32 keys a turn in a loop (24 packed prompts 72 us).
 //
-// Values behind the end of a sequence are another one's, or nobody's: the MMA warp sets them to zero in shared memory, since 0 x NaN would reach every row.
+// Values behind the end of a sequence are another one's, or nobody's: an MMA warp sets them to zero in shared memory, since 0 x NaN would reach every row.
 //
 // Every wait is bounded (2 s, or 2 s and 100 us a step) and is for another role of the CTA; if one runs out all roles leave, TMEM is freed and the rows of out that were in work become NaN.
 #pragma once
@@ -45,6 +45,9 @@ struct Shape {
     static constexpr int OUT_BYTES = 4 * 2048;                      // where a warp turns its outputs round
     static constexpr int SMEM = 2 * QUERIES * BYTES + 2 * STAGES * BYTES + OUT_BYTES + 1024;
     static constexpr bool OWN_P = DIM == 64;
+    // With weights of their own the tiles need nothing of each other, and a warp for each lets them: 24 packed prompts 46.9 us, 48.7 with one for both.  Without, one warp keeps the products
+    // of one tile behind the other's: 4 long prompts 224.6 us, 229.4 with two.
+    static constexpr int MMA_WARPS = OWN_P ? 2 : 1;
     static constexpr unsigned S = 0, O = 256, P = OWN_P ? 384 : 0, P_APART = OWN_P ? 64 : 128;      // TMEM columns
 };
 
@@ -73,7 +76,7 @@ constexpr unsigned JOBS = 2;                       // the one in work and the ne
 struct Shared {
     uint4 answer;                                  // to a request for another CTA's work
     unsigned long long answered, wanted, job_full[JOBS], job_empty[JOBS];
-    unsigned long long q_full[2][2], q_empty[2][2], k_full[4], k_empty[4], v_full[4], v_empty[4];      // q: [buffer][tile]
+    unsigned long long q_full[2][2], q_empty[2][2], k_full[4], k_empty[4], v_full[4], v_empty[4], v_clean[4];      // q: [buffer][tile]
     unsigned long long s_full[2], s_free[2], p_full[2][2], o_full[2];
     unsigned long long o_done[2], o_free[2], l_full[2];                                                // a job's sums: complete, read; the rows' factors
     Job jobs[JOBS];

@@ -459,6 +459,27 @@ def test_a_neighbours_nan_does_not_reach_a_sequence(kind, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_more_pieces_of_work_than_multiprocessors(kind, dim):
+    """Each takes several, most of them short and all with keys that end inside a tile; every third sequence's values are NaN, behind the others' last ones too."""
+    rng = np.random.default_rng(dim)
+    lengths = rng.integers(65, 260, 90)
+    starts = np.concatenate([[0], np.cumsum(lengths)])
+    q, k, v = (rounded(rng.standard_normal((starts[-1], h, dim)), kind) for h in (12, 6, 6))
+    for s in range(2, 90, 3):
+        v[starts[s]:starts[s + 1]] = np.nan
+    got = prompt(*(to_device(a, kind) for a in (q, k, v)), starts, starts, kind, True, 0.2)
+    for s in range(90):
+        a, b = starts[s], starts[s + 1]
+        if s % 3 == 2:
+            assert got[a:b].isnan().all()
+        else:
+            want, away, size = attend(q[a:b], k[a:b], v[a:b], 0.2, seen_by(b - a, b - a, True))
+            check(got[a:b], want, away, size, kind)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [api.FP32, api.BF16], ids=ids)
 def test_a_prompt_inside_a_fused_projection(kind):
     """Queries, keys and values as columns of one matrix, outputs with a gap between heads."""
