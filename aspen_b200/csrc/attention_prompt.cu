@@ -358,8 +358,8 @@ struct Walk {
     fused::Shared *sh;
     unsigned slot = 0, lap = 0;
     __device__ __forceinline__ const fused::Job &job() const { return sh->jobs[slot]; }
-    __device__ __forceinline__ bool next() {
-        if (!fused::warp_wait(&sh->job_full[slot], lap & 1u, &sh->gave_up)) return false;
+    __device__ __forceinline__ bool next(unsigned long long limit = fused::LIMIT_NS) {
+        if (!fused::warp_wait(&sh->job_full[slot], lap & 1u, &sh->gave_up, limit)) return false;
         return tc::uniform(job().live) != 0;
     }
     __device__ __forceinline__ void done() {
@@ -680,9 +680,11 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
         const Pair scale2 = pair(a.scale, a.scale);
         unsigned done = 0, outs = 0;
         bool ok = true;
-        for (Walk walk{&sh}; ok && walk.next(); walk.done()) {
+        int both = 0;                                  // steps of the job before: without a tile of their own these warps wait for all of them
+        for (Walk walk{&sh}; ok && walk.next(whole_job(both)); walk.done()) {
             const Job &job = walk.job();
             const int first = job.first[w], steps = tc::uniform(job.steps[w]);
+            both = job.both();
             if (first < 0 || steps == 0) continue;
             const int query = first + (int)(row * a.part >> 16);
             const int seen = a.masked ? min(job.keys, query + job.behind() + 1) : job.keys;              // first key that the row does not see
@@ -986,9 +988,11 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
         const Pair scale2 = pair(a.scale, a.scale);
         unsigned done = 0;
         bool ok = true;
-        for (Walk walk{&sh}; walk.next(); walk.done()) {
+        int both = 0;                                  // steps of the job before: without a tile of their own these warps wait for all of them
+        for (Walk walk{&sh}; walk.next(whole_job(both)); walk.done()) {
             const Job &job = walk.job();
             const int first = job.first[w], steps = tc::uniform(job.steps[w]);
+            both = job.both();
             if (first < 0) continue;
             if (steps) {
                 // the tile's queries; the scores that were multiplied with the last ones have been read

@@ -480,6 +480,17 @@ def test_many_more_pieces_of_work_than_multiprocessors(kind, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,keys", [(api.BF16, 3 << 27), (api.FP32, 1 << 27)], ids=["bf16", "fp32"])
+def test_a_single_query_over_keys_for_seconds(kind, keys):
+    """Longer than one role of a CTA waits for another within a step.  All weight is on the last key."""
+    import torch
+    k, v = (torch.zeros((keys, 1, 8), dtype=torch_type(kind), device="cuda") for _ in range(2))
+    k[-1], v[-1] = 40, 3
+    got = prompt(torch.ones((1, 1, 8), dtype=torch_type(kind), device="cuda"), k, v, [0, 1], [0, keys], kind, False, 0.5)
+    assert (got == 3).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [api.FP32, api.BF16], ids=ids)
 def test_a_prompt_inside_a_fused_projection(kind):
     """Queries, keys and values as columns of one matrix, outputs with a gap between heads."""
