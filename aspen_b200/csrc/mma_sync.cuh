@@ -1,4 +1,4 @@
-// Warp-level matrix products (mma.sync) over operands that lanes hold as 16-byte pieces of rows, for fp32, bf16 and fp16.
+// Warp-level matrix products (mma.sync) over operands that lanes hold as 16-byte pieces of rows (32-byte ones are two of them for the same lane), for fp32, bf16 and fp16.
 //
 // The products run over features or keys in any order, as long as both operands agree, so a lane takes the 16 bytes it has loaded as its part of
 // consecutive k steps and nothing is rearranged:
