@@ -84,12 +84,17 @@ template <int LEFT> __device__ __forceinline__ void wait_copies() { asm volatile
 template <int TYPE, int DIM>
 struct Rows {
     static constexpr int SIZE = TYPE == ASPEN_B200_FP32 ? 4 : 2, VALUES = 16 / SIZE, BYTES = DIM * SIZE;
-    static constexpr int QUERIES = 64, KEYS = BYTES > 512 ? 32 : 64, THREADS = 128;
+    static constexpr int QUERIES = 64, THREADS = 128;
+    // fp32 rows of 512 bytes: tiles of 32 keys leave room for two CTAs on an SM (8 prompts of 512 tokens, 12 heads of 128: 207 us, 287 with 64); 16-bit ones of 512 take 64 (24 us, 30)
+    static constexpr int KEYS = SIZE == 4 && BYTES >= 512 ? 32 : 64;
     static constexpr int KPITCH = BYTES + 64, VPITCH = BYTES + 16, STAGE = KEYS * (KPITCH + VPITCH);
     static constexpr bool HELD = BYTES <= 256;                  // queries stay in registers
     static constexpr int SMEM = 2 * STAGE + (HELD ? 0 : QUERIES * KPITCH);
     static constexpr int PIECES = DIM / (4 * VALUES);           // of a lane and row, product over features
     static constexpr int VPIECES = DIM / (8 * VALUES);
+    // Pieces of the product over features in a turn of its loop.  fp32 that reads its queries again takes one: all of them spill registers and are more code than is fetched in time
+    // (the 8 prompts 197 us instead of 207, 4 of 300 tokens with 8 heads of 256 106 instead of 129); 16 bits are faster with all (24 us, 26).
+    static constexpr int TURN = HELD || SIZE == 2 ? PIECES : 1;
 };
 
 template <int TYPE, int DIM>
@@ -150,7 +155,7 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
         for (int n = 0; n < KT; n++)
             #pragma unroll
             for (int j = 0; j < 4; j++) s[n][j] = 0.f;
-        #pragma unroll
+        #pragma unroll R::TURN
         for (int i = 0; i < R::PIECES; i++) {
             const int f = (i * 4 * VALUES + t * VALUES) * SIZE;
             const uint4 x = R::HELD ? held[R::HELD ? 2 * i : 0] : *reinterpret_cast<const uint4 *>(own + g * R::KPITCH + f);
