@@ -19,6 +19,7 @@ using attn::wait_for_previous_kernel;
 
 constexpr unsigned BOOK = 1024;                // threads of the CTA that keeps the books
 constexpr unsigned MOST_PAGES = 1u << 21;      // for one entry of an extend: sums over the CTA's threads stay below 2^32
+constexpr unsigned PLACED = 4;                 // new pages that a thread of extend finds the places of at once
 constexpr unsigned COPY = 256, IN_FLIGHT = 2, COPY_CTAS = 8;        // threads of a copying CTA, 16-byte loads in flight of each, CTAs on an SM
 
 struct Pool {
@@ -72,18 +73,30 @@ __device__ __forceinline__ unsigned before_me(unsigned v, unsigned &all, unsigne
 
 constexpr unsigned SCAN = 8;                   // pages a thread looks at in a turn
 
-// The `want` lowest free pages, in order, to `list`; returns how many there are (up to `want`).
+// The `want` lowest free pages, in order, to `list`; returns how many there are (up to `want`).  A warp looks at 256 pages in a row, 32 a load, and those of the next
+// turn are on their way while these are counted.
 __device__ unsigned lowest_free(const int *refs, unsigned pages, unsigned want, int *list, unsigned *sums) {
+    const unsigned lane = threadIdx.x % 32, mine = threadIdx.x / 32 * (32 * SCAN) + lane;
     unsigned found = 0;
+    int v[SCAN];
+    auto load = [&](unsigned first) {
+        #pragma unroll
+        for (unsigned i = 0; i < SCAN; i++) v[i] = first + i * 32 < pages ? refs[first + i * 32] : 1;
+    };
+    if (want) load(mine);
     for (unsigned p0 = 0; p0 < pages && found < want; p0 += BOOK * SCAN) {
-        const unsigned first = p0 + threadIdx.x * SCAN;
-        unsigned free = 0;
+        unsigned free[SCAN], count = 0;
         #pragma unroll
-        for (unsigned i = 0; i < SCAN; i++) if (first + i < pages && refs[first + i] == 0) free |= 1u << i;
-        unsigned all, rank = found + before_me(__popc(free), all, sums);
+        for (unsigned i = 0; i < SCAN; i++) { free[i] = __ballot_sync(0xffffffffu, v[i] == 0); count += __popc(free[i]); }
+        load(p0 + BOOK * SCAN + mine);
+        unsigned all, rank = found + before_me(lane == 0 ? count : 0u, all, sums);
+        rank = __shfl_sync(0xffffffffu, rank, 0);
         #pragma unroll
-        for (unsigned i = 0; i < SCAN; i++)
-            if (free >> i & 1u) { if (rank < want) list[rank] = (int)(first + i); rank++; }
+        for (unsigned i = 0; i < SCAN; i++) {
+            const unsigned at = rank + __popc(free[i] & ((1u << lane) - 1u));
+            if (free[i] >> lane & 1u && at < want) list[at] = (int)(p0 + mine + i * 32);
+            rank += __popc(free[i]);
+        }
         found += all;
     }
     __syncthreads();
@@ -135,12 +148,24 @@ __global__ void __launch_bounds__(BOOK) extend_kernel(const Pool pool, const Spa
         if (threadIdx.x == 0) atomicOr(pool.at.status, refused | ASPEN_B200_CACHE_REFUSED);
         return;
     }
-    for (unsigned i = threadIdx.x; i < total; i += BOOK) {
-        unsigned lo = 0, hi = entries;              // the last entry that starts at i or before; empty ones start where the next does
-        while (hi - lo > 1) { const unsigned mid = (lo + hi) / 2; if ((unsigned)w.start[mid] <= i) lo = mid; else hi = mid; }
-        const int slot = slots ? slots[lo] : (int)lo, p = w.to[i];
-        pool.table[(size_t)slot * pool.at.max_pages + pages_for(attn::sequence_length(pool.at, slot), page) + (i - (unsigned)w.start[lo])] = p;
-        pool.refs[p] = 1;
+    unsigned top = 1;                               // the largest power of two that is not above the last entry
+    while (top * 2 < entries) top *= 2;
+    for (unsigned i0 = threadIdx.x; i0 < total; i0 += BOOK * PLACED) {
+        // the last entry that starts at i or before; empty ones start where the next does
+        unsigned entry[PLACED];
+        #pragma unroll
+        for (unsigned u = 0; u < PLACED; u++) entry[u] = 0;
+        for (unsigned step = top; step > 0; step /= 2)
+            #pragma unroll
+            for (unsigned u = 0; u < PLACED; u++) { const unsigned e = entry[u] + step; if (e < entries && (unsigned)w.start[e] <= i0 + u * BOOK) entry[u] = e; }
+        #pragma unroll
+        for (unsigned u = 0; u < PLACED; u++) {
+            const unsigned i = i0 + u * BOOK, e = entry[u];
+            if (i >= total) continue;
+            const int slot = slots ? slots[e] : (int)e, p = w.to[i];
+            pool.table[(size_t)slot * pool.at.max_pages + pages_for(attn::sequence_length(pool.at, slot), page) + (i - (unsigned)w.start[e])] = p;
+            pool.refs[p] = 1;
+        }
     }
     __syncthreads();
     for (unsigned e = threadIdx.x; e < entries; e += BOOK) {
