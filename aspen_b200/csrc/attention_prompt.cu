@@ -327,7 +327,9 @@ struct Finder {
         unsigned sum = mine;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const unsigned u = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= (unsigned)o) sum += u; }
-        const int at = __ffs(__ballot_sync(0xffffffffu, sum > rank)) - 1;
+        const unsigned behind = __ballot_sync(0xffffffffu, sum > rank);
+        if (!behind) return -1;                 // sequences that share rows: more pairs than are counted in 32 bits
+        const int at = __ffs(behind) - 1;
         unsigned left = rank - (sum - mine), which = 0;
         #pragma unroll
         for (unsigned k = 0; k < 4; k++) if (n[k] > lo) { if (left == 0) which = k; left--; }
@@ -1215,8 +1217,8 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     if (rc) return rc;
     if (!p->heads || !p->kv_heads || p->heads % p->kv_heads) { ASPEN_ERR("%s: %u heads of queries, %u of keys\n", what, p->heads, p->kv_heads); return -1; }
     if (!(p->scale - p->scale == 0.f)) { ASPEN_ERR("%s: scale is not finite\n", what); return -1; }
-    // rows are int on the device; block numbers and 128 rows past the end stay below 2^31
-    if (p->q_rows > 0x3fffffffu || p->kv_rows > 0x3fffffffu || p->sequences > 0x3fffffffu || p->heads > 0xffffu) { ASPEN_ERR("%s: too many rows, sequences or heads\n", what); return -2; }
+    // rows are int on the device; block numbers and 128 rows past the end stay below 2^31; a CTA reads the starts of 2^24 sequences in less time than its roles wait for one another
+    if (p->q_rows > 0x3fffffffu || p->kv_rows > 0x3fffffffu || p->sequences > 1u << 24 || p->heads > 0xffffu) { ASPEN_ERR("%s: too many rows, sequences or heads\n", what); return -2; }
     if (!p->sequences || !p->q_rows) return 0;
     if (!p->q_starts || !p->kv_starts) { ASPEN_ERR("%s: q_starts or kv_starts is NULL\n", what); return -1; }
     if ((rc = attn::check_rows(p->q, p->q_row_stride, p->q_head_stride, p->type, "q", what)) || (rc = attn::check_rows(p->out, p->out_row_stride, p->out_head_stride, p->type, "out", what))) return rc;

@@ -301,7 +301,7 @@ typedef enum { ASPEN_B200_FP32, ASPEN_B200_BF16, ASPEN_B200_FP16, ASPEN_B200_NUM
  * its keys, the one before it all but the last, and so on; with more queries than keys the first ones see none.  A row that sees nothing becomes zeros.
  * Rows of no sequence are neither read into a result nor written.  Starts outside 0 ... q_rows (kv_rows) are taken as the nearest one inside, a sequence that would
  * end before it starts is empty; sequences must not share rows of out.  Values behind a query's last key, but within its sequence, must be finite (they are
- * multiplied by zero). */
+ * multiplied by zero).  Up to 2^24 sequences, 2^30 - 1 rows. */
 typedef struct {
     const void *q, *k, *v;         /* [q_rows][heads][head_dim], [kv_rows][kv_heads][head_dim] twice */
     void *out;                     /* [q_rows][heads][head_dim]; not q, k or v */

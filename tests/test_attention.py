@@ -216,7 +216,7 @@ def test_a_prompt_that_cannot_be_is_refused():
     good = dict(type=api.FP16, heads=4, kv_heads=2, head_dim=64, scale=1.0, sequences=1, q_rows=3, kv_rows=3, q_starts=64, kv_starts=64, q=4096, k=4096, v=4096, out=8192)
     for change, rc in [(dict(type=7), -1), (dict(heads=5), -1), (dict(heads=0), -1), (dict(kv_heads=0), -1), (dict(head_dim=20), -1), (dict(head_dim=512), -1), (dict(scale=math.nan), -1),
                        (dict(q=0), -1), (dict(k=0), -1), (dict(v=0), -1), (dict(out=0), -1), (dict(q=4100), -1), (dict(q_starts=0), -1), (dict(kv_starts=0), -1),
-                       (dict(out_row_stride=257), -1), (dict(k_head_stride=2**30), -2), (dict(q_rows=2**31), -2), (dict(heads=2**16, kv_heads=2**16), -2)]:
+                       (dict(out_row_stride=257), -1), (dict(k_head_stride=2**30), -2), (dict(q_rows=2**31), -2), (dict(sequences=2**24 + 1), -2), (dict(heads=2**16, kv_heads=2**16), -2)]:
         assert L.aspen_b200_attention_prompt(C.byref(api.PromptArgs(**{**good, **change})), None) == rc, change
     assert L.aspen_b200_attention_prompt(None, None) == -1
     for change in (dict(sequences=0), dict(q_rows=0)):
