@@ -340,7 +340,8 @@ struct Finder {
         job.keys = max(0, clamped(a.kv_starts, s + 1, a.kv_rows) - job.k0);
         return (int)lo;
     }
-    __device__ __forceinline__ bool find(const Args &a, unsigned index, unsigned kv_heads, fused::Job &job) {
+    // turned: the later tile, which has more keys with a mask, is the first one
+    __device__ __forceinline__ bool find(const Args &a, unsigned index, unsigned kv_heads, unsigned turned, fused::Job &job) {
         const unsigned number = index / kv_heads;
         const int pair = levelled ? by_level(a, number, job) : find_piece(a, number, place, [&](unsigned queries) { return pairs(a, queries); }, job.q0, job.queries, job.k0, job.keys);
         if (pair < 0) return false;
@@ -348,7 +349,7 @@ struct Finder {
         job.block = (int)a.block;
         #pragma unroll
         for (int w = 0; w < 2; w++) {
-            job.first[w] = (pair * 2 + w) * (int)a.block;
+            job.first[w] = (pair * 2 + (w ^ (int)turned)) * (int)a.block;
             const bool there = job.first[w] < job.queries;
             job.steps[w] = there ? (job.end(w, a.masked) + (int)fused::TILE - 1) / (int)fused::TILE : 0;
             if (!there) job.first[w] = -1;
@@ -386,7 +387,7 @@ __device__ __forceinline__ void deal(fused::Shared &sh, const Args &a, unsigned 
     const unsigned lane = threadIdx.x % 32;
     Finder finder(a);
     Job begin;
-    bool ok = true, found = finder.find(a, blockIdx.x, kv_heads, begin);
+    bool ok = true, found = finder.find(a, blockIdx.x, kv_heads, 0u, begin);
     unsigned index, slot = 0, lap = 0, asked = 0, wanted = 0;
     while (true) {
         if (found) {
@@ -405,7 +406,7 @@ __device__ __forceinline__ void deal(fused::Shared &sh, const Args &a, unsigned 
         tc::fence_proxy_async_smem();          // the answer has been read before the next one is written
         __syncwarp();
         if (!more) break;
-        found = finder.find(a, index, kv_heads, begin);
+        found = finder.find(a, index, kv_heads, slot, begin);          // slots alternate, and so do the warps that get the longer tile
     }
     if (warp_wait(&sh.job_empty[slot], (lap & 1u) ^ 1u, &sh.gave_up) && lane == 0) { sh.jobs[slot].live = 0; tc::mbar_arrive(&sh.job_full[slot]); }
     __syncwarp();
