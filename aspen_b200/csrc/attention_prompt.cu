@@ -8,7 +8,7 @@
 // prompt_rows (what is left: wider heads, scales that are not positive, short sequences): a warp has 16 queries, its operands and sums in registers as mma.sync takes them (mma_sync.cuh); keys and values of a tile go through
 // shared memory for the four warps of a CTA, asked for one tile ahead.  Rows in shared memory are 64 (keys) and 16 bytes (values) longer than a power of two, so that the 16-byte pieces
 // that eight lanes read together lie in different banks.  It is bounded by mma.sync and, with one block to a sequence, by its chain of loads, products and exp2: 12 heads of 64, one prompt
-// of 37 tokens in fp32 9 us with the call, 32 prompts of 100 tokens in bf16 12 us (8 of 512 in fp32: 92 us, prompt_parts 34; 24 of up to 1024 in bf16: 101 us, prompt_tiles 47).
+// of 37 tokens in fp32 9 us with the call, 32 prompts of 100 tokens in bf16 12 us (8 of 512 in fp32: 92 us, prompt_parts 33; 24 of up to 1024 in bf16: 101 us, prompt_tiles 46.5).  8 of 512 with heads of 128 in fp32: 197 us.
 #include "attention_tc.cuh"
 #include "early_launch.cuh"
 #include "gemm_split.cuh"
@@ -1191,8 +1191,8 @@ bool try_tiles(const Args &a, int type, cudaStream_t stream, cudaError_t *err) {
     // a row's largest score is its largest product only for a scale above 0
     if (!a.kv_rows || !(a.scale > 0.f) || a.group > fused::TILE || jobs_of(a) > 0x7fffffffull) return false;
     // Short sequences, going by the mean: a job of one step takes 4 us (fp32 5), and a block of prompt_rows 1.2 (3), several at once on an SM.  12 heads of 64, bf16 and fp32, 32 prompts of 60
-    // tokens 10.5 and 14.5 us (in tiles 14 and 22), of 100 tokens 12 and 35 (14 and 28).  Where one sequence of a few is long and the others short, the blocks take up to three times as long,
-    // of 4096 rows at most.
+    // tokens 8.6 and 14.3 us (in tiles 14.5 and 21), of 100 tokens 12 and 35 (14.5 and 24.6); 8 heads of 128, fp16, of 96 tokens 14.7 (12.5).  Where one sequence of a few is long and the others
+    // short, the blocks take up to three times as long, of 4096 rows at most.
     if (a.group <= 2 && a.q_rows <= 4096 && a.q_rows <= 64ull * a.sequences && a.kv_rows <= 64ull * a.sequences) return false;
     if (type == ASPEN_B200_FP32) {
         if (a.head_dim > 64) return false;

@@ -20,9 +20,12 @@
 // What bounds it.  With 128 features a step of two tiles takes 2048 cycles of the tensor pipe at best, and as many of shared memory (Q and K are read from there for each
 // product, 128 bytes a cycle; the copies of K and V come on top); with 64 features 1024, and 2048 of the unit for exp2.  4 prompts of 1231 to 4096 tokens, 32 heads over 8 of
 // 128: 227 us, 1100 TFLOP/s of visible products, 3600 cycles a step: the chain of a tile (scores from TMEM 100, maximum 270, exponentials and sums 1250, then its products 900)
-// is as long as that with the other tile's in between.  24 packed prompts of 12 heads of 64: 47 us.
+// is as long as that with the other tile's in between.  24 packed prompts of 12 heads of 64: 46.5 us; the exp2 unit is busy for 45 %
+// of it: two tiles in the same phase of a step take 1.7 us for it, in opposite ones 1.35, and starts and ends of jobs of 2.2 steps a tile come on top.
 // Tried and slower: two threads a query (16 warps: registers), a quarter of the exponentials by polynomials in packed multiply-adds (FMA and ALU then take what the exp2 unit gives; their
-// second copy of the code costs instruction fetches), weights from the maximum of the step before with a second try (the same), 32 keys a turn in a loop (24 packed prompts 72 us).
+// second copy of the code costs instruction fetches), weights from the maximum of the step before with a second try (the same), 32 keys a turn in a loop (24 packed prompts 72 us), blocks of keys
+// that a warp does not see left out by branches (50 us), a late start for the second tile (the same), and for 64 features two CTAs on an SM with steps of 64 keys (49 us; one prompt of 4096 tokens
+// 79 instead of 56: a tile alone is slower).
 //
 // Values behind the end of a sequence are another one's, or nobody's: an MMA warp sets them to zero in shared memory, since 0 x NaN would reach every row.
 //
