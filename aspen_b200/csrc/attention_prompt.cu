@@ -5,10 +5,11 @@
 // prompt_tiles (16 bits, up to 128 features) and prompt_parts (fp32, up to 64): tcgen05, two tiles of 128 rows to a CTA, warps with a role each; attention_tc.cuh has the plan, what
 // bounds it and what it measured.
 //
-// prompt_rows (what is left: wider heads, scales that are not positive, short sequences): a warp has 16 queries, its operands and sums in registers as mma.sync takes them (mma_sync.cuh); keys and values of a tile go through
-// shared memory for the four warps of a CTA, asked for one tile ahead.  Rows in shared memory are 64 (keys) and 16 bytes (values) longer than a power of two, so that the 16-byte pieces
-// that eight lanes read together lie in different banks.  It is bounded by mma.sync and, with one block to a sequence, by its chain of loads, products and exp2: 12 heads of 64, one prompt
-// of 37 tokens in fp32 9 us with the call, 32 prompts of 100 tokens in bf16 12 us (8 of 512 in fp32: 92 us, prompt_parts 33; 24 of up to 1024 in bf16: 101 us, prompt_tiles 46.5).  8 of 512 with heads of 128 in fp32: 197 us.
+// prompt_rows (what is left: wider heads, scales that are not positive, short sequences): a warp has 16 queries, its operands and sums in registers as mma.sync takes them (mma_sync.cuh);
+// keys and values of a tile go through shared memory for the four warps of a CTA, asked for one tile ahead.  Rows in shared memory are 64 (keys) and 16 bytes (values) longer than a
+// power of two, so that the 16-byte pieces that eight lanes read together lie in different banks.  It is bounded by the instructions around mma.sync (fp32: splitting) and, with one block to a
+// sequence, by its chain of loads, products and exp2: 12 heads of 64, one prompt of 37 tokens in fp32 9 us with the call, 32 prompts of 100 tokens in bf16 12 us (8 of 512 in fp32 92 us,
+// prompt_parts 33; 24 of up to 1024 in bf16 101 us, prompt_tiles 46.5); 8 of 512 with heads of 128 in fp32 197 us.
 #include "attention_tc.cuh"
 #include "early_launch.cuh"
 #include "gemm_split.cuh"
@@ -794,13 +795,14 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
 
 // ---- fp32 on tcgen05: operands of three bf16 parts each (attention_tc.cuh) ----
 //
-// x = x0 + x1 + x2, each part what bf16 holds of what is left: 24 bits.  Of the nine products of parts the six largest are multiplied, those left out are below 2^-22 of the whole; the sums of a
-// step are added to those of the steps before in registers, because the tensor cores cut off what they add to a sum (8 x 512 tokens: error of the outputs 2.4e-7, plain fp32 4.1e-7).
+// x = x0 + x1 + x2, each part what bf16 holds of what is left: 24 bits.  Of the nine products of parts the six largest are multiplied, those left out are below 2^-22 of the whole; the
+// sums of a step are added to those of the steps before in registers, because the tensor cores cut off what they add to a sum (8 x 512 tokens: error of the outputs 2.4e-7, plain
+// fp32 4.1e-7).
 //
-// What bounds it.  A step of a tile takes 3400 cycles of the tensor pipe (24 MMAs of 64 and 48 of 32 cycles at best), two tiles in turn; shared memory holds one buffer each of keys and values, so that
-// the splitting of the next ones (four warps, 0.5 us) follows their last use.  Each tile's own warps split its queries, beside the first keys (8 x 512 tokens, 12 heads of 64: 35.1 us,
-// split one after another by the same four warps 40.5), and what is split next is asked for while this is being split (33.7).  Of the 12 us that the products of the heaviest CTA
-// take, 5 us until the first, and the ends of the last tile come on top.  A warp to issue each tile's products, as prompt_tiles has for 64 features, gains nothing here.
+// What bounds it.  A step of a tile takes 3400 cycles of the tensor pipe (24 MMAs of 64 and 48 of 32 cycles at best), two tiles in turn; shared memory holds one buffer each of keys and
+// values, so that the splitting of the next ones (four warps, 0.5 us) follows their last use.  Each tile's own warps split its queries, beside the first keys (8 x 512 tokens, 12 heads
+// of 64: 35.1 us, split one after another by the same four warps 40.5), and what is split next is asked for while this is being split (33.7).  Beside the 12 us that the products of the
+// heaviest CTA take there are 5 us until the first, and the ends of the last tile.  A warp to issue each tile's products, as prompt_tiles has for 64 features, gains nothing here.
 
 // Eight features of a row to the three parts of a tile.
 __device__ __forceinline__ void split_piece(const float4 (&v)[2], char *put) {
