@@ -5,11 +5,13 @@
 // prompt_tiles (16 bits, up to 128 features) and prompt_parts (fp32, up to 64): tcgen05, two tiles of 128 rows to a CTA, warps with a role each; attention_tc.cuh has the plan, what
 // bounds it and what it measured.
 //
-// prompt_rows (what is left: wider heads, scales that are not positive, short sequences): a warp has 16 queries, its operands and sums in registers as mma.sync takes them (mma_sync.cuh);
+// prompt_rows (what is left: wider heads, scales that are not positive, short sequences, few rows over many keys): a warp has 16 queries, its operands and sums in registers as mma.sync takes them (mma_sync.cuh);
 // keys and values of a tile go through shared memory for the four warps of a CTA, asked for one tile ahead.  Rows in shared memory are 64 (keys) and 16 bytes (values) longer than a
 // power of two, so that the 16-byte pieces that eight lanes read together lie in different banks.  It is bounded by the instructions around mma.sync (fp32: splitting) and, with one block to a
 // sequence, by its chain of loads, products and exp2: 12 heads of 64, one prompt of 37 tokens in fp32 9 us with the call, 32 prompts of 100 tokens in bf16 12 us (8 of 512 in fp32 92 us,
 // prompt_parts 33; 24 of up to 1024 in bf16 101 us, prompt_tiles 46.5); 8 of 512 with heads of 128 in fp32 197 us.
+// Where there are few blocks, the CTAs of a cluster walk the tiles of one in turn and join maxima, sums and values through each other's shared memory, in the order of their ranks: 8 heads of 128,
+// one query over 30000 keys in bf16 108 us instead of 392 (prompt_tiles), 4 queries of 12 heads of 64 over 2004 keys in fp32 19 instead of 75 (prompt_parts).
 #include "attention_tc.cuh"
 #include "early_launch.cuh"
 #include "gemm_split.cuh"
@@ -82,6 +84,15 @@ __device__ __forceinline__ void copy16(unsigned to, const char *from, bool ok) {
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
+// A cluster's CTAs: how many, a wait for all of them, and a value that one of them has in shared memory where this one has `at`.
+__device__ __forceinline__ unsigned cluster_size() { unsigned n; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n)); return n; }
+__device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ float load_of_rank(unsigned at, unsigned rank) {
+    float v;
+    asm volatile("{\n\t.reg .u32 x;\n\tmapa.shared::cluster.u32 x, %1, %2;\n\tld.shared::cluster.f32 %0, [x];\n\t}" : "=f"(v) : "r"(at), "r"(rank) : "memory");
+    return v;
+}
+
 template <int TYPE, int DIM>
 struct Rows {
     static constexpr int SIZE = TYPE == ASPEN_B200_FP32 ? 4 : 2, VALUES = 16 / SIZE, BYTES = DIM * SIZE;
@@ -98,7 +109,8 @@ struct Rows {
     static constexpr int TURN = HELD || SIZE == 2 ? PIECES : 1;
 };
 
-template <int TYPE, int DIM>
+// SPLIT: the CTAs of a cluster walk a block's tiles in turn, and join what they have.
+template <int TYPE, int DIM, bool SPLIT>
 __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
     typedef Rows<TYPE, DIM> R;
     constexpr int SIZE = R::SIZE, VALUES = R::VALUES, KT = R::KEYS / 8;
@@ -106,7 +118,8 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
     const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane >> 2, t = lane & 3, head = blockIdx.y, kv_head = head / a.group;
     Block b;
     attn::wait_for_previous_kernel();
-    if (!find_block(a, blockIdx.x, R::QUERIES, b)) return;
+    const unsigned ranks = SPLIT ? cluster_size() : 1u, rank = SPLIT ? blockIdx.x % ranks : 0u;
+    if (!find_block(a, blockIdx.x / ranks, R::QUERIES, b)) return;
     const int behind = b.keys - b.queries;                      // query i sees keys up to i + behind
     const int last = min(b.queries, b.first + R::QUERIES) - 1;
     const int end = a.masked ? min(b.keys, last + behind + 1) : b.keys;
@@ -125,7 +138,7 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
         copies_done();
     };
     const int tiles = end > 0 ? (end + R::KEYS - 1) / R::KEYS : 0;
-    if (tiles > 0) fetch(0, 0);
+    if ((int)rank < tiles) fetch((int)rank, 0);
     // queries, rows g and g + 8 of the warp's 16
     const char *const q = a.q + ((size_t)b.q0 * a.q_row + (size_t)head * a.q_head) * SIZE;
     char *const own = smem + 2 * R::STAGE + warp * 16 * R::KPITCH;
@@ -147,10 +160,10 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
     for (int i = 0; i < DIM / 8; i++)
         #pragma unroll
         for (int j = 0; j < 4; j++) o[i][j] = 0.f;
-    for (int tile = 0; tile < tiles; tile++) {
-        if (tile + 1 < tiles) { fetch(tile + 1, (tile + 1) & 1); wait_copies<1>(); } else wait_copies<0>();
+    for (int tile = (int)rank, stage = 0; tile < tiles; tile += (int)ranks, stage ^= 1) {
+        if (tile + (int)ranks < tiles) { fetch(tile + (int)ranks, stage ^ 1); wait_copies<1>(); } else wait_copies<0>();
         __syncthreads();
-        const char *const ks = smem + (tile & 1) * R::STAGE, *const vs = ks + R::KEYS * R::KPITCH;
+        const char *const ks = smem + stage * R::STAGE, *const vs = ks + R::KEYS * R::KPITCH;
         float s[KT][4];
         #pragma unroll
         for (int n = 0; n < KT; n++)
@@ -251,41 +264,91 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
     for (int h = 0; h < 2; h++) {
         sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
         sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+    }
+    // column n = 2 t + c of tile j holds the value j of piece n
+    constexpr int PER = TYPE == ASPEN_B200_FP32 ? 4 : 8;
+    auto store = [&](int h, int c, int i, const float *x) {
         const int row = h ? row8 : row0;
-        if (row >= b.queries) continue;
-        const float inv = sum[h] == 0.f ? 0.f : 1.f / sum[h];
-        char *const out = a.out + ((size_t)(b.q0 + row) * a.out_row + (size_t)head * a.out_head) * SIZE;
-        // column n = 2 t + c of tile j holds the value j of piece n
-        constexpr int PER = TYPE == ASPEN_B200_FP32 ? 4 : 8;
+        const unsigned f = i * 8 * PER + (2 * t + c) * PER;
+        if (row >= b.queries || f >= a.head_dim) return;
+        char *const out = a.out + ((size_t)(b.q0 + row) * a.out_row + (size_t)head * a.out_head + f) * SIZE;
+        if constexpr (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float4 *>(out) = make_float4(x[0], x[1], x[2], x[3]);
+        else {
+            typedef mma::Of<TYPE> T;
+            *reinterpret_cast<uint4 *>(out) = make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
+        }
+    };
+    if constexpr (!SPLIT) {
         #pragma unroll
-        for (int i = 0; i < R::VPIECES; i++)
+        for (int h = 0; h < 2; h++) {
+            const float inv = sum[h] == 0.f ? 0.f : 1.f / sum[h];
             #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const unsigned f = i * 8 * PER + (2 * t + c) * PER;
-                float x[PER];
+            for (int i = 0; i < R::VPIECES; i++)
                 #pragma unroll
-                for (int j = 0; j < PER; j++) x[j] = o[i * PER + j][2 * h + c] * inv;
-                if (f >= a.head_dim) continue;
-                if constexpr (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float4 *>(out + f * SIZE) = make_float4(x[0], x[1], x[2], x[3]);
-                else {
-                    typedef mma::Of<TYPE> T;
-                    *reinterpret_cast<uint4 *>(out + f * SIZE) = make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
+                for (int c = 0; c < 2; c++) {
+                    float x[PER];
+                    #pragma unroll
+                    for (int j = 0; j < PER; j++) x[j] = o[i * PER + j][2 * h + c] * inv;
+                    store(h, c, i, x);
                 }
+        }
+    } else {
+        // [value of a thread][thread]; a thread joins every `ranks`-th piece of its own place
+        float *const mine = reinterpret_cast<float *>(smem) + threadIdx.x;
+        constexpr int STATS = DIM / 8 * 4;
+        static_assert((STATS + 4) * R::THREADS * 4 <= 2 * R::STAGE, "in place of keys and values");
+        #pragma unroll
+        for (int i = 0; i < DIM / 8; i++)
+            #pragma unroll
+            for (int j = 0; j < 4; j++) mine[(i * 4 + j) * R::THREADS] = o[i][j];
+        #pragma unroll
+        for (int h = 0; h < 2; h++) { mine[(STATS + h) * R::THREADS] = max[h]; mine[(STATS + 2 + h) * R::THREADS] = sum[h]; }
+        cluster_barrier();
+        const unsigned at = shared_address(mine);
+        for (unsigned q = rank; q < 4 * R::VPIECES; q += ranks) {
+            const int h = (int)(q & 1u), c = (int)(q >> 1 & 1u), i = (int)(q >> 2);
+            float most = -INFINITY, all = 0.f, x[PER];
+            #pragma unroll
+            for (int j = 0; j < PER; j++) x[j] = 0.f;
+            for (unsigned r = 0; r < ranks; r++) most = fmaxf(most, load_of_rank(at + (STATS + h) * R::THREADS * 4, r));
+            const float ref = most == -INFINITY ? 0.f : most;
+            for (unsigned r = 0; r < ranks; r++) {
+                const float w = mma::exp2_fast(load_of_rank(at + (STATS + h) * R::THREADS * 4, r) - ref);
+                all = fmaf(w, load_of_rank(at + (STATS + 2 + h) * R::THREADS * 4, r), all);
+                #pragma unroll
+                for (int j = 0; j < PER; j++) x[j] = fmaf(w, load_of_rank(at + ((i * PER + j) * 4 + 2 * h + c) * R::THREADS * 4, r), x[j]);
             }
+            const float inv = all == 0.f ? 0.f : 1.f / all;
+            #pragma unroll
+            for (int j = 0; j < PER; j++) x[j] *= inv;
+            store(h, c, i, x);
+        }
+        cluster_barrier();                          // the others have read what is here
     }
 }
 
+// CTAs to a block.  Few blocks leave SMs without work; up to 8 CTAs share a block's keys then, 128 or more each, as long as all of them run at once.  An SM has room for two, heads of 256
+// features for one.
+unsigned blocks_of(const Args &a) { return a.q_rows / 64 + (a.sequences < a.q_rows ? a.sequences : a.q_rows); }
+unsigned ranks_of(const Args &a, unsigned sms) {
+    const unsigned long long blocks = (unsigned long long)blocks_of(a) * a.heads, room = a.head_dim <= 128 ? 2 * sms : sms;
+    const unsigned keys = a.kv_rows / a.sequences;
+    unsigned ranks = 1;
+    while (ranks < 8 && blocks * ranks * 2 <= room && keys >= ranks * 256) ranks *= 2;
+    return ranks;
+}
 template <int TYPE, int DIM>
-cudaError_t launch_rows(const Args &a, cudaStream_t stream) {
+cudaError_t launch_rows(const Args &a, unsigned ranks, cudaStream_t stream) {
     typedef Rows<TYPE, DIM> R;
-    cudaError_t err = cudaFuncSetAttribute(prompt_rows<TYPE, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM);
+    static_assert(R::QUERIES == 64 && R::SMEM <= (DIM <= 128 ? 112 : 226) * 1024, "as blocks_of and ranks_of have it");
+    void (*const kernel)(Args) = ranks > 1 ? prompt_rows<TYPE, DIM, true> : prompt_rows<TYPE, DIM, false>;
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM);
     if (err != cudaSuccess) return err;
-    const unsigned blocks = a.q_rows / R::QUERIES + (a.sequences < a.q_rows ? a.sequences : a.q_rows);
-    return attn::launch_early(prompt_rows<TYPE, DIM>, dim3(blocks, a.heads), R::THREADS, R::SMEM, stream, a);
+    return attn::launch_early_in_clusters(ranks, kernel, dim3(blocks_of(a) * ranks, a.heads), R::THREADS, R::SMEM, stream, a);
 }
 template <int TYPE>
-cudaError_t launch_rows(const Args &a, cudaStream_t stream) {
-    return a.head_dim <= 64 ? launch_rows<TYPE, 64>(a, stream) : a.head_dim <= 128 ? launch_rows<TYPE, 128>(a, stream) : launch_rows<TYPE, 256>(a, stream);
+cudaError_t launch_rows(const Args &a, unsigned ranks, cudaStream_t stream) {
+    return a.head_dim <= 64 ? launch_rows<TYPE, 64>(a, ranks, stream) : a.head_dim <= 128 ? launch_rows<TYPE, 128>(a, ranks, stream) : launch_rows<TYPE, 256>(a, ranks, stream);
 }
 
 // ---- tcgen05 (attention_tc.cuh) ----
@@ -1189,9 +1252,12 @@ cudaError_t launch_tiles(const Args &a, const CUtensorMap *maps, cudaStream_t st
     return attn::launch_early(prompt_tiles<TYPE, DIM>, (unsigned)jobs_of(a), fused::THREADS, fused::Shape<DIM>::SMEM, stream, maps[0], maps[1], maps[2], a, a.heads / a.group);
 }
 // False: not a call for these kernels.
-bool try_tiles(const Args &a, int type, cudaStream_t stream, cudaError_t *err) {
+bool try_tiles(const Args &a, int type, unsigned ranks, cudaStream_t stream, cudaError_t *err) {
     // a row's largest score is its largest product only for a scale above 0
     if (!a.kv_rows || !(a.scale > 0.f) || a.group > fused::TILE || jobs_of(a) > 0x7fffffffull) return false;
+    // A step of 128 keys takes a CTA about half as long as two tiles of 64 take one of prompt_rows, so four of these beside each other are faster, where there is room for them: 12 heads of 64, two
+    // sequences of 16 queries over 2016 keys 12.4 us, in tiles 24.4; one prompt of 512 tokens, 8 heads of 64, 9.0 and 11.8 (fp32 17.6 and 27.5).
+    if (ranks >= 4) return false;
     // Short sequences, going by the mean: a job of one step takes 4 us (fp32 5), and a block of prompt_rows 1.2 (3), several at once on an SM.  12 heads of 64, bf16 and fp32, 32 prompts of 60
     // tokens 8.6 and 14.3 us (in tiles 14.5 and 21), of 100 tokens 12 and 35 (14.5 and 24.6); 8 heads of 128, fp16, of 96 tokens 14.7 (12.5).  Where one sequence of a few is long and the others
     // short, the blocks take up to three times as long, of 4096 rows at most.
@@ -1259,8 +1325,9 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     a.scale = p->scale * 1.4426950408889634f;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t err = cudaSuccess;
-    if (!try_tiles(a, p->type, stream, &err))
-        err = p->type == ASPEN_B200_FP32 ? launch_rows<ASPEN_B200_FP32>(a, stream) : p->type == ASPEN_B200_BF16 ? launch_rows<ASPEN_B200_BF16>(a, stream) : launch_rows<ASPEN_B200_FP16>(a, stream);
+    const unsigned ranks = ranks_of(a, (unsigned)sms);
+    if (!try_tiles(a, p->type, ranks, stream, &err))
+        err = p->type == ASPEN_B200_FP32 ? launch_rows<ASPEN_B200_FP32>(a, ranks, stream) : p->type == ASPEN_B200_BF16 ? launch_rows<ASPEN_B200_BF16>(a, ranks, stream) : launch_rows<ASPEN_B200_FP16>(a, ranks, stream);
     if (err != cudaSuccess) { cudaGetLastError(); ASPEN_ERR("%s: %s\n", what, cudaGetErrorString(err)); return -3; }
     return 0;
 }

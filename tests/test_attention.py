@@ -479,6 +479,63 @@ def test_many_more_pieces_of_work_than_multiprocessors(kind, dim):
             check(got[a:b], want, away, size, kind)
 
 
+FEW_ROWS = [  # heads, kv_heads, dim, lengths of queries, lengths of keys: CTAs of a cluster share a block's keys, two to eight of them
+    (2, 1, 8, [1], [4000]), (4, 4, 64, [1, 5], [1500, 900]), (3, 3, 96, [70, 3, 0], [20, 4000, 7]), (6, 2, 128, [100], [100 + 513]), (2, 2, 256, [65, 1], [70, 1200]), (2, 2, 128, [200], [300]),
+    (1, 1, 256, [1], [257]), (8, 2, 80, [1, 1, 1], [0, 2049, 128]), (2, 2, 32, [1000], [1000]), (2, 1, 64, [300], [700])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("masked", [True, False], ids=["masked", "full"])
+@pytest.mark.parametrize("heads,kv_heads,dim,q_len,kv_len", FEW_ROWS)
+def test_few_rows_over_many_keys(heads, kv_heads, dim, q_len, kv_len, masked, kind):
+    """Keys and values of nobody, NaN, stand between the sequences; out's rows of nobody stay."""
+    rng = np.random.default_rng(dim + sum(kv_len))
+    q_starts, kv_starts = np.concatenate([[0], np.cumsum(q_len)]), np.concatenate([[0], np.cumsum(kv_len)]) + 3
+    q = rounded(rng.standard_normal((q_starts[-1] + 2, heads, dim)) * 1.5, kind)
+    k, v = (rounded(rng.standard_normal((kv_starts[-1] + 9, kv_heads, dim)), kind) for _ in range(2))
+    for a in (k, v):
+        a[:3] = a[kv_starts[-1]:] = np.nan
+    got = prompt(*(to_device(a, kind) for a in (q, k, v)), q_starts, kv_starts, kind, masked, dim ** -0.5)
+    for s in range(len(q_len)):
+        a, b, x, y = q_starts[s], q_starts[s + 1], kv_starts[s], kv_starts[s + 1]
+        want, away, size = attend(q[a:b], k[x:y], v[x:y], dim ** -0.5, seen_by(b - a, y - x, masked))
+        check(got[a:b], want, away, size, kind)
+    assert got[q_starts[-1]:].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("dim", [64, 256])
+def test_few_rows_with_a_nan_an_infinity_and_nothing_to_see(kind, dim):
+    """A NaN key makes its rows NaN whichever CTA has it; scores of -inf everywhere and rows before the first key give what one CTA gives: NaN and zeros."""
+    rng = np.random.default_rng(4)
+    q, k, v = (rounded(rng.standard_normal((n, 2, dim)), kind) for n in (12, 2000, 2000))
+    k[1500, 1, 3] = np.nan
+    got = prompt(*(to_device(a, kind) for a in (q, k, v)), [0, 12], [0, 2000], kind, False, 0.1)
+    assert got[:, 1].isnan().all()
+    want, away, size = attend(q[:, :1], k[:, :1], v[:, :1], 0.1, seen_by(12, 2000, False))
+    check(got[:, :1], want, away, size, kind)
+    # two sequences: one without keys, one whose first queries see none
+    got = prompt(*(to_device(a, kind) for a in (q, k[:1024], v[:1024])), [0, 5, 12], [0, 0, 4], kind, True, 0.1)
+    assert (got[:8] == 0).all() and got[8:, 0].isfinite().all() and (got[8:, 0] != 0).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("masked", [True, False], ids=["masked", "full"])
+@pytest.mark.parametrize("kv_heads,dim", [(4, 64), (16, 64), (4, 128), (16, 80)])
+def test_long_prompts_of_many_heads(kv_heads, dim, masked, kind):
+    rng = np.random.default_rng(kv_heads + dim)
+    starts = np.array([0, 700, 1001])
+    q, k, v = (rounded(rng.standard_normal((1001, h, dim)), kind) for h in (16, kv_heads, kv_heads))
+    got = prompt(*(to_device(a, kind) for a in (q, k, v)), starts, starts, kind, masked, dim ** -0.5)
+    for s in range(2):
+        a, b = starts[s], starts[s + 1]
+        want, away, size = attend(q[a:b], k[a:b], v[a:b], dim ** -0.5, seen_by(b - a, b - a, masked))
+        check(got[a:b], want, away, size, kind)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,keys", [(api.BF16, 3 << 27), (api.FP32, 1 << 27)], ids=["bf16", "fp32"])
 def test_a_single_query_over_keys_for_seconds(kind, keys):
@@ -486,7 +543,8 @@ def test_a_single_query_over_keys_for_seconds(kind, keys):
     import torch
     k, v = (torch.zeros((keys, 1, 8), dtype=torch_type(kind), device="cuda") for _ in range(2))
     k[-1], v[-1] = 40, 3
-    got = prompt(torch.ones((1, 1, 8), dtype=torch_type(kind), device="cuda"), k, v, [0, 1], [0, keys], kind, False, 0.5)
+    # heads enough that CTAs do not share the keys
+    got = prompt(torch.ones((1, 96, 8), dtype=torch_type(kind), device="cuda"), k, v, [0, 1], [0, keys], kind, False, 0.5)
     assert (got == 3).all()
 
 
@@ -608,6 +666,37 @@ def test_a_captured_prompt_follows_the_starts(kind, dim):
             want, away, size = attend(q[a:b], k[a:b], v[a:b], 0.2, seen_by(b - a, b - a, True))
             check(out[a:b], want, away, size, kind)
         assert out[ends[-1]:].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dim", [(api.FP32, 64), (api.BF16, 128)], ids=str)
+def test_a_captured_call_of_few_rows_follows_the_starts(kind, dim):
+    """Two calls in a row in the graph, the second of which attends to what the first has written; CTAs share the keys of a block."""
+    import torch
+    rng = np.random.default_rng(31)
+    q, k, v = (rounded(rng.standard_normal((n, 2, dim)), kind) for n in (20, 2100, 2100))
+    dq, dk, dv = (to_device(a, kind) for a in (q, k, v))
+    first, second, q_starts, kv_starts = torch.full_like(dq, math.nan), torch.full_like(dq, math.nan), ints([0, 0, 0]), ints([0, 0, 0])
+    def args(q, out):
+        return api.PromptArgs(type=kind, heads=2, kv_heads=2, head_dim=dim, masked=1, scale=0.2, sequences=2, q_rows=20, kv_rows=2100, q_starts=q_starts.data_ptr(), kv_starts=kv_starts.data_ptr(),
+                              q=q.data_ptr(), k=dk.data_ptr(), v=dv.data_ptr(), out=out.data_ptr())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        api.attention_prompt(args(dq, first), torch.cuda.current_stream().cuda_stream)
+        api.attention_prompt(args(first, second), torch.cuda.current_stream().cuda_stream)
+    for qs, ks in (([0, 20, 20], [0, 2100, 2100]), ([0, 1, 20], [0, 900, 930]), ([0, 0, 7], [5, 5, 1800])):
+        first.fill_(math.nan); second.fill_(math.nan)
+        q_starts.copy_(ints(qs)); kv_starts.copy_(ints(ks))
+        graph.replay()
+        torch.cuda.synchronize()
+        between = first.float().cpu().numpy().astype(np.float64)
+        for s in range(2):
+            a, b, x, y = qs[s], qs[s + 1], ks[s], ks[s + 1]
+            for given, got in ((q, first), (between, second)):
+                want, away, size = attend(given[a:b], k[x:y], v[x:y], 0.2, seen_by(b - a, y - x, True))
+                check(got[a:b], want, away, size, kind)
+        assert first[qs[2]:].isnan().all() and second[qs[2]:].isnan().all()
 
 
 # ---- the pool's books --------------------------------------------------------------------------------------------------------
