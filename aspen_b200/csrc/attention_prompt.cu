@@ -328,10 +328,11 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
 }
 
 // CTAs to a block.  Few blocks leave SMs without work; up to 8 CTAs share a block's keys then, 128 or more each, as long as all of them run at once.  An SM has room for two, heads of 256
-// features for one.
+// features for one.  Wide fp32 heads with a mask take two rounds of CTAs: their last blocks have twice the keys of the mean (one prompt of 549 tokens, 21 heads of 128, 84 us instead of 112; bf16
+// heads of 256, two of 400 tokens, take 37 instead of 24).
 unsigned blocks_of(const Args &a) { return a.q_rows / 64 + (a.sequences < a.q_rows ? a.sequences : a.q_rows); }
-unsigned ranks_of(const Args &a, unsigned sms) {
-    const unsigned long long blocks = (unsigned long long)blocks_of(a) * a.heads, room = a.head_dim <= 128 ? 2 * sms : sms;
+unsigned ranks_of(const Args &a, int type, unsigned sms) {
+    const unsigned long long blocks = (unsigned long long)blocks_of(a) * a.heads, rounds = type == ASPEN_B200_FP32 && a.head_dim > 64 && a.masked ? 2 : 1, room = a.head_dim <= 128 ? 2 * sms * rounds : sms;
     const unsigned keys = a.kv_rows / a.sequences;
     unsigned ranks = 1;
     while (ranks < 8 && blocks * ranks * 2 <= room && keys >= ranks * 256) ranks *= 2;
@@ -1325,7 +1326,7 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     a.scale = p->scale * 1.4426950408889634f;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t err = cudaSuccess;
-    const unsigned ranks = ranks_of(a, (unsigned)sms);
+    const unsigned ranks = ranks_of(a, p->type, (unsigned)sms);
     if (!try_tiles(a, p->type, ranks, stream, &err))
         err = p->type == ASPEN_B200_FP32 ? launch_rows<ASPEN_B200_FP32>(a, ranks, stream) : p->type == ASPEN_B200_BF16 ? launch_rows<ASPEN_B200_BF16>(a, ranks, stream) : launch_rows<ASPEN_B200_FP16>(a, ranks, stream);
     if (err != cudaSuccess) { cudaGetLastError(); ASPEN_ERR("%s: %s\n", what, cudaGetErrorString(err)); return -3; }
