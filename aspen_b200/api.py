@@ -363,9 +363,9 @@ def attention_prompt(args: PromptArgs, stream: int = 0) -> None:
 
 class Cache(C.Structure):
     """aspen_b200_cache_t and the calls on it: a paged key-value cache in device memory of the caller.  All pointers are device addresses;
-    every call enqueues on `stream` and returns."""
+    every call enqueues on `stream` and returns.  `refused` may be 0 where the status is looked at behind every extend and fork."""
     _fields_ = _struct("k v page_table lengths refs status", "layer_stride page_stride head_stride token_stride", "type",
-                       "layers pages page_size kv_heads head_dim sequences max_pages")
+                       "layers pages page_size kv_heads head_dim sequences max_pages") + [("refused", C.c_void_p)]
 
     def workspace(self, entries: int = 0) -> int:
         """Bytes for extend and fork of so many entries, and for compact."""

@@ -54,6 +54,7 @@ Pages pages_of(const aspen_b200_cache_t &c) {
     p.head_stride = packed(c.head_stride, p.token_stride * c.page_size);
     p.page_stride = packed(c.page_stride, p.head_stride * c.kv_heads);
     p.pages = c.pages; p.page_size = c.page_size; p.sequences = c.sequences; p.max_pages = c.max_pages;
+    p.refused = c.refused;
     return p;
 }
 

@@ -23,6 +23,7 @@ struct Pages {
     int *status;
     size_t page_stride, head_stride, token_stride;
     unsigned pages, page_size, sequences, max_pages;
+    int *refused;                       // or nullptr
 };
 
 // Tokens of a sequence: 0 for one that does not exist, never more than its row of the table has room for.
@@ -32,6 +33,8 @@ ATTN_FN unsigned sequence_length(const Pages &c, int slot) {
     const unsigned room = c.max_pages * c.page_size;         // < 2^31 (checked)
     return n <= 0 ? 0u : (unsigned)n < room ? (unsigned)n : room;
 }
+// A sequence that a refused call would have given tokens to; also where the cache keeps no list of them: never.
+ATTN_FN bool is_refused(const Pages &c, int slot) { return c.refused && slot >= 0 && (unsigned)slot < c.sequences && c.refused[slot] != 0; }
 // Offset of a token's first row (of head 0) in elements; -1 if its page does not exist.  The token is below sequence_length.
 ATTN_FN long long token_offset(const Pages &c, int slot, unsigned token) {
     const unsigned i = token / c.page_size;

@@ -103,6 +103,15 @@ __device__ unsigned lowest_free(const int *refs, unsigned pages, unsigned want, 
     return found < want ? found : want;
 }
 
+// The sequences that a refused call would have given tokens to.
+__device__ __forceinline__ void refuse(const Pool &pool, const int *slots, unsigned entries) {
+    if (!pool.at.refused) return;
+    for (unsigned e = threadIdx.x; e < entries; e += BOOK) {
+        const int slot = slots ? slots[e] : (int)e;
+        if (slot >= 0 && (unsigned)slot < pool.at.sequences) pool.at.refused[slot] = 1;
+    }
+}
+
 __device__ __forceinline__ unsigned pages_for(unsigned long long tokens, unsigned page) { return (unsigned)((tokens + page - 1) / page); }
 
 __global__ void __launch_bounds__(BOOK) extend_kernel(const Pool pool, const Space w, const int *slots, const int *starts, unsigned entries) {
@@ -124,6 +133,7 @@ __global__ void __launch_bounds__(BOOK) extend_kernel(const Pool pool, const Spa
             const long long more = starts ? (long long)starts[e + 1] - starts[e] : 1;
             if (slot < 0 || (unsigned)slot >= pool.at.sequences || more < 0) why |= ASPEN_B200_CACHE_BAD_INDEX;
             else if (slots && atomicAdd(&w.mark[slot], 1) != 0) why |= ASPEN_B200_CACHE_BAD_INDEX;
+            else if (attn::is_refused(pool.at, slot)) why |= ASPEN_B200_CACHE_REFUSED;
             else {
                 const unsigned now = attn::sequence_length(pool.at, slot);
                 const unsigned long long then = now + (unsigned long long)more;
@@ -145,6 +155,7 @@ __global__ void __launch_bounds__(BOOK) extend_kernel(const Pool pool, const Spa
         __syncthreads();
     }
     if (refused) {
+        refuse(pool, slots, entries);
         if (threadIdx.x == 0) atomicOr(pool.at.status, refused | ASPEN_B200_CACHE_REFUSED);
         return;
     }
@@ -193,6 +204,7 @@ __global__ void __launch_bounds__(BOOK) fork_kernel(const Pool pool, const Space
             unsigned len = 0;
             if (a < 0 || (unsigned)a >= pool.at.sequences || b < 0 || (unsigned)b >= pool.at.sequences) why |= ASPEN_B200_CACHE_BAD_INDEX;
             else if (atomicAdd(&w.mark[b], 1) != 0 || pool.lengths[b] != 0) why |= ASPEN_B200_CACHE_BAD_INDEX;
+            else if (attn::is_refused(pool.at, a) || attn::is_refused(pool.at, b)) why |= ASPEN_B200_CACHE_REFUSED;
             else {
                 len = attn::sequence_length(pool.at, a);
                 part = len % page != 0;
@@ -218,8 +230,9 @@ __global__ void __launch_bounds__(BOOK) fork_kernel(const Pool pool, const Space
     }
     if (!refused)
         for (unsigned i = threadIdx.x; i < total; i += BOOK) pool.refs[w.to[i]] = 1;
+    else refuse(pool, to, entries);
     if (threadIdx.x == 0) {
-        if (refused) atomicOr(pool.at.status, refused);
+        if (refused) atomicOr(pool.at.status, refused | (pool.at.refused ? ASPEN_B200_CACHE_REFUSED : 0));
         w.head[OK] = !refused;
     }
 }
@@ -312,6 +325,7 @@ __global__ void __launch_bounds__(COPY) free_kernel(const Pool pool, const int *
     const unsigned room = pool.at.max_pages * pool.at.page_size;
     if (threadIdx.x == 0) {
         // the first to take the length frees the pages
+        if (pool.at.refused) pool.at.refused[slot] = 0;
         const int n = atomicExch(&pool.lengths[slot], 0);
         length = n <= 0 ? 0u : (unsigned)n < room ? (unsigned)n : room;
     }
@@ -417,8 +431,8 @@ struct New {
 __global__ void __launch_bounds__(COPY) append_kernel(const Pages at /* strides in vectors */, const New n) {
     const unsigned lane = threadIdx.x % 32, r = blockIdx.x * (COPY / 32) + threadIdx.x / 32;
     wait_for_previous_kernel();
-    // behind an extend that was refused the last places of a sequence are not the new tokens'
-    if (r >= n.rows || *reinterpret_cast<volatile int *>(at.status) & ASPEN_B200_CACHE_REFUSED) return;
+    // behind an extend that was refused the last places of a sequence are not the new tokens'; without a list of such sequences that goes for all
+    if (r >= n.rows || (!at.refused && *reinterpret_cast<volatile int *>(at.status) & ASPEN_B200_CACHE_REFUSED)) return;
     unsigned e = r;
     int begin = (int)r, end = (int)r + 1;
     if (n.starts) {
@@ -437,6 +451,7 @@ __global__ void __launch_bounds__(COPY) append_kernel(const Pages at /* strides 
     }
     if (begin > (int)r || end <= (int)r) { if (lane == 0) atomicOr(at.status, ASPEN_B200_CACHE_BAD_INDEX); return; }
     const int slot = e >= n.entries ? -1 : n.slots ? n.slots[e] : (int)e;
+    if (attn::is_refused(at, slot)) return;
     const long long position = (long long)attn::sequence_length(at, slot) - ((long long)end - r);
     const long long offset = position < 0 ? -1 : attn::token_offset(at, slot, (unsigned)position);
     if (offset < 0) { if (lane == 0) atomicOr(at.status, ASPEN_B200_CACHE_BAD_INDEX); return; }
@@ -502,8 +517,8 @@ extern "C" int aspen_b200_cache_extend(const aspen_b200_cache_t *cache, const in
     if (!rc) rc = check_space(cache, entries, workspace, workspace_bytes, what);
     if (rc || !entries) return rc;
     const attn::Named all[] = {{cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->refs, "refs"}, {cache->status, "status"},
-                               {slots, "slots"}, {starts, "starts"}, {workspace, "workspace"}};
-    if ((rc = attn::check_device(all, 7, what))) return rc;
+                               {slots, "slots"}, {starts, "starts"}, {workspace, "workspace"}, {cache->refused, "refused"}};
+    if ((rc = attn::check_device(all, 8, what))) return rc;
     return done(launch_early(extend_kernel, 1, BOOK, 0, static_cast<cudaStream_t>(cuda_stream), pool_of(*cache), space_of(*cache, entries, workspace), slots, starts, entries), what);
 }
 
@@ -520,8 +535,8 @@ extern "C" int aspen_b200_cache_append(const aspen_b200_cache_t *cache, unsigned
     if ((rc = attn::check_rows(a->k, a->k_row_stride, a->k_head_stride, cache->type, "k", what)) ||
         (rc = attn::check_rows(a->v, a->v_row_stride, a->v_head_stride, cache->type, "v", what))) return rc;
     const attn::Named all[] = {{cache->k, "the cache's k"}, {cache->v, "the cache's v"}, {cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->status, "status"},
-                               {a->k, "k"}, {a->v, "v"}, {a->slots, "slots"}, {a->starts, "starts"}};
-    if ((rc = attn::check_device(all, 9, what))) return rc;
+                               {a->k, "k"}, {a->v, "v"}, {a->slots, "slots"}, {a->starts, "starts"}, {cache->refused, "refused"}};
+    if ((rc = attn::check_device(all, 10, what))) return rc;
     const Plane p = plane_of(*cache);
     const size_t per = 16 / attn::type_size(cache->type);
     Pages at = attn::pages_of(*cache);
@@ -554,8 +569,8 @@ extern "C" int aspen_b200_cache_fork(const aspen_b200_cache_t *cache, const int 
     if (rc || !entries) return rc;
     if (!from || !to) { ASPEN_ERR("%s: no list of sequences\n", what); return -1; }
     const attn::Named all[] = {{cache->k, "the cache's k"}, {cache->v, "the cache's v"}, {cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->refs, "refs"},
-                               {cache->status, "status"}, {from, "from"}, {to, "to"}, {workspace, "workspace"}};
-    if ((rc = attn::check_device(all, 9, what))) return rc;
+                               {cache->status, "status"}, {from, "from"}, {to, "to"}, {workspace, "workspace"}, {cache->refused, "refused"}};
+    if ((rc = attn::check_device(all, 10, what))) return rc;
     const int sms = attn::sm_count(what);
     if (sms < 0) return sms;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
@@ -571,8 +586,8 @@ extern "C" int aspen_b200_cache_free(const aspen_b200_cache_t *cache, const int 
     if (!rc) rc = check_entries(entries, what);
     if (rc || !entries) return rc;
     if (!slots) { ASPEN_ERR("%s: no list of sequences\n", what); return -1; }
-    const attn::Named all[] = {{cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->refs, "refs"}, {cache->status, "status"}, {slots, "slots"}};
-    if ((rc = attn::check_device(all, 5, what))) return rc;
+    const attn::Named all[] = {{cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->refs, "refs"}, {cache->status, "status"}, {slots, "slots"}, {cache->refused, "refused"}};
+    if ((rc = attn::check_device(all, 6, what))) return rc;
     return done(launch_early(free_kernel, entries, COPY, 0, static_cast<cudaStream_t>(cuda_stream), pool_of(*cache), slots), what);
 }
 

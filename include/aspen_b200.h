@@ -319,27 +319,32 @@ int aspen_b200_attention_prompt(const aspen_b200_prompt_t *prompt, void *cuda_st
  *     page_table   [sequences][max_pages]: token t of sequence s is row t % page_size of page page_table[s][t / page_size], in every layer
  *     lengths      [sequences]: tokens
  *     refs         [pages]: how often page_table names the page; 0 = free
- *     status       a word to which the calls add ASPEN_B200_CACHE_* bits; the caller clears it */
+ *     status       a word to which the calls add ASPEN_B200_CACHE_* bits; the caller clears it
+ *     refused      [sequences], 0 at first, or NULL: a refused extend or fork writes 1 for each sequence that it would have given tokens to.  Such a sequence stays as it is: extend and
+ *                  fork refuse a call that names it, append leaves its rows out, until the caller writes 0 or it is freed.  Other sequences go on.
+ * A program that may call extend or fork behind a refusal it has not seen (a captured step, several batches in one pool) needs refused.  Without it append cannot tell the tokens of one
+ * extend from those of another: the status word stops it for all sequences, but extend goes on taking places, which stay unwritten; the program has to look at *status first. */
 typedef struct {
     void *k, *v;
     int *page_table, *lengths, *refs, *status;
     size_t layer_stride, page_stride, head_stride, token_stride;
     int type;
     unsigned int layers, pages, page_size, kv_heads, head_dim, sequences, max_pages;
+    int *refused;
 } aspen_b200_cache_t;
 #define ASPEN_B200_CACHE_BAD_INDEX 1    /* a sequence or page that does not exist, named twice where it must not be, or a fork onto one that is not empty */
 #define ASPEN_B200_CACHE_NO_PAGES 2     /* the pool has too few free pages, or one sequence asked for more than 2^21 at once */
 #define ASPEN_B200_CACHE_TOO_LONG 4     /* a sequence would need more than max_pages pages */
-#define ASPEN_B200_CACHE_REFUSED 8      /* an extend has changed nothing; until this bit is cleared, append writes nothing */
+#define ASPEN_B200_CACHE_REFUSED 8      /* an extend (with refused a fork, too) has changed nothing; without refused, append writes nothing until this bit is cleared */
 
 /* Bytes of workspace of extend, fork (entries: how many are given) and compact (0); 0 on bad arguments. */
 size_t aspen_b200_cache_workspace(const aspen_b200_cache_t *cache, unsigned int entries);
 /* Room for new tokens: entry i adds starts[i + 1] - starts[i] of them (starts NULL: one) to sequence slots[i] (slots NULL: i).  Pages are taken lowest number
- * first, in the order of the entries.  If an index is bad, a sequence is named twice or gets too long, or the pages do not suffice, nothing changes but the status. */
+ * first, in the order of the entries.  If an index is bad, a sequence is named twice or gets too long, or the pages do not suffice, nothing changes but status and refused. */
 int aspen_b200_cache_extend(const aspen_b200_cache_t *cache, const int *slots, const int *starts, unsigned int entries, void *workspace,
                             size_t workspace_bytes, void *cuda_stream);
 /* Writes keys and values of one layer behind an extend with the same slots and starts: row starts[i] + j is the token j of the starts[i + 1] - starts[i] that
- * sequence slots[i] was extended by last, as its length says.  Rows that have no such place are left out (status). */
+ * sequence slots[i] was extended by last, as its length says.  Rows that have no such place are left out (status), and those behind an extend that was refused (above). */
 typedef struct {
     const void *k, *v;             /* [rows][kv_heads][head_dim] */
     const int *slots, *starts;     /* [entries], [entries + 1], or NULL as in extend */
@@ -348,7 +353,7 @@ typedef struct {
 } aspen_b200_append_t;
 int aspen_b200_cache_append(const aspen_b200_cache_t *cache, unsigned int layer, const aspen_b200_append_t *append, void *cuda_stream);
 /* Sequence to[i] becomes a copy of sequence from[i] as it was before the call: full pages are shared, the tokens of a last page that is not full are copied in all
- * layers.  A sequence may be forked many times; each to[i] must be empty and named once, else (or without enough pages) nothing changes but the status. */
+ * layers.  A sequence may be forked many times; each to[i] must be empty and named once, else (or without enough pages) nothing changes but status and refused. */
 int aspen_b200_cache_fork(const aspen_b200_cache_t *cache, const int *from, const int *to, unsigned int entries, void *workspace, size_t workspace_bytes,
                           void *cuda_stream);
 /* Gives back the pages of the sequences, which become empty.  One that is named twice is freed once. */

@@ -1088,3 +1088,195 @@ def test_calls_on_two_streams_do_not_disturb_each_other():
     torch.cuda.synchronize()
     for o, (want, away, size) in zip(outs, wants):
         check(o, want, away, size, api.BF16)
+
+
+# ---- refusals and what comes behind them -------------------------------------------------------------------------------------
+
+def with_refused(pool):
+    pool.refused = ints(np.zeros(pool.lengths.numel()))
+    pool.cache.refused = pool.refused.data_ptr()
+    return pool
+
+
+class Sequences:
+    """Tokens with keys and values of their own, given to a pool call by call; `kept`: what each sequence has to hold."""
+
+    def __init__(self, pool):
+        self.pool, self.kept, self.next = pool, {s: [] for s in range(pool.lengths.numel())}, 1
+
+    def extend(self, slots, counts):
+        """The extend alone; returns its append."""
+        import torch
+        kv_heads, dim = self.pool.shape[2], self.pool.shape[4]
+        values = np.arange(self.next, self.next + sum(counts))
+        self.next += sum(counts)
+        at, starts = ints(slots), ints(np.concatenate([[0], np.cumsum(counts)]))
+        rows = torch.from_numpy(values).to(torch_type(self.pool.kind)).cuda()[:, None, None].expand(-1, kv_heads, dim).contiguous()
+        self.pool.cache.extend(at.data_ptr(), starts.data_ptr(), len(slots), *self.pool.space(len(slots)))
+
+        def append():
+            if len(values):
+                for layer in range(self.pool.shape[0]):
+                    self.pool.cache.append(layer, api.AppendArgs(k=rows.data_ptr(), v=rows.data_ptr(), slots=at.data_ptr(), starts=starts.data_ptr(), entries=len(slots), rows=len(values)))
+            torch.cuda.synchronize()
+        append.rows = [list(x) for x in np.split(values, np.cumsum(counts)[:-1])]
+        return append
+
+    def give(self, slots, counts, ok):
+        append = self.extend(slots, counts)
+        append()
+        if ok:
+            for s, rows in zip(slots, append.rows):
+                self.kept[s] += rows
+
+    def check(self):
+        table, lengths = self.pool.table.cpu().numpy(), self.pool.lengths.cpu().numpy()
+        page = self.pool.shape[3]
+        for s, rows in self.kept.items():
+            assert lengths[s] == len(rows), s
+            for c in (self.pool.k, self.pool.v):
+                held = c.float().cpu().numpy()
+                for t, x in enumerate(rows):
+                    assert (held[:, table[s, t // page], :, t % page] == x).all(), (s, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("why", ["pages", "length", "index", "twice"])
+def test_a_refused_extend_stops_its_sequences_and_no_others(why):
+    bit = dict(pages=api.CACHE_NO_PAGES, length=api.CACHE_TOO_LONG, index=api.CACHE_BAD_INDEX, twice=api.CACHE_BAD_INDEX)[why] | api.CACHE_REFUSED
+    pool = with_refused(Pool(api.FP16, 2, 8, 4, 6, 4, 4, layers=2))
+    s = Sequences(pool)
+    s.give([0, 1, 2], [3, 5, 2], True)
+    assert pool.status.item() == 0
+    bad = dict(pages=([0, 2], [10, 6]), length=([0, 2], [14, 1]), index=([0, 2, 4], [1, 1, 1]), twice=([0, 2, 0], [1, 1, 1]))[why]
+    late = s.extend([1], [1])                      # one that went through before, and is written behind the refusal
+    s.kept[1] += late.rows[0]
+    refused = s.extend(*bad)
+    late()
+    # the others go on, whatever the order of the calls; the refused ones' rows are not written
+    other = s.extend([1, 3], [1, 2])
+    refused()
+    other()
+    for x, rows in zip([1, 3], other.rows):
+        s.kept[x] += rows
+    s.check()
+    assert pool.status.item() == bit and pool.refused.tolist() == [1, 0, 1, 0]
+    # they stay as they are, and so does who is named with them, until the host has seen it
+    pool.status.zero_()
+    s.give([3, 2], [1, 1], False)
+    s.check()
+    assert pool.status.item() == api.CACHE_REFUSED and pool.refused.tolist() == [1, 0, 1, 1]
+    s.give([1], [1], True)
+    s.check()
+    pool.refused.zero_()
+    s.give([0, 3, 2], [1, 1, 1], True)
+    s.check()
+    assert pool.refused.tolist() == [0] * 4
+
+
+@pytest.mark.gpu
+def test_a_freed_sequence_is_no_longer_refused():
+    pool = with_refused(Pool(api.BF16, 1, 16, 4, 2, 3, 2))
+    s = Sequences(pool)
+    s.give([0], [5], True)
+    s.give([1, 2], [1, 1], False)
+    s.give([1], [0], False)
+    s.check()
+    assert pool.refused.tolist() == [0, 1, 1] and pool.status.item() == api.CACHE_NO_PAGES | api.CACHE_REFUSED
+    slots = ints([0, 1, 1])
+    pool.cache.free(slots.data_ptr(), 3)
+    s.kept[0] = []
+    s.give([1, 0], [4, 3], True)
+    s.check()
+    assert pool.refused.tolist() == [0, 0, 1]
+
+
+@pytest.mark.gpu
+def test_tokens_behind_a_refused_fork_go_nowhere():
+    pool = with_refused(Pool(api.FP32, 1, 8, 4, 3, 4, 2))
+    s = Sequences(pool)
+    s.give([0], [6], True)
+
+    def fork(sources, to):
+        a, b = ints(sources), ints(to)
+        pool.cache.fork(a.data_ptr(), b.data_ptr(), len(to), *pool.space(len(to)))
+
+    fork([0, 0], [2, 3])                           # one page is free, two are needed
+    s.give([2, 3], [1, 1], False)
+    s.give([0], [1], True)
+    s.check()
+    assert pool.status.item() == api.CACHE_NO_PAGES | api.CACHE_REFUSED and pool.refused.tolist() == [0, 0, 1, 1]
+    got = decode(pool, to_device(np.ones((4, 1, 8)), api.FP32), 1)
+    assert got[0].isfinite().all() and (got[0] != 0).all() and (got[1:] == 0).all()
+    # neither onto a refused one nor from one
+    pool.status.zero_()
+    fork([0], [2])
+    pool.refused[2] = 0
+    pool.refused[0] = 1
+    fork([0], [1])
+    s.check()
+    assert pool.status.item() == api.CACHE_REFUSED and pool.refused.tolist() == [1, 1, 0, 1]
+    pool.refused.zero_()
+    fork([0], [2])
+    s.kept[2] = list(s.kept[0])
+    s.check()
+    s.give([2], [1], True)
+    s.check()
+    assert pool.refused.tolist() == [0] * 4
+
+
+@pytest.mark.gpu
+def test_captured_steps_go_on_behind_a_refusal():
+    """Two batches in one pool, a captured step each, replayed without a look at the status: the one that finds no pages stands still, also when there are pages again, until its sequences
+    are freed or set to go on."""
+    import torch
+    pool = with_refused(Pool(api.BF16, 1, 8, 2, 6, 4, 4))
+    kept, steps = {s: [] for s in range(4)}, []
+    for slots in ([0, 1], [2, 3]):
+        at, row = ints(slots), torch.zeros(2, 1, 8, dtype=torch.bfloat16, device="cuda")
+        space = torch.empty(pool.cache.workspace(2), dtype=torch.uint8, device="cuda")
+        args = api.AppendArgs(k=row.data_ptr(), v=row.data_ptr(), slots=at.data_ptr(), entries=2, rows=2)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            stream = torch.cuda.current_stream().cuda_stream
+            pool.cache.extend(at.data_ptr(), 0, 2, space.data_ptr(), space.numel(), stream)
+            pool.cache.append(0, args, stream)
+        steps.append((slots, row, graph, at, space, args))
+
+    def step(which, x, ok):
+        slots, row, graph = steps[which][:3]
+        row.copy_(torch.tensor([x, x + 100.0]).to(torch.bfloat16)[:, None, None].expand(2, 1, 8))
+        graph.replay()
+        torch.cuda.synchronize()
+        if ok:
+            for s, v in zip(slots, (x, x + 100)):
+                kept[s].append(v)
+        table, page = pool.table.cpu().numpy(), pool.shape[3]
+        for s, rows in kept.items():
+            assert pool.lengths[s].item() == len(rows)
+            for t, v in enumerate(rows):
+                assert (pool.k[0, table[s, t // page], 0, t % page] == v).all() and (pool.v[0, table[s, t // page], 0, t % page] == v).all()
+
+    for x, which, ok in [(1, 0, True), (2, 0, True), (3, 1, True), (4, 0, True), (5, 0, True), (6, 1, True), (7, 1, False), (8, 0, False)]:      # six pages of two tokens
+        step(which, x, ok)
+    slots = ints([0])
+    pool.cache.free(slots.data_ptr(), 1)
+    kept[0] = []
+    step(1, 9, False)                # two pages are free now
+    step(0, 10, False)               # sequence 1 stands still
+    pool.refused[2:] = 0
+    step(1, 11, True)
+    assert pool.refused.tolist() == [1, 1, 0, 0] and pool.status.item() == api.CACHE_NO_PAGES | api.CACHE_REFUSED
+
+
+@pytest.mark.gpu
+def test_a_list_of_refused_sequences_in_host_memory_is_refused():
+    import torch
+    host, d = torch.zeros(64, dtype=torch.int32), torch.zeros(1 << 20, dtype=torch.uint8, device="cuda").data_ptr()
+    L, c = api.lib(), good_cache(refused=host.data_ptr(), **{name: d for name in ("k", "v", "page_table", "lengths", "refs", "status")})
+    rows = api.AppendArgs(k=d, v=d, entries=1, rows=1)
+    assert L.aspen_b200_cache_extend(C.byref(c), None, None, 1, d, 1 << 20, None) == -1 and "refused" in api.last_error()
+    assert L.aspen_b200_cache_append(C.byref(c), 0, C.byref(rows), None) == -1
+    assert L.aspen_b200_cache_fork(C.byref(c), d, d, 1, d, 1 << 20, None) == -1
+    assert L.aspen_b200_cache_free(C.byref(c), d, 1, None) == -1
