@@ -277,8 +277,8 @@ struct Kernel {
                 const float ref = m == -INFINITY ? 0.f : m;
                 down[j] = mma::exp2_fast(run.max[n][j] - ref);
                 run.max[n][j] = m;
-                w[j] = mma::exp2_fast(x[j] - ref);
-                w[2 + j] = mma::exp2_fast(x[2 + j] - ref);
+                w[j] = mma::exp2_fast(x[j] - (ref - mma::Of<TYPE>::TOP));
+                w[2 + j] = mma::exp2_fast(x[2 + j] - (ref - mma::Of<TYPE>::TOP));
                 run.sum[n][j] = run.sum[n][j] * down[j] + (w[j] + w[2 + j]);
             }
             if (__any_sync(0xffffffffu, down[0] != 1.f || down[1] != 1.f)) {

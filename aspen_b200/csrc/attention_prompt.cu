@@ -209,6 +209,7 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
             m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
             ref[h] = m[h] == -INFINITY ? 0.f : m[h];
             down[h] = mma::exp2_fast(max[h] - ref[h]);
+            ref[h] -= mma::Of<TYPE>::TOP;
             max[h] = m[h];
             sum[h] *= down[h];
         }
@@ -755,6 +756,8 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
         const int w = (int)(warp >> 2);
         const unsigned row = (warp & 3u) * 32u + lane, lanes = tmem + ((warp & 3u) << 21), s_at = lanes + H::S + w * 128, p_at = lanes + H::P + w * H::P_APART, o_at = lanes + H::O + w * DIM;
         const Pair scale2 = pair(a.scale, a.scale);
+        // a row's largest weight is 2^LEVEL, and 2^(LEVEL + LOOSE) until its maximum is followed
+        constexpr float LOOSE = TYPE == ASPEN_B200_FP16 ? 4.f : 8.f, LEVEL = mma::Of<TYPE>::TOP > 0.f ? mma::Of<TYPE>::TOP - LOOSE : 0.f;
         unsigned done = 0, outs = 0;
         bool ok = true;
         int both = 0;                                  // steps of the job before: without a tile of their own these warps wait for all of them
@@ -801,7 +804,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                 const float top = max2(max3(m0, m1, m2), m3);
                 if (H::OWN_P && done > 0) { ok = warp_wait(&sh.o_full[w], (done & 1u) ^ 1u, gave_up); tc::tc_fence_after(); }
                 if (j == 0) grow(top);
-                else if (__any_sync(0xffffffffu, (top - max) * a.scale > 8.f || (top != top && max == max))) {
+                else if (__any_sync(0xffffffffu, (top - max) * a.scale > LOOSE || (top != top && max == max))) {
                     const float before = max;
                     grow(top);
                     const float down = max == -INFINITY ? 1.f : mma::exp2_fast((before - max) * a.scale);
@@ -816,7 +819,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
                     }
                     sum *= down;
                 }
-                const float ref = max == -INFINITY ? 0.f : -max * a.scale;
+                const float ref = max == -INFINITY ? 0.f : fmaf(-max, a.scale, LEVEL);
                 const Pair ref2 = pair(ref, ref);
                 Pair part[4] = {0ull, 0ull, 0ull, 0ull};
                 #pragma unroll

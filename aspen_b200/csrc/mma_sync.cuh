@@ -53,21 +53,25 @@ __device__ __forceinline__ unsigned transpose8(unsigned x) {
 // 2^x; -inf gives 0.
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
-// Per type: VALUES of 16 bytes; one loaded piece is two k steps of the product over features (`features`), and a piece of each of four keys' rows is PIECE_TILES
+// Per type: TOP, the binary logarithm of the largest softmax weight.  fp16 ends at 2^-24, so with 2^15 at the top a weight keeps its 11 bits down to 2^-29 of the largest one; with 1 there, many keys
+// of 2^-20 each beside one large one were off by up to 3 %, and those below 2^-25 were lost while the sum below the fraction had them.  The factor cancels in the fraction.
+// VALUES of 16 bytes; one loaded piece is two k steps of the product over features (`features`), and a piece of each of four keys' rows is PIECE_TILES
 // 16-row tiles of the product over 16 keys.
 template <int TYPE> struct Of;
 
 template <> struct Of<ASPEN_B200_BF16> {
     static constexpr int SIZE = 2, VALUES = 8;
+    static constexpr float TOP = 0.f;
     static __device__ __forceinline__ void step(float *d, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) { bf16_16816(d, a0, a1, a2, a3, b0, b1); }
     static __device__ __forceinline__ unsigned pack(float lo, float hi) { unsigned r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
 };
 template <> struct Of<ASPEN_B200_FP16> {
     static constexpr int SIZE = 2, VALUES = 8;
+    static constexpr float TOP = 15.f;
     static __device__ __forceinline__ void step(float *d, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) { fp16_16816(d, a0, a1, a2, a3, b0, b1); }
     static __device__ __forceinline__ unsigned pack(float lo, float hi) { unsigned r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
 };
-template <> struct Of<ASPEN_B200_FP32> { static constexpr int SIZE = 4, VALUES = 4; };
+template <> struct Of<ASPEN_B200_FP32> { static constexpr int SIZE = 4, VALUES = 4; static constexpr float TOP = 0.f; };
 
 // Two rows' pieces (x row 2 t, y row 2 t + 1 of 8 keys): the pairs of keys of value j.
 __device__ __forceinline__ unsigned pair_of(unsigned x, unsigned y, bool high) { return __byte_perm(x, y, high ? 0x7632 : 0x5410); }

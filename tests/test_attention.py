@@ -1280,3 +1280,62 @@ def test_a_list_of_refused_sequences_in_host_memory_is_refused():
     assert L.aspen_b200_cache_append(C.byref(c), 0, C.byref(rows), None) == -1
     assert L.aspen_b200_cache_fork(C.byref(c), d, d, 1, d, 1 << 20, None) == -1
     assert L.aspen_b200_cache_free(C.byref(c), d, 1, None) == -1
+
+
+# ---- small weights beside a large one ----------------------------------------------------------------------------------------
+#
+# One key takes nearly all weight and has values of zero, the others share 2^-24 or 2^-20 of it each, so an output is as exact as their weights.
+# Off by at most: u |o| its own rounding, u A the weights' (16 bits), 2 delta A the scores', and sums of n terms: products 16 at a time, cut off at 2^-23 of
+# the sum, and weights four to a thread and 16 keys at most, rounded to 2^-24: n (2^-27 + 2^-26) < n 2^-25; joins and exp2 2^-20.
+
+def sink_and_tail(keys, kv_heads, dim, apart, kind):
+    """k, v of `keys` tokens, the first one `apart` above the others for a query of (1, 0, 0 ...)."""
+    rng = np.random.default_rng(int(apart * 1000) + keys)
+    k, v = rng.standard_normal((keys, kv_heads, dim)), 64 * (1 + rng.random((keys, kv_heads, dim)))
+    k[:, :, 0] = 0
+    k[0, :, 0], v[0] = apart, 0
+    return rounded(k, kind), rounded(v, kind)
+
+
+def check_tail(got, q, k, v, kind):
+    want, _, size = attend(q, k, v, 1.0, np.ones((len(q), len(k)), bool))
+    away = size * (2 * np.abs(k[:, :, 0]).max() * (q.shape[2] * 2.0 ** -23 + 2.0 ** -20) + len(k) * 2.0 ** -25 + 2.0 ** -20)
+    check(got, want, away, size, kind)
+
+
+APART = [pytest.param(14.03125, id="2^-20"), pytest.param(16.875, id="2^-24")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("apart", APART)
+@pytest.mark.parametrize("heads,dim,q_len,kv_len", [(12, 64, [512], [4000]), (12, 128, [512], [4000]), (8, 64, [1], [60000]), (2, 256, [1], [9000]), (8, 256, [1] * 64, [1000] * 64), (24, 32, [3] * 40, [50] * 40)])
+def test_prompts_weigh_many_small_keys_beside_a_large_one(heads, dim, q_len, kv_len, apart, kind):
+    k, v = sink_and_tail(kv_len[0], heads, dim, apart, kind)
+    q = np.zeros((q_len[0], heads, dim))
+    q[:, :, 0] = 1
+    n = len(q_len)
+    got = prompt(*(to_device(np.concatenate([a] * n), kind) for a in (q, k, v)), np.arange(n + 1) * q_len[0], np.arange(n + 1) * kv_len[0], kind, False, 1.0)
+    for s in (0, n // 2, n - 1):
+        check_tail(got[s * q_len[0]:(s + 1) * q_len[0]], q, k, v, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("apart", APART)
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens,entries", [(4, 4, 64, 320, 600), (8, 4, 128, 320, 600), (4, 4, 256, 320, 400), (16, 1, 64, 700, 3), (2, 2, 64, 60000, 1)])
+def test_a_token_weighs_many_small_keys_beside_a_large_one(heads, kv_heads, dim, tokens, entries, apart, kind):
+    """Many entries: a warp walks a whole sequence; few: it is shared."""
+    rng = np.random.default_rng(30)
+    pool = Pool(kind, kv_heads, dim, 16, -(-tokens // 16), 1, -(-tokens // 16))
+    pool.fill([tokens], rng)
+    k, v = sink_and_tail(tokens, kv_heads, dim, apart, kind)
+    for t in range(tokens):
+        p, r = pool.host_table[0, t // 16], t % 16
+        pool.host_k[0, p, :, r], pool.host_v[0, p, :, r] = k[t], v[t]
+    pool.k.copy_(to_device(pool.host_k, kind)); pool.v.copy_(to_device(pool.host_v, kind))
+    q = np.zeros((1, heads, dim))
+    q[:, :, 0] = 1
+    got = decode(pool, to_device(np.concatenate([q] * entries), kind), heads, slots=[0] * entries, scale=1.0)
+    for i in (0, entries // 2, entries - 1):
+        check_tail(got[i:i + 1], q, k, v, kind)
