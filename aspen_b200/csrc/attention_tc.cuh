@@ -6,7 +6,7 @@
 //     P = exp2(S - max)                      a thread a row: its scores from TMEM to registers, weights back to TMEM as 16-bit pairs
 //     O [128 rows x features] += P V         P from TMEM, V as it lies in memory (features contiguous: the MN-major operand), sums in TMEM
 // The maximum is followed loosely, a known variant of the running softmax: O and the sum are scaled again only when a row's maximum has grown by more than 2^8 (weights up to 256 are as
-// exact as weights up to 1), so the sums in TMEM are hardly ever read before the end.  fp16: by more than 2^4, from 2^11, so that weights stay below 2^15 and small ones keep their bits (mma_sync.cuh).
+// exact as weights up to 1), so the sums in TMEM are hardly ever read before the end.  fp16: by more than 2^5, from 2^10, so that weights stay below 2^15 and small ones keep their bits (mma_sync.cuh).
 //
 // Warps: 0 - 3 and 4 - 7 the softmax of the two tiles, 8 TMA, 9 MMA (with 64 features 9 and 11, a tile each), 10 finds the work, 12 - 15 write outputs; nothing but mbarriers connects them, and while one tile's scores are weighed
 // the other's are multiplied.  The first three quarters of a tile's weights are multiplied while the last one is computed.  TMEM, 512 columns: scores 2 x 128, sums 2 x features, and with 64
