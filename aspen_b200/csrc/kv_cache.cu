@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(BOOK) extend_kernel(const Pool pool, const Spa
     }
 }
 
+enum { TARGET = 1, SOURCE = 2 };               // marks of a sequence
 __global__ void __launch_bounds__(BOOK) fork_kernel(const Pool pool, const Space w, const int *from, const int *to, unsigned entries) {
     __shared__ unsigned sums[32];
     __shared__ int refused;
@@ -199,14 +200,16 @@ __global__ void __launch_bounds__(BOOK) fork_kernel(const Pool pool, const Space
     for (unsigned e0 = 0; e0 < entries; e0 += BOOK) {
         const unsigned e = e0 + threadIdx.x;
         unsigned part = 0;
+        bool first = false;                         // of the entries with this source
         if (e < entries) {
             const int a = from[e], b = to[e];
             unsigned len = 0;
             if (a < 0 || (unsigned)a >= pool.at.sequences || b < 0 || (unsigned)b >= pool.at.sequences) why |= ASPEN_B200_CACHE_BAD_INDEX;
-            else if (atomicAdd(&w.mark[b], 1) != 0 || pool.lengths[b] != 0) why |= ASPEN_B200_CACHE_BAD_INDEX;
+            else if (atomicOr(&w.mark[b], TARGET) & TARGET || pool.lengths[b] != 0) why |= ASPEN_B200_CACHE_BAD_INDEX;
             else if (attn::is_refused(pool.at, a) || attn::is_refused(pool.at, b)) why |= ASPEN_B200_CACHE_REFUSED;
             else {
                 len = attn::sequence_length(pool.at, a);
+                first = !(atomicOr(&w.mark[a], SOURCE) & SOURCE);
                 part = len % page != 0;
                 if (part) {
                     const int last = pool.table[(size_t)a * pool.at.max_pages + len / page];
@@ -215,6 +218,7 @@ __global__ void __launch_bounds__(BOOK) fork_kernel(const Pool pool, const Space
                 }
             }
             w.length[e] = (int)len;
+            w.to[e] = first;
         }
         unsigned all;
         const unsigned at = total + before_me(part, all, sums);
@@ -223,6 +227,26 @@ __global__ void __launch_bounds__(BOOK) fork_kernel(const Pool pool, const Space
         if (total > pool.at.pages) { why |= ASPEN_B200_CACHE_NO_PAGES; break; }
     }
     if (why) atomicOr(&refused, why);
+    __syncthreads();
+    const bool go_on = !refused;
+    __syncthreads();                                // all have read it
+    if (go_on) {
+        // the sources' full pages, each source's once: 32 pages at a time, the first ones of the source of entry i by warp i
+        const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+        bool bad = false;
+        for (unsigned e0 = 0; e0 < entries; e0 += 32) {
+            const unsigned e = e0 + lane;
+            const bool mine = e < entries && w.to[e];
+            const int a = mine ? from[e] : 0;
+            const unsigned full = mine ? (unsigned)w.length[e] / page : 0u;
+            for (unsigned left = __ballot_sync(0xffffffffu, full > 0); left; left &= left - 1) {
+                const unsigned at = __ffs(left) - 1, n = __shfl_sync(0xffffffffu, full, at);
+                const int *const row = pool.table + (size_t)__shfl_sync(0xffffffffu, a, at) * pool.at.max_pages;
+                for (unsigned i = ((warp - at) % 32) * 32 + lane; i < n; i += BOOK) bad |= (unsigned)row[i] >= pool.at.pages;
+            }
+        }
+        if (bad) atomicOr(&refused, ASPEN_B200_CACHE_BAD_INDEX);
+    }
     __syncthreads();
     if (!refused) {
         if (lowest_free(pool.refs, pool.at.pages, total, w.to, sums) < total && threadIdx.x == 0) refused = ASPEN_B200_CACHE_NO_PAGES;
@@ -306,8 +330,7 @@ __global__ void __launch_bounds__(COPY, COPY_CTAS) fork_copy_kernel(const Pool p
         int p = -1;
         if (i < full) {
             p = pool.table[(size_t)from[e] * max_pages + i];
-            if (p >= 0 && (unsigned)p < pool.at.pages) atomicAdd(&pool.refs[p], 1);
-            else atomicOr(pool.at.status, ASPEN_B200_CACHE_BAD_INDEX);
+            if ((unsigned)p < pool.at.pages) atomicAdd(&pool.refs[p], 1);
         } else if (i == full && len % page) p = w.to[w.start[e]];
         pool.table[(size_t)to[e] * max_pages + i] = p;
         if (i == 0) pool.lengths[to[e]] = (int)len;

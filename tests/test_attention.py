@@ -1339,3 +1339,29 @@ def test_a_token_weighs_many_small_keys_beside_a_large_one(heads, kv_heads, dim,
     got = decode(pool, to_device(np.concatenate([q] * entries), kind), heads, slots=[0] * entries, scale=1.0)
     for i in (0, entries // 2, entries - 1):
         check_tail(got[i:i + 1], q, k, v, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,lengths,broken,value", [(4, [9, 6], (0, 0), -1), (4, [9, 6], (0, 1), 13), (4, [8, 6], (0, 1), 2**31 - 1), (1, [3000, 2], (0, 2999), -7), (4, [9, 6], (1, 1), -1), (4, [9, 6], (0, 2), -1)])
+def test_fork_of_a_sequence_with_a_page_that_is_none_changes_nothing(page, lengths, broken, value):
+    """Its neighbours in the call are not forked either."""
+    pool = Pool(api.FP16, 1, 8, page, 8 + sum(-(-n // page) for n in lengths), 6, -(-max(lengths) // page) + 1)
+    pool.fill(lengths, np.random.default_rng(31))
+    table = pool.host_table.copy()
+    table[broken] = value
+    pool.table.copy_(ints(table))
+    k, books = bits(pool.k), Books(pool)
+    a, b = ints([1, 0, 1]), ints([2, 3, 5])
+    pool.cache.fork(a.data_ptr(), b.data_ptr(), 3, *pool.space(3))
+    books.status |= api.CACHE_BAD_INDEX
+    books.same(pool)
+    np.testing.assert_array_equal(bits(pool.k), k)
+    # the pool goes on: pages taken for nothing are free
+    pool.status.zero_(); pool.table.copy_(ints(pool.host_table))
+    books = Books(pool)
+    pool.cache.fork(a.data_ptr(), b.data_ptr(), 3, *pool.space(3))
+    copied = books.fork([1, 0, 1], [2, 3, 5])
+    books.same(pool)
+    for x, y, tokens in copied:
+        k[:, y, :, :tokens] = k[:, x, :, :tokens]
+    np.testing.assert_array_equal(bits(pool.k), k)
