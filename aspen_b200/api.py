@@ -22,9 +22,10 @@ LAYER_TYPES = ["NO_LAYER_TYPE", "INPUT", "CONV", "FC", "RESIDUAL", "BATCHNORM", 
 
 LDATA_FIELDS = ("type", "act", "H", "W", "stride", "tile_h", "tile_w", "num_ninst", "flop_per_output",
                 "parent0", "parent1", "mem_size")
-# ASPEN_B200_TYPE, ASPEN_B200_CACHE_* (include/aspen_b200.h)
+# ASPEN_B200_TYPE, ASPEN_B200_CACHE_*, ASPEN_B200_PROMPT_* (include/aspen_b200.h)
 FP32, BF16, FP16 = range(3)
 CACHE_BAD_INDEX, CACHE_NO_PAGES, CACHE_TOO_LONG, CACHE_REFUSED = 1, 2, 4, 8
+PROMPT_STALLED = 1
 
 NINST_FIELDS = ("pos_h", "pos_w", "tile_h", "tile_w", "num_parents", "num_children", "num_input_pos")
 
@@ -338,7 +339,7 @@ def _struct(pointers: str, sizes: str, ints: str, unsigneds: str, floats: str = 
 class PromptArgs(C.Structure):
     """aspen_b200_prompt_t; pointers are device addresses."""
     _fields_ = _struct("q k v out q_starts kv_starts", "q_row_stride q_head_stride k_row_stride k_head_stride v_row_stride v_head_stride out_row_stride out_head_stride",
-                       "type masked", "heads kv_heads head_dim sequences q_rows kv_rows", "scale")
+                       "type masked", "heads kv_heads head_dim sequences q_rows kv_rows", "scale") + [("status", C.c_void_p)]
 
 
 class AppendArgs(C.Structure):

@@ -31,6 +31,7 @@ struct Args {
     Divisor by_block;
     int masked;
     float scale;                        // with log2(e)
+    int *status;                        // or nullptr
 };
 
 // A block of queries: rows first ... of the sequence that begins at row q0.
@@ -743,6 +744,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
         __syncthreads();
         if (warp == 9) {
             if (sh.gave_up) {
+                if (a.status && lane == 0) atomicOr(a.status, ASPEN_B200_PROMPT_STALLED);
                 // copies and MMAs may still be in flight; they take microseconds
                 unsigned long long t0, now;
                 asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
@@ -1062,6 +1064,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_parts(const Args a, 
         __syncthreads();
         if (warp == 9) {
             if (sh.gave_up) {
+                if (a.status && lane == 0) atomicOr(a.status, ASPEN_B200_PROMPT_STALLED);
                 // MMAs may still be in flight; they take microseconds
                 unsigned long long t0, now;
                 asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
@@ -1299,8 +1302,8 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     if (p->kv_rows && ((rc = attn::check_rows(p->k, p->k_row_stride, p->k_head_stride, p->type, "k", what)) || (rc = attn::check_rows(p->v, p->v_row_stride, p->v_head_stride, p->type, "v", what)))) return rc;
     const int sms = attn::sm_count(what);
     if (sms < 0) return sms;
-    const attn::Named all[] = {{p->q, "q"}, {p->out, "out"}, {p->q_starts, "q_starts"}, {p->kv_starts, "kv_starts"}, {p->kv_rows ? p->k : nullptr, "k"}, {p->kv_rows ? p->v : nullptr, "v"}};
-    if ((rc = attn::check_device(all, 6, what))) return rc;
+    const attn::Named all[] = {{p->q, "q"}, {p->out, "out"}, {p->q_starts, "q_starts"}, {p->kv_starts, "kv_starts"}, {p->kv_rows ? p->k : nullptr, "k"}, {p->kv_rows ? p->v : nullptr, "v"}, {p->status, "status"}};
+    if ((rc = attn::check_device(all, 7, what))) return rc;
     Args a;
     a.q = static_cast<const char *>(p->q);
     a.k = static_cast<const char *>(p->k);
@@ -1328,6 +1331,7 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     a.head_dim = p->head_dim;
     a.masked = p->masked != 0;
     a.scale = p->scale * 1.4426950408889634f;
+    a.status = p->status;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t err = cudaSuccess;
     const unsigned ranks = ranks_of(a, p->type, (unsigned)sms);

@@ -29,7 +29,8 @@
 //
 // Values behind the end of a sequence are another one's, or nobody's: an MMA warp sets them to zero in shared memory, since 0 x NaN would reach every row.
 //
-// Every wait is bounded (2 s, or 2 s and 100 us a step) and is for another role of the CTA; if one runs out all roles leave, TMEM is freed and the rows of out that were in work become NaN.
+// Every wait is bounded (2 s, or 2 s and 100 us a step) and is for another role of the CTA; if one runs out all roles leave, TMEM is freed, the rows of out that were in work become NaN, those
+// not begun stay, and the caller's status word says so.
 #pragma once
 #include "tiles_tc.cuh"
 

@@ -301,7 +301,10 @@ typedef enum { ASPEN_B200_FP32, ASPEN_B200_BF16, ASPEN_B200_FP16, ASPEN_B200_NUM
  * its keys, the one before it all but the last, and so on; with more queries than keys the first ones see none.  A row that sees nothing becomes zeros.
  * Rows of no sequence are neither read into a result nor written.  Starts outside 0 ... q_rows (kv_rows) are taken as the nearest one inside, a sequence that would
  * end before it starts is empty; sequences must not share rows of out.  Values behind a query's last key, but within its sequence, must be finite (they are
- * multiplied by zero).  Up to 2^24 sequences, 2^30 - 1 rows. */
+ * multiplied by zero).  Up to 2^24 sequences, 2^30 - 1 rows.
+ * The kernels' parts wait for one another for 2 s and 100 us for each 128 keys at most, so that a device that stalls them gets them back: rows of out that they were at or had not come to are
+ * then NaN or what they were, and *status has ASPEN_B200_PROMPT_STALLED. */
+#define ASPEN_B200_PROMPT_STALLED 1
 typedef struct {
     const void *q, *k, *v;         /* [q_rows][heads][head_dim], [kv_rows][kv_heads][head_dim] twice */
     void *out;                     /* [q_rows][heads][head_dim]; not q, k or v */
@@ -310,6 +313,7 @@ typedef struct {
     int type, masked;
     unsigned int heads, kv_heads, head_dim, sequences, q_rows, kv_rows;
     float scale;
+    int *status;                   /* a word to which that bit is added, or NULL; the caller clears it */
 } aspen_b200_prompt_t;
 int aspen_b200_attention_prompt(const aspen_b200_prompt_t *prompt, void *cuda_stream);
 

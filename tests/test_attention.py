@@ -1365,3 +1365,20 @@ def test_fork_of_a_sequence_with_a_page_that_is_none_changes_nothing(page, lengt
     for x, y, tokens in copied:
         k[:, y, :, :tokens] = k[:, x, :, :tokens]
     np.testing.assert_array_equal(bits(pool.k), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_status_word_of_prompts_stays_as_it_was_where_nothing_stalls(dim, kind):
+    import torch
+    rng = np.random.default_rng(40)
+    q, k, v = (rounded(rng.standard_normal((300, 8, dim)), kind) for _ in range(3))
+    status = ints([6])
+    got = prompt(*(to_device(a, kind) for a in (q, k, v)), [0, 300], [0, 300], kind, True, 0.1, status=status.data_ptr())
+    want, away, size = attend(q, k, v, 0.1, seen_by(300, 300, True))
+    check(got, want, away, size, kind)
+    assert status.item() == 6
+    d, host = got.data_ptr(), torch.zeros(4, dtype=torch.int32)
+    good = dict(type=kind, heads=1, kv_heads=1, head_dim=8, scale=1.0, sequences=1, q_rows=1, kv_rows=1, q_starts=status.data_ptr(), kv_starts=status.data_ptr(), q=d, k=d, v=d, out=d + 4096)
+    assert api.lib().aspen_b200_attention_prompt(C.byref(api.PromptArgs(**good, status=host.data_ptr())), None) == -1 and "status" in api.last_error()
