@@ -771,7 +771,7 @@ __global__ void __launch_bounds__(fused::THREADS, 1) prompt_tiles(const __grid_c
             if (first < 0 || steps == 0) continue;
             const int query = first + (int)(row * a.part >> 16);
             const int seen = a.masked ? min(job.keys, query + job.behind() + 1) : job.keys;              // first key that the row does not see
-            const int least_seen = __shfl_sync(0xffffffffu, seen, 0), most_seen = __shfl_sync(0xffffffffu, seen, 31);       // of the warp's rows
+            const int least_seen = __shfl_sync(0xffffffffu, seen, 0);            // of the warp's rows
             float max = -INFINITY, sum = 0.f;
             // a NaN stays the maximum, and so it becomes if a score is infinite: then all weights of the row are NaN
             auto grow = [&](float most) { max = max2(max, most); if (max == INFINITY) max = NAN; };

@@ -1382,3 +1382,20 @@ def test_a_status_word_of_prompts_stays_as_it_was_where_nothing_stalls(dim, kind
     d, host = got.data_ptr(), torch.zeros(4, dtype=torch.int32)
     good = dict(type=kind, heads=1, kv_heads=1, head_dim=8, scale=1.0, sequences=1, q_rows=1, kv_rows=1, q_starts=status.data_ptr(), kv_starts=status.data_ptr(), q=d, k=d, v=d, out=d + 4096)
     assert api.lib().aspen_b200_attention_prompt(C.byref(api.PromptArgs(**good, status=host.data_ptr())), None) == -1 and "status" in api.last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("heads,kv_heads,dim,q_len,kv_len", [(2, 2, 64, [300, 40], [50, 200]), (2, 2, 32, [40, 300, 130], [200, 50, 2]), (2, 2, 128, [300, 40], [50, 200]), (16, 2, 64, [60, 5], [20, 40])])
+def test_masked_prompts_whose_first_tile_sees_no_key(heads, kv_heads, dim, q_len, kv_len, kind):
+    """Its second tile does, in the same piece of work: 48 short sequences beside them, so that the calls run in tiles."""
+    rng = np.random.default_rng(dim + heads)
+    q_len, kv_len = q_len + [300] * 48, kv_len + [50] * 48
+    qs, ks = np.concatenate([[0], np.cumsum(q_len)]), np.concatenate([[0], np.cumsum(kv_len)])
+    q, k, v = (rounded(rng.standard_normal((n, h, dim)), kind) for n, h in ((qs[-1], heads), (ks[-1], kv_heads), (ks[-1], kv_heads)))
+    got = prompt(*(to_device(a, kind) for a in (q, k, v)), qs, ks, kind, True, dim ** -0.5)
+    for s in range(len(q_len)):
+        a, b, x, y = qs[s], qs[s + 1], ks[s], ks[s + 1]
+        want, away, size = attend(q[a:b], k[x:y], v[x:y], dim ** -0.5, seen_by(b - a, y - x, True))
+        check(got[a:b], want, away, size, kind)
+        assert (got[a:b][:max(0, (b - a) - (y - x))] == 0).all()
