@@ -25,9 +25,17 @@ int check_rows(const void *p, size_t row, size_t head, int type, const char *nam
     return 0;
 }
 
+int check_ints(const Named *list, unsigned n, const char *what) {
+    for (unsigned i = 0; i < n; i++)
+        if (reinterpret_cast<uintptr_t>(list[i].p) % sizeof(int)) { ASPEN_ERR("%s: %s does not start on a 4-byte boundary\n", what, list[i].name); return -1; }
+    return 0;
+}
+
 int check_cache(const aspen_b200_cache_t *c, const char *what, bool pool) {
     if (!c) { ASPEN_ERR("%s: no cache\n", what); return -1; }
     if (!c->page_table || !c->lengths || !c->status || (pool && !c->refs)) { ASPEN_ERR("%s: the cache has no page_table, lengths, status or refs\n", what); return -1; }
+    const Named ints[] = {{c->page_table, "page_table"}, {c->lengths, "lengths"}, {c->refs, "refs"}, {c->status, "status"}, {c->refused, "refused"}};
+    if (check_ints(ints, 5, what)) return -1;
     if (!c->layers || !c->pages || !c->page_size || !c->kv_heads || !c->sequences || !c->max_pages) { ASPEN_ERR("%s: a size of the cache is 0\n", what); return -1; }
     const int bad = check_type(c->type, c->head_dim, what);
     if (bad) return bad;

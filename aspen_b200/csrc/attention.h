@@ -67,6 +67,8 @@ int check_rows(const void *p, size_t row, size_t head, int type, const char *nam
 // All of these are memory of the current device (NULL ones are not looked at).
 struct Named { const void *p; const char *name; };
 int check_device(const Named *list, unsigned n, const char *what);
+// All of these start on a 4-byte boundary (NULL does).
+int check_ints(const Named *list, unsigned n, const char *what);
 int sm_count(const char *what);            // of the current device, which is an sm_100 one; or a negative return value
 size_t packed(size_t stride, size_t dense);
 

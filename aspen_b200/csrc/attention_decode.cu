@@ -669,6 +669,8 @@ extern "C" int aspen_b200_attention_decode(const aspen_b200_cache_t *cache, unsi
     if (!d->slots && d->entries > cache->sequences) { ASPEN_ERR("%s: %u entries, %u sequences\n", what, d->entries, cache->sequences); return -1; }
     if ((rc = attn::check_rows(d->q, d->q_row_stride, d->q_head_stride, cache->type, "q", what)) ||
         (rc = attn::check_rows(d->out, d->out_row_stride, d->out_head_stride, cache->type, "out", what))) return rc;
+    const attn::Named ints[] = {{d->slots, "slots"}};
+    if ((rc = attn::check_ints(ints, 1, what))) return rc;
     if (!d->workspace || reinterpret_cast<uintptr_t>(d->workspace) % 16) { ASPEN_ERR("%s: no workspace, or not on a 16-byte boundary\n", what); return -1; }
     const int sms = attn::sm_count(what);
     if (sms < 0) return sms;

@@ -1298,6 +1298,8 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     if (p->q_rows > 0x3fffffffu || p->kv_rows > 0x3fffffffu || p->sequences > 1u << 24 || p->heads > 0xffffu) { ASPEN_ERR("%s: too many rows, sequences or heads\n", what); return -2; }
     if (!p->sequences || !p->q_rows) return 0;
     if (!p->q_starts || !p->kv_starts) { ASPEN_ERR("%s: q_starts or kv_starts is NULL\n", what); return -1; }
+    const attn::Named ints[] = {{p->q_starts, "q_starts"}, {p->kv_starts, "kv_starts"}, {p->status, "status"}};
+    if ((rc = attn::check_ints(ints, 3, what))) return rc;
     if ((rc = attn::check_rows(p->q, p->q_row_stride, p->q_head_stride, p->type, "q", what)) || (rc = attn::check_rows(p->out, p->out_row_stride, p->out_head_stride, p->type, "out", what))) return rc;
     if (p->kv_rows && ((rc = attn::check_rows(p->k, p->k_row_stride, p->k_head_stride, p->type, "k", what)) || (rc = attn::check_rows(p->v, p->v_row_stride, p->v_head_stride, p->type, "v", what)))) return rc;
     const int sms = attn::sm_count(what);

@@ -539,6 +539,8 @@ extern "C" int aspen_b200_cache_extend(const aspen_b200_cache_t *cache, const in
     if (!rc) rc = check_entries(entries, what);
     if (!rc) rc = check_space(cache, entries, workspace, workspace_bytes, what);
     if (rc || !entries) return rc;
+    const attn::Named ints[] = {{slots, "slots"}, {starts, "starts"}};
+    if ((rc = attn::check_ints(ints, 2, what))) return rc;
     const attn::Named all[] = {{cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->refs, "refs"}, {cache->status, "status"},
                                {slots, "slots"}, {starts, "starts"}, {workspace, "workspace"}, {cache->refused, "refused"}};
     if ((rc = attn::check_device(all, 8, what))) return rc;
@@ -557,6 +559,8 @@ extern "C" int aspen_b200_cache_append(const aspen_b200_cache_t *cache, unsigned
     const size_t row = (size_t)cache->kv_heads * cache->head_dim;
     if ((rc = attn::check_rows(a->k, a->k_row_stride, a->k_head_stride, cache->type, "k", what)) ||
         (rc = attn::check_rows(a->v, a->v_row_stride, a->v_head_stride, cache->type, "v", what))) return rc;
+    const attn::Named ints[] = {{a->slots, "slots"}, {a->starts, "starts"}};
+    if ((rc = attn::check_ints(ints, 2, what))) return rc;
     const attn::Named all[] = {{cache->k, "the cache's k"}, {cache->v, "the cache's v"}, {cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->status, "status"},
                                {a->k, "k"}, {a->v, "v"}, {a->slots, "slots"}, {a->starts, "starts"}, {cache->refused, "refused"}};
     if ((rc = attn::check_device(all, 10, what))) return rc;
@@ -591,6 +595,8 @@ extern "C" int aspen_b200_cache_fork(const aspen_b200_cache_t *cache, const int 
     if (!rc) rc = check_space(cache, entries, workspace, workspace_bytes, what);
     if (rc || !entries) return rc;
     if (!from || !to) { ASPEN_ERR("%s: no list of sequences\n", what); return -1; }
+    const attn::Named ints[] = {{from, "from"}, {to, "to"}};
+    if ((rc = attn::check_ints(ints, 2, what))) return rc;
     const attn::Named all[] = {{cache->k, "the cache's k"}, {cache->v, "the cache's v"}, {cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->refs, "refs"},
                                {cache->status, "status"}, {from, "from"}, {to, "to"}, {workspace, "workspace"}, {cache->refused, "refused"}};
     if ((rc = attn::check_device(all, 10, what))) return rc;
@@ -609,6 +615,8 @@ extern "C" int aspen_b200_cache_free(const aspen_b200_cache_t *cache, const int 
     if (!rc) rc = check_entries(entries, what);
     if (rc || !entries) return rc;
     if (!slots) { ASPEN_ERR("%s: no list of sequences\n", what); return -1; }
+    const attn::Named ints[] = {{slots, "slots"}};
+    if ((rc = attn::check_ints(ints, 1, what))) return rc;
     const attn::Named all[] = {{cache->page_table, "page_table"}, {cache->lengths, "lengths"}, {cache->refs, "refs"}, {cache->status, "status"}, {slots, "slots"}, {cache->refused, "refused"}};
     if ((rc = attn::check_device(all, 6, what))) return rc;
     return done(launch_early(free_kernel, entries, COPY, 0, static_cast<cudaStream_t>(cuda_stream), pool_of(*cache), slots), what);
@@ -636,6 +644,8 @@ extern "C" int aspen_b200_cache_copy(const aspen_b200_cache_t *cache, const int 
     if (!rc) rc = check_entries(count, what);
     if (rc || !count) return rc;
     if (!from || !to) { ASPEN_ERR("%s: no list of pages\n", what); return -1; }
+    const attn::Named ints[] = {{from, "from"}, {to, "to"}};
+    if ((rc = attn::check_ints(ints, 2, what))) return rc;
     const attn::Named all[] = {{cache->k, "the cache's k"}, {cache->v, "the cache's v"}, {cache->status, "status"}, {from, "from"}, {to, "to"}};
     if ((rc = attn::check_device(all, 5, what))) return rc;
     const int sms = attn::sm_count(what);

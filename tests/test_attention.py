@@ -1399,3 +1399,32 @@ def test_masked_prompts_whose_first_tile_sees_no_key(heads, kv_heads, dim, q_len
         want, away, size = attend(q[a:b], k[x:y], v[x:y], dim ** -0.5, seen_by(b - a, y - x, True))
         check(got[a:b], want, away, size, kind)
         assert (got[a:b][:max(0, (b - a) - (y - x))] == 0).all()
+
+
+# ---- more refusals -----------------------------------------------------------------------------------------------------------
+
+def test_words_off_a_4_byte_boundary_are_refused():
+    L, good = api.lib(), good_cache()
+    for name in ("page_table", "lengths", "refs", "status", "refused"):
+        c = good_cache(**{name: 66})
+        call, rows = api.DecodeArgs(entries=1, heads=2, scale=1.0, q=4096, out=4096, workspace=4096, workspace_bytes=1 << 30), api.AppendArgs(k=4096, v=4096, entries=1, rows=1)
+        assert L.aspen_b200_attention_decode(C.byref(c), 0, C.byref(call), None) == -1 and name in api.last_error()
+        assert L.aspen_b200_cache_append(C.byref(c), 0, C.byref(rows), None) == -1
+        assert L.aspen_b200_cache_extend(C.byref(c), None, None, 1, 4096, 1 << 30, None) == -1
+        assert L.aspen_b200_cache_fork(C.byref(c), 64, 64, 1, 4096, 1 << 30, None) == -1
+        assert L.aspen_b200_cache_free(C.byref(c), 64, 1, None) == -1
+        assert L.aspen_b200_cache_compact(C.byref(c), 4096, 1 << 30, None) == -1
+        assert L.aspen_b200_cache_copy(C.byref(c), 64, 64, 1, None) == -1
+    c = C.byref(good)
+    for at in (65, 66, 67):
+        assert L.aspen_b200_cache_extend(c, at, None, 1, 4096, 1 << 30, None) == L.aspen_b200_cache_extend(c, None, at, 1, 4096, 1 << 30, None) == -1
+        assert L.aspen_b200_cache_fork(c, at, 64, 1, 4096, 1 << 30, None) == L.aspen_b200_cache_fork(c, 64, at, 1, 4096, 1 << 30, None) == -1
+        assert L.aspen_b200_cache_copy(c, at, 64, 1, None) == L.aspen_b200_cache_copy(c, 64, at, 1, None) == -1
+        assert L.aspen_b200_cache_free(c, at, 1, None) == -1
+        for name in ("slots", "starts"):
+            assert L.aspen_b200_cache_append(c, 0, C.byref(api.AppendArgs(k=4096, v=4096, entries=1, rows=1, **{name: at})), None) == -1 and name in api.last_error()
+        assert L.aspen_b200_attention_decode(c, 0, C.byref(api.DecodeArgs(entries=1, heads=2, scale=1.0, q=4096, out=4096, slots=at, workspace=4096, workspace_bytes=1 << 30)), None) == -1
+        for name in ("q_starts", "kv_starts", "status"):
+            args = dict(type=api.FP16, heads=4, kv_heads=2, head_dim=64, scale=1.0, sequences=1, q_rows=3, kv_rows=3, q_starts=64, kv_starts=64, q=4096, k=4096, v=4096, out=8192)
+            args[name] = at
+            assert L.aspen_b200_attention_prompt(C.byref(api.PromptArgs(**args)), None) == -1 and name in api.last_error()
