@@ -28,6 +28,7 @@ struct Args {
     unsigned sequences, q_rows, kv_rows, heads, group, head_dim;
     unsigned part;                      // of 2^16 that is one over the group, rounded up: r / group = r * part >> 16 for r and group up to 128
     unsigned block;                     // 128 / group
+    unsigned in_a_row;                  // blocks of a CTA of prompt_rows
     Divisor by_block;
     int masked;
     float scale;                        // with log2(e)
@@ -71,8 +72,7 @@ __device__ __forceinline__ int find_piece(const Args &a, unsigned index, Place &
     }
     return -1;
 }
-__device__ __forceinline__ bool find_block(const Args &a, unsigned index, unsigned size, Block &b) {
-    Place from;
+__device__ __forceinline__ bool find_block(const Args &a, unsigned index, Place &from, unsigned size, Block &b) {
     const int i = find_piece(a, index, from, [=](unsigned queries) { return (queries + size - 1) / size; }, b.q0, b.queries, b.k0, b.keys);
     b.first = i * (int)size;
     return i >= 0;
@@ -110,222 +110,228 @@ struct Rows {
     static constexpr int TURN = HELD || SIZE == 2 ? PIECES : 1;
 };
 
-// SPLIT: the CTAs of a cluster walk a block's tiles in turn, and join what they have.
-template <int TYPE, int DIM, bool SPLIT>
+// How a CTA has its work: a block of queries; with the CTAs of a cluster, which walk a block's tiles in turn and join what they have; several blocks one after the other.
+enum { ALONE, SHARED, IN_A_ROW };
+template <int TYPE, int DIM, int WORK>
 __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
     typedef Rows<TYPE, DIM> R;
     constexpr int SIZE = R::SIZE, VALUES = R::VALUES, KT = R::KEYS / 8;
+    constexpr bool SPLIT = WORK == SHARED;
     extern __shared__ __align__(128) char smem[];
     const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane >> 2, t = lane & 3, head = blockIdx.y, kv_head = head / a.group;
-    Block b;
     attn::wait_for_previous_kernel();
     const unsigned ranks = SPLIT ? cluster_size() : 1u, rank = SPLIT ? blockIdx.x % ranks : 0u;
-    if (!find_block(a, blockIdx.x / ranks, R::QUERIES, b)) return;
-    const int behind = b.keys - b.queries;                      // query i sees keys up to i + behind
-    const int last = min(b.queries, b.first + R::QUERIES) - 1;
-    const int end = a.masked ? min(b.keys, last + behind + 1) : b.keys;
-    const int row0 = b.first + (int)warp * 16 + (int)g, row8 = row0 + 8;
-    const char *const k = a.k + ((size_t)b.k0 * a.k_row + (size_t)kv_head * a.k_head) * SIZE, *const v = a.v + ((size_t)b.k0 * a.v_row + (size_t)kv_head * a.v_head) * SIZE;
-    auto fetch = [&](int tile, int stage) {
-        char *const at = smem + stage * R::STAGE;
-        constexpr int PER_ROW = R::BYTES / 16;
-        #pragma unroll 4
-        for (int i = threadIdx.x; i < R::KEYS * PER_ROW; i += R::THREADS) {
-            const int r = i / PER_ROW, x = i % PER_ROW, j = tile * R::KEYS + r;
-            const bool ok = j < end && x * VALUES < (int)a.head_dim;
-            copy16(shared_address(at + r * R::KPITCH + x * 16), k + (ok ? ((size_t)j * a.k_row + x * VALUES) * SIZE : 0), ok);
-            copy16(shared_address(at + R::KEYS * R::KPITCH + r * R::VPITCH + x * 16), v + (ok ? ((size_t)j * a.v_row + x * VALUES) * SIZE : 0), ok);
-        }
-        copies_done();
-    };
-    const int tiles = end > 0 ? (end + R::KEYS - 1) / R::KEYS : 0;
-    if ((int)rank < tiles) fetch((int)rank, 0);
-    // queries, rows g and g + 8 of the warp's 16
-    const char *const q = a.q + ((size_t)b.q0 * a.q_row + (size_t)head * a.q_head) * SIZE;
-    char *const own = smem + 2 * R::STAGE + warp * 16 * R::KPITCH;
-    uint4 held[R::HELD ? R::PIECES * 2 : 1];
-    #pragma unroll
-    for (int i = 0; i < R::PIECES; i++)
-        #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int row = h ? row8 : row0;
-            const unsigned f = i * 4 * VALUES + t * VALUES;
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (row < b.queries && f < a.head_dim) x = __ldg(reinterpret_cast<const uint4 *>(q + ((size_t)row * a.q_row + f) * SIZE));
-            if (R::HELD) held[2 * i + h] = x;
-            else *reinterpret_cast<uint4 *>(own + (g + 8 * h) * R::KPITCH + f * SIZE) = x;
-        }
-    __syncwarp();
-    float o[DIM / 8][4], max[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-    #pragma unroll
-    for (int i = 0; i < DIM / 8; i++)
-        #pragma unroll
-        for (int j = 0; j < 4; j++) o[i][j] = 0.f;
-    for (int tile = (int)rank, stage = 0; tile < tiles; tile += (int)ranks, stage ^= 1) {
-        if (tile + (int)ranks < tiles) { fetch(tile + (int)ranks, stage ^ 1); wait_copies<1>(); } else wait_copies<0>();
-        __syncthreads();
-        const char *const ks = smem + stage * R::STAGE, *const vs = ks + R::KEYS * R::KPITCH;
-        float s[KT][4];
-        #pragma unroll
-        for (int n = 0; n < KT; n++)
-            #pragma unroll
-            for (int j = 0; j < 4; j++) s[n][j] = 0.f;
-        #pragma unroll R::TURN
-        for (int i = 0; i < R::PIECES; i++) {
-            const int f = (i * 4 * VALUES + t * VALUES) * SIZE;
-            const uint4 x = R::HELD ? held[R::HELD ? 2 * i : 0] : *reinterpret_cast<const uint4 *>(own + g * R::KPITCH + f);
-            const uint4 y = R::HELD ? held[R::HELD ? 2 * i + 1 : 0] : *reinterpret_cast<const uint4 *>(own + (g + 8) * R::KPITCH + f);
-            #pragma unroll
-            for (int n = 0; n < KT; n++) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(ks + (n * 8 + g) * R::KPITCH + f);
-                if constexpr (TYPE == ASPEN_B200_FP32) {
-                    // sums of 16 features are added outside: the tensor cores cut off what they add to a sum
-                    const unsigned a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w}, b0[2] = {w.x, w.y}, b1[2] = {w.z, w.w};
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma::tf32x3(part, a0, b0);
-                    mma::tf32x3(part, a1, b1);
-                    #pragma unroll
-                    for (int j = 0; j < 4; j++) s[n][j] += part[j];
-                } else {
-                    mma::Of<TYPE>::step(s[n], x.x, y.x, x.y, y.y, w.x, w.y);
-                    mma::Of<TYPE>::step(s[n], x.z, y.z, x.w, y.w, w.z, w.w);
-                }
+    Place from;
+    #pragma unroll 1
+    for (unsigned n = 0; n < (WORK == IN_A_ROW ? a.in_a_row : 1u); n++) {
+        Block b;
+        if (!find_block(a, WORK == IN_A_ROW ? blockIdx.x * a.in_a_row + n : blockIdx.x / ranks, from, R::QUERIES, b)) return;
+        const int behind = b.keys - b.queries;                      // query i sees keys up to i + behind
+        const int last = min(b.queries, b.first + R::QUERIES) - 1;
+        const int end = a.masked ? min(b.keys, last + behind + 1) : b.keys;
+        const int row0 = b.first + (int)warp * 16 + (int)g, row8 = row0 + 8;
+        const char *const k = a.k + ((size_t)b.k0 * a.k_row + (size_t)kv_head * a.k_head) * SIZE, *const v = a.v + ((size_t)b.k0 * a.v_row + (size_t)kv_head * a.v_head) * SIZE;
+        auto fetch = [&](int tile, int stage) {
+            char *const at = smem + stage * R::STAGE;
+            constexpr int PER_ROW = R::BYTES / 16;
+            #pragma unroll 4
+            for (int i = threadIdx.x; i < R::KEYS * PER_ROW; i += R::THREADS) {
+                const int r = i / PER_ROW, x = i % PER_ROW, j = tile * R::KEYS + r;
+                const bool ok = j < end && x * VALUES < (int)a.head_dim;
+                copy16(shared_address(at + r * R::KPITCH + x * 16), k + (ok ? ((size_t)j * a.k_row + x * VALUES) * SIZE : 0), ok);
+                copy16(shared_address(at + R::KEYS * R::KPITCH + r * R::VPITCH + x * 16), v + (ok ? ((size_t)j * a.v_row + x * VALUES) * SIZE : 0), ok);
             }
-        }
-        // columns 2 t and 2 t + 1 of each eight keys; rows g and g + 8
-        const int j0 = tile * R::KEYS + 2 * (int)t;
-        const int see0 = a.masked ? min(end, row0 + behind + 1) : end, see8 = a.masked ? min(end, row8 + behind + 1) : end;      // first key that is not seen
-        float m[2] = {max[0], max[1]};
+            copies_done();
+        };
+        const int tiles = end > 0 ? (end + R::KEYS - 1) / R::KEYS : 0;
+        if ((int)rank < tiles) fetch((int)rank, 0);
+        // queries, rows g and g + 8 of the warp's 16
+        const char *const q = a.q + ((size_t)b.q0 * a.q_row + (size_t)head * a.q_head) * SIZE;
+        char *const own = smem + 2 * R::STAGE + warp * 16 * R::KPITCH;
+        uint4 held[R::HELD ? R::PIECES * 2 : 1];
         #pragma unroll
-        for (int n = 0; n < KT; n++)
+        for (int i = 0; i < R::PIECES; i++)
             #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                s[n][j] = j0 + n * 8 + (j & 1) < (j < 2 ? see0 : see8) ? s[n][j] * a.scale : -INFINITY;
-                m[j / 2] = fmaxf(m[j / 2], s[n][j]);
+            for (int h = 0; h < 2; h++) {
+                const int row = h ? row8 : row0;
+                const unsigned f = i * 4 * VALUES + t * VALUES;
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                if (row < b.queries && f < a.head_dim) x = __ldg(reinterpret_cast<const uint4 *>(q + ((size_t)row * a.q_row + f) * SIZE));
+                if (R::HELD) held[2 * i + h] = x;
+                else *reinterpret_cast<uint4 *>(own + (g + 8 * h) * R::KPITCH + f * SIZE) = x;
             }
-        float down[2], ref[2];
-        #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
-            m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
-            ref[h] = m[h] == -INFINITY ? 0.f : m[h];
-            down[h] = mma::exp2_fast(max[h] - ref[h]);
-            ref[h] -= mma::Of<TYPE>::TOP;
-            max[h] = m[h];
-            sum[h] *= down[h];
-        }
-        #pragma unroll
-        for (int n = 0; n < KT; n++)
-            #pragma unroll
-            for (int j = 0; j < 4; j++) { s[n][j] = mma::exp2_fast(s[n][j] - ref[j / 2]); sum[j / 2] += s[n][j]; }
-        if (__any_sync(0xffffffffu, down[0] != 1.f || down[1] != 1.f)) {
-            #pragma unroll
-            for (int i = 0; i < DIM / 8; i++)
-                #pragma unroll
-                for (int j = 0; j < 4; j++) o[i][j] *= down[j / 2];
-        }
-        if constexpr (TYPE == ASPEN_B200_FP32) {
-            #pragma unroll
-            for (int i = 0; i < R::VPIECES; i++) {
-                float part[4][4];
-                #pragma unroll
-                for (int j = 0; j < 16; j++) part[j / 4][j % 4] = 0.f;
-                #pragma unroll
-                for (int n = 0; n < KT; n++) {
-                    const unsigned p[4] = {__float_as_uint(s[n][0]), __float_as_uint(s[n][2]), __float_as_uint(s[n][1]), __float_as_uint(s[n][3])};
-                    const char *const row = vs + (n * 8 + 2 * t) * R::VPITCH + (i * 32 + g * 4) * SIZE;
-                    const uint4 x = *reinterpret_cast<const uint4 *>(row), y = *reinterpret_cast<const uint4 *>(row + R::VPITCH);
-                    const unsigned w0[4] = {x.x, x.y, x.z, x.w}, w1[4] = {y.x, y.y, y.z, y.w};
-                    #pragma unroll
-                    for (int j = 0; j < 4; j++) { const unsigned w[2] = {w0[j], w1[j]}; mma::tf32x3(part[j], p, w); }
-                }
-                #pragma unroll
-                for (int j = 0; j < 16; j++) o[i * 4 + j / 4][j % 4] += part[j / 4][j % 4];
-            }
-        } else {
-            typedef mma::Of<TYPE> T;
-            #pragma unroll
-            for (int n = 0; n < KT; n += 2) {
-                const unsigned p0 = T::pack(s[n][0], s[n][1]), p1 = T::pack(s[n][2], s[n][3]), p2 = T::pack(s[n + 1][0], s[n + 1][1]), p3 = T::pack(s[n + 1][2], s[n + 1][3]);
-                const char *const row = vs + (n * 8 + 2 * t) * R::VPITCH;
-                #pragma unroll
-                for (int i = 0; i < R::VPIECES; i++) {
-                    const char *const at = row + (i * 64 + g * 8) * SIZE;
-                    const uint4 x0 = *reinterpret_cast<const uint4 *>(at), x1 = *reinterpret_cast<const uint4 *>(at + R::VPITCH);
-                    const uint4 x8 = *reinterpret_cast<const uint4 *>(at + 8 * R::VPITCH), x9 = *reinterpret_cast<const uint4 *>(at + 9 * R::VPITCH);
-                    const unsigned w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w}, w8[4] = {x8.x, x8.y, x8.z, x8.w}, w9[4] = {x9.x, x9.y, x9.z, x9.w};
-                    #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        T::step(o[i * 8 + j], p0, p1, p2, p3, mma::pair_of(w0[j / 2], w1[j / 2], j & 1), mma::pair_of(w8[j / 2], w9[j / 2], j & 1));
-                }
-            }
-        }
-        __syncthreads();
-    }
-    #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-    }
-    // column n = 2 t + c of tile j holds the value j of piece n
-    constexpr int PER = TYPE == ASPEN_B200_FP32 ? 4 : 8;
-    auto store = [&](int h, int c, int i, const float *x) {
-        const int row = h ? row8 : row0;
-        const unsigned f = i * 8 * PER + (2 * t + c) * PER;
-        if (row >= b.queries || f >= a.head_dim) return;
-        char *const out = a.out + ((size_t)(b.q0 + row) * a.out_row + (size_t)head * a.out_head + f) * SIZE;
-        if constexpr (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float4 *>(out) = make_float4(x[0], x[1], x[2], x[3]);
-        else {
-            typedef mma::Of<TYPE> T;
-            *reinterpret_cast<uint4 *>(out) = make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
-        }
-    };
-    if constexpr (!SPLIT) {
-        #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const float inv = sum[h] == 0.f ? 0.f : 1.f / sum[h];
-            #pragma unroll
-            for (int i = 0; i < R::VPIECES; i++)
-                #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    float x[PER];
-                    #pragma unroll
-                    for (int j = 0; j < PER; j++) x[j] = o[i * PER + j][2 * h + c] * inv;
-                    store(h, c, i, x);
-                }
-        }
-    } else {
-        // [value of a thread][thread]; a thread joins every `ranks`-th piece of its own place
-        float *const mine = reinterpret_cast<float *>(smem) + threadIdx.x;
-        constexpr int STATS = DIM / 8 * 4;
-        static_assert((STATS + 4) * R::THREADS * 4 <= 2 * R::STAGE, "in place of keys and values");
+        __syncwarp();
+        float o[DIM / 8][4], max[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
         #pragma unroll
         for (int i = 0; i < DIM / 8; i++)
             #pragma unroll
-            for (int j = 0; j < 4; j++) mine[(i * 4 + j) * R::THREADS] = o[i][j];
-        #pragma unroll
-        for (int h = 0; h < 2; h++) { mine[(STATS + h) * R::THREADS] = max[h]; mine[(STATS + 2 + h) * R::THREADS] = sum[h]; }
-        cluster_barrier();
-        const unsigned at = shared_address(mine);
-        for (unsigned q = rank; q < 4 * R::VPIECES; q += ranks) {
-            const int h = (int)(q & 1u), c = (int)(q >> 1 & 1u), i = (int)(q >> 2);
-            float most = -INFINITY, all = 0.f, x[PER];
+            for (int j = 0; j < 4; j++) o[i][j] = 0.f;
+        for (int tile = (int)rank, stage = 0; tile < tiles; tile += (int)ranks, stage ^= 1) {
+            if (tile + (int)ranks < tiles) { fetch(tile + (int)ranks, stage ^ 1); wait_copies<1>(); } else wait_copies<0>();
+            __syncthreads();
+            const char *const ks = smem + stage * R::STAGE, *const vs = ks + R::KEYS * R::KPITCH;
+            float s[KT][4];
             #pragma unroll
-            for (int j = 0; j < PER; j++) x[j] = 0.f;
-            for (unsigned r = 0; r < ranks; r++) most = fmaxf(most, load_of_rank(at + (STATS + h) * R::THREADS * 4, r));
-            const float ref = most == -INFINITY ? 0.f : most;
-            for (unsigned r = 0; r < ranks; r++) {
-                const float w = mma::exp2_fast(load_of_rank(at + (STATS + h) * R::THREADS * 4, r) - ref);
-                all = fmaf(w, load_of_rank(at + (STATS + 2 + h) * R::THREADS * 4, r), all);
+            for (int n = 0; n < KT; n++)
                 #pragma unroll
-                for (int j = 0; j < PER; j++) x[j] = fmaf(w, load_of_rank(at + ((i * PER + j) * 4 + 2 * h + c) * R::THREADS * 4, r), x[j]);
+                for (int j = 0; j < 4; j++) s[n][j] = 0.f;
+            #pragma unroll R::TURN
+            for (int i = 0; i < R::PIECES; i++) {
+                const int f = (i * 4 * VALUES + t * VALUES) * SIZE;
+                const uint4 x = R::HELD ? held[R::HELD ? 2 * i : 0] : *reinterpret_cast<const uint4 *>(own + g * R::KPITCH + f);
+                const uint4 y = R::HELD ? held[R::HELD ? 2 * i + 1 : 0] : *reinterpret_cast<const uint4 *>(own + (g + 8) * R::KPITCH + f);
+                #pragma unroll
+                for (int n = 0; n < KT; n++) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(ks + (n * 8 + g) * R::KPITCH + f);
+                    if constexpr (TYPE == ASPEN_B200_FP32) {
+                        // sums of 16 features are added outside: the tensor cores cut off what they add to a sum
+                        const unsigned a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w}, b0[2] = {w.x, w.y}, b1[2] = {w.z, w.w};
+                        float part[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma::tf32x3(part, a0, b0);
+                        mma::tf32x3(part, a1, b1);
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) s[n][j] += part[j];
+                    } else {
+                        mma::Of<TYPE>::step(s[n], x.x, y.x, x.y, y.y, w.x, w.y);
+                        mma::Of<TYPE>::step(s[n], x.z, y.z, x.w, y.w, w.z, w.w);
+                    }
+                }
             }
-            const float inv = all == 0.f ? 0.f : 1.f / all;
+            // columns 2 t and 2 t + 1 of each eight keys; rows g and g + 8
+            const int j0 = tile * R::KEYS + 2 * (int)t;
+            const int see0 = a.masked ? min(end, row0 + behind + 1) : end, see8 = a.masked ? min(end, row8 + behind + 1) : end;      // first key that is not seen
+            float m[2] = {max[0], max[1]};
             #pragma unroll
-            for (int j = 0; j < PER; j++) x[j] *= inv;
-            store(h, c, i, x);
+            for (int n = 0; n < KT; n++)
+                #pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    s[n][j] = j0 + n * 8 + (j & 1) < (j < 2 ? see0 : see8) ? s[n][j] * a.scale : -INFINITY;
+                    m[j / 2] = fmaxf(m[j / 2], s[n][j]);
+                }
+            float down[2], ref[2];
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
+                m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
+                ref[h] = m[h] == -INFINITY ? 0.f : m[h];
+                down[h] = mma::exp2_fast(max[h] - ref[h]);
+                ref[h] -= mma::Of<TYPE>::TOP;
+                max[h] = m[h];
+                sum[h] *= down[h];
+            }
+            #pragma unroll
+            for (int n = 0; n < KT; n++)
+                #pragma unroll
+                for (int j = 0; j < 4; j++) { s[n][j] = mma::exp2_fast(s[n][j] - ref[j / 2]); sum[j / 2] += s[n][j]; }
+            if (__any_sync(0xffffffffu, down[0] != 1.f || down[1] != 1.f)) {
+                #pragma unroll
+                for (int i = 0; i < DIM / 8; i++)
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++) o[i][j] *= down[j / 2];
+            }
+            if constexpr (TYPE == ASPEN_B200_FP32) {
+                #pragma unroll
+                for (int i = 0; i < R::VPIECES; i++) {
+                    float part[4][4];
+                    #pragma unroll
+                    for (int j = 0; j < 16; j++) part[j / 4][j % 4] = 0.f;
+                    #pragma unroll
+                    for (int n = 0; n < KT; n++) {
+                        const unsigned p[4] = {__float_as_uint(s[n][0]), __float_as_uint(s[n][2]), __float_as_uint(s[n][1]), __float_as_uint(s[n][3])};
+                        const char *const row = vs + (n * 8 + 2 * t) * R::VPITCH + (i * 32 + g * 4) * SIZE;
+                        const uint4 x = *reinterpret_cast<const uint4 *>(row), y = *reinterpret_cast<const uint4 *>(row + R::VPITCH);
+                        const unsigned w0[4] = {x.x, x.y, x.z, x.w}, w1[4] = {y.x, y.y, y.z, y.w};
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) { const unsigned w[2] = {w0[j], w1[j]}; mma::tf32x3(part[j], p, w); }
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < 16; j++) o[i * 4 + j / 4][j % 4] += part[j / 4][j % 4];
+                }
+            } else {
+                typedef mma::Of<TYPE> T;
+                #pragma unroll
+                for (int n = 0; n < KT; n += 2) {
+                    const unsigned p0 = T::pack(s[n][0], s[n][1]), p1 = T::pack(s[n][2], s[n][3]), p2 = T::pack(s[n + 1][0], s[n + 1][1]), p3 = T::pack(s[n + 1][2], s[n + 1][3]);
+                    const char *const row = vs + (n * 8 + 2 * t) * R::VPITCH;
+                    #pragma unroll
+                    for (int i = 0; i < R::VPIECES; i++) {
+                        const char *const at = row + (i * 64 + g * 8) * SIZE;
+                        const uint4 x0 = *reinterpret_cast<const uint4 *>(at), x1 = *reinterpret_cast<const uint4 *>(at + R::VPITCH);
+                        const uint4 x8 = *reinterpret_cast<const uint4 *>(at + 8 * R::VPITCH), x9 = *reinterpret_cast<const uint4 *>(at + 9 * R::VPITCH);
+                        const unsigned w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w}, w8[4] = {x8.x, x8.y, x8.z, x8.w}, w9[4] = {x9.x, x9.y, x9.z, x9.w};
+                        #pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            T::step(o[i * 8 + j], p0, p1, p2, p3, mma::pair_of(w0[j / 2], w1[j / 2], j & 1), mma::pair_of(w8[j / 2], w9[j / 2], j & 1));
+                    }
+                }
+            }
+            __syncthreads();
         }
-        cluster_barrier();                          // the others have read what is here
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+            sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+        }
+        // column n = 2 t + c of tile j holds the value j of piece n
+        constexpr int PER = TYPE == ASPEN_B200_FP32 ? 4 : 8;
+        auto store = [&](int h, int c, int i, const float *x) {
+            const int row = h ? row8 : row0;
+            const unsigned f = i * 8 * PER + (2 * t + c) * PER;
+            if (row >= b.queries || f >= a.head_dim) return;
+            char *const out = a.out + ((size_t)(b.q0 + row) * a.out_row + (size_t)head * a.out_head + f) * SIZE;
+            if constexpr (TYPE == ASPEN_B200_FP32) *reinterpret_cast<float4 *>(out) = make_float4(x[0], x[1], x[2], x[3]);
+            else {
+                typedef mma::Of<TYPE> T;
+                *reinterpret_cast<uint4 *>(out) = make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
+            }
+        };
+        if constexpr (!SPLIT) {
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float inv = sum[h] == 0.f ? 0.f : 1.f / sum[h];
+                #pragma unroll
+                for (int i = 0; i < R::VPIECES; i++)
+                    #pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float x[PER];
+                        #pragma unroll
+                        for (int j = 0; j < PER; j++) x[j] = o[i * PER + j][2 * h + c] * inv;
+                        store(h, c, i, x);
+                    }
+            }
+        } else {
+            // [value of a thread][thread]; a thread joins every `ranks`-th piece of its own place
+            float *const mine = reinterpret_cast<float *>(smem) + threadIdx.x;
+            constexpr int STATS = DIM / 8 * 4;
+            static_assert((STATS + 4) * R::THREADS * 4 <= 2 * R::STAGE, "in place of keys and values");
+            #pragma unroll
+            for (int i = 0; i < DIM / 8; i++)
+                #pragma unroll
+                for (int j = 0; j < 4; j++) mine[(i * 4 + j) * R::THREADS] = o[i][j];
+            #pragma unroll
+            for (int h = 0; h < 2; h++) { mine[(STATS + h) * R::THREADS] = max[h]; mine[(STATS + 2 + h) * R::THREADS] = sum[h]; }
+            cluster_barrier();
+            const unsigned at = shared_address(mine);
+            for (unsigned q = rank; q < 4 * R::VPIECES; q += ranks) {
+                const int h = (int)(q & 1u), c = (int)(q >> 1 & 1u), i = (int)(q >> 2);
+                float most = -INFINITY, all = 0.f, x[PER];
+                #pragma unroll
+                for (int j = 0; j < PER; j++) x[j] = 0.f;
+                for (unsigned r = 0; r < ranks; r++) most = fmaxf(most, load_of_rank(at + (STATS + h) * R::THREADS * 4, r));
+                const float ref = most == -INFINITY ? 0.f : most;
+                for (unsigned r = 0; r < ranks; r++) {
+                    const float w = mma::exp2_fast(load_of_rank(at + (STATS + h) * R::THREADS * 4, r) - ref);
+                    all = fmaf(w, load_of_rank(at + (STATS + 2 + h) * R::THREADS * 4, r), all);
+                    #pragma unroll
+                    for (int j = 0; j < PER; j++) x[j] = fmaf(w, load_of_rank(at + ((i * PER + j) * 4 + 2 * h + c) * R::THREADS * 4, r), x[j]);
+                }
+                const float inv = all == 0.f ? 0.f : 1.f / all;
+                #pragma unroll
+                for (int j = 0; j < PER; j++) x[j] *= inv;
+                store(h, c, i, x);
+            }
+            cluster_barrier();                          // the others have read what is here
+        }
     }
 }
 
@@ -340,14 +346,21 @@ unsigned ranks_of(const Args &a, int type, unsigned sms) {
     while (ranks < 8 && blocks * ranks * 2 <= room && keys >= ranks * 256) ranks *= 2;
     return ranks;
 }
+// Blocks in a row of a CTA.  It looks for its first one from the first sequence on, 32 a turn, and goes on from there; with a CTA to a block the search is quadratic in the number of sequences
+// (20000 of 5 tokens, 12 fp32 heads of 128, 7.3 ms instead of 103; 4000 of one token, 12 bf16 heads of 64, 0.42 instead of 1.9; 300 of 10 45 us instead of 50).  Eight CTAs to an SM: 16 7.7 ms, 4 7.2
+// but 4000 of 30 tokens 2.0 instead of 1.6.
+unsigned in_a_row_of(const Args &a, unsigned sms) {
+    const unsigned long long ctas = (unsigned long long)blocks_of(a) * a.heads;
+    return a.sequences > 128 && ctas > 8 * sms ? (unsigned)(ctas / (8 * sms)) : 1u;
+}
 template <int TYPE, int DIM>
 cudaError_t launch_rows(const Args &a, unsigned ranks, cudaStream_t stream) {
     typedef Rows<TYPE, DIM> R;
     static_assert(R::QUERIES == 64 && R::SMEM <= (DIM <= 128 ? 112 : 226) * 1024, "as blocks_of and ranks_of have it");
-    void (*const kernel)(Args) = ranks > 1 ? prompt_rows<TYPE, DIM, true> : prompt_rows<TYPE, DIM, false>;
+    void (*const kernel)(Args) = ranks > 1 ? prompt_rows<TYPE, DIM, SHARED> : a.in_a_row > 1 ? prompt_rows<TYPE, DIM, IN_A_ROW> : prompt_rows<TYPE, DIM, ALONE>;
     cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM);
     if (err != cudaSuccess) return err;
-    return attn::launch_early_in_clusters(ranks, kernel, dim3(blocks_of(a) * ranks, a.heads), R::THREADS, R::SMEM, stream, a);
+    return attn::launch_early_in_clusters(ranks, kernel, dim3((blocks_of(a) + a.in_a_row - 1) / a.in_a_row * ranks, a.heads), R::THREADS, R::SMEM, stream, a);
 }
 template <int TYPE>
 cudaError_t launch_rows(const Args &a, unsigned ranks, cudaStream_t stream) {
@@ -1337,6 +1350,7 @@ extern "C" int aspen_b200_attention_prompt(const aspen_b200_prompt_t *p, void *c
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t err = cudaSuccess;
     const unsigned ranks = ranks_of(a, p->type, (unsigned)sms);
+    a.in_a_row = ranks > 1 ? 1u : in_a_row_of(a, (unsigned)sms);
     if (!try_tiles(a, p->type, ranks, stream, &err))
         err = p->type == ASPEN_B200_FP32 ? launch_rows<ASPEN_B200_FP32>(a, ranks, stream) : p->type == ASPEN_B200_BF16 ? launch_rows<ASPEN_B200_BF16>(a, ranks, stream) : launch_rows<ASPEN_B200_FP16>(a, ranks, stream);
     if (err != cudaSuccess) { cudaGetLastError(); ASPEN_ERR("%s: %s\n", what, cudaGetErrorString(err)); return -3; }

@@ -1428,3 +1428,23 @@ def test_words_off_a_4_byte_boundary_are_refused():
             args = dict(type=api.FP16, heads=4, kv_heads=2, head_dim=64, scale=1.0, sequences=1, q_rows=3, kv_rows=3, q_starts=64, kv_starts=64, q=4096, k=4096, v=4096, out=8192)
             args[name] = at
             assert L.aspen_b200_attention_prompt(C.byref(api.PromptArgs(**args)), None) == -1 and name in api.last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES, ids=ids)
+@pytest.mark.parametrize("heads,kv_heads,dim,scale", [(12, 6, 64, 0.2), (4, 4, 128, -0.1), (6, 2, 256, 0.1), (3, 3, 40, 0.2)])
+def test_hundreds_of_short_prompts(heads, kv_heads, dim, scale, kind):
+    """A CTA takes several blocks of queries, of one sequence and of the next ones.  Among 700 sequences of up to five tokens are empty ones, one of 200, and a first one that would end
+    before it starts."""
+    rng = np.random.default_rng(heads)
+    lengths = rng.integers(0, 6, 700)
+    lengths[350] = 200
+    starts = np.concatenate([[0], np.cumsum(lengths)]) + 2
+    q, k, v = (rounded(rng.standard_normal((starts[-1] + 3, h, dim)), kind) for h in (heads, kv_heads, kv_heads))
+    starts[0] = 9
+    got = prompt(*(to_device(a, kind) for a in (q, k, v)), starts, starts, kind, True, scale)
+    for s in range(1, 700):
+        a, b = starts[s], starts[s + 1]
+        want, away, size = attend(q[a:b], k[a:b], v[a:b], scale, seen_by(b - a, b - a, True))
+        check(got[a:b], want, away, size, kind)
+    assert got[:starts[1]].isnan().all() and got[starts[-1]:].isnan().all()
