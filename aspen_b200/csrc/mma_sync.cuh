@@ -7,7 +7,7 @@
 //     keys       lane (g, t) holds rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of 16 keys, values 8 g ... of 64 (fp32: 4 g ... of 32); two rows are interleaved by byte permutes
 //
 // fp32: TF32 operands of 11 bits.  x = hi + lo, hi is x rounded to 11 bits and lo the rest, of which TF32 keeps 11 again (2^-22 of x is lost); hi hi + hi lo + lo hi leave
-// out lo lo, 2^-22 of a product: 2^-20 in all at most.  Sums are fp32.
+// out lo lo, 2^-22 of a product: 2^-20 in all at most.  Below 2^-104 lo loses bits that TF32 has no exponent for (2^-126 at most), and what hi rounds past the range becomes an infinity.  Sums are fp32.
 #pragma once
 #include "attention.h"
 

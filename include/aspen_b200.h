@@ -290,8 +290,9 @@ int aspen_b200_matmul_noalloc(const float *x_dev, const float *w_dev, const floa
  * a CUDA launch itself fails.
  *
  * Types: queries, keys, values, outputs and the cache of one call have the same.  Scores, softmax and sums are fp32, rounded once to the output's type; the
- * weights are rounded to bf16 / fp16 before they multiply 16-bit values.  fp32 operands are split into parts that tensor cores hold (a product is
- * off by 2^-20 of itself at most); an infinity among them makes the outputs that see it NaN.
+ * weights are rounded to bf16 / fp16 before they multiply 16-bit values.  fp32 operands are split into parts that tensor cores hold: an operand is off by 2^-22 of itself or by 2^-126, whichever is
+ * more, and a product by 2^-20 of itself besides.  An infinity among them makes the outputs that see it NaN, and so may a finite operand of 2^128 - 2^119 or more in size.  The values of a row are
+ * added up with weights of up to 1 (16 bits: 2^15) before the sum is divided by the weights', so that sum has to stay in fp32's range.
  * Heads have 8 ... 256 features, a multiple of 8; `heads` is a multiple of `kv_heads`, head h reads key head h / (heads / kv_heads).
  * Strides are in elements, 0 = packed; features are contiguous, and every row starts on a 16-byte boundary. */
 typedef enum { ASPEN_B200_FP32, ASPEN_B200_BF16, ASPEN_B200_FP16, ASPEN_B200_NUM_TYPES } ASPEN_B200_TYPE;

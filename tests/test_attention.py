@@ -1448,3 +1448,28 @@ def test_hundreds_of_short_prompts(heads, kv_heads, dim, scale, kind):
         want, away, size = attend(q[a:b], k[a:b], v[a:b], scale, seen_by(b - a, b - a, True))
         check(got[a:b], want, away, size, kind)
     assert got[:starts[1]].isnan().all() and got[starts[-1]:].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dim,n", [(12, 64, 512), (2, 64, 40), (12, 128, 200)])
+def test_fp32_values_of_any_size(heads, dim, n):
+    """An operand is off by 2^-22 of itself, which the usual tolerance has, or by 2^-126; so is a mean of values, and it may lose 2^-126 when it is written.  2^128 - 2^120 is a value, too."""
+    rng = np.random.default_rng(50)
+    q, k, base = (rounded(rng.standard_normal((n, heads, dim)), api.FP32) for _ in range(3))
+    q[0] = 0
+    for power in (-126, -116, -108, -100, 100, 127):
+        v = rounded(base * 2.0 ** min(power, 100), api.FP32)
+        if power == 127:
+            v[0, :, ::3] = 2.0 ** 128 - 2.0 ** 120
+        got = prompt(*(to_device(a, api.FP32) for a in (q, k, v)), [0, n], [0, n], api.FP32, True, 0.1).cpu().numpy().astype(np.float64)
+        want, away, _ = attend(q, k, v, 0.1, seen_by(n, n, True))
+        assert (np.abs(got - want) <= away + 2.0 ** -24 * np.abs(want) + 2.0 ** -125).all(), power
+        pool = Pool(api.FP32, heads, dim, 16, n // 16 + 1, 1, n // 16 + 1)
+        pool.fill([n], rng)
+        pool.host_v = rounded(np.nan_to_num(pool.host_v) * 2.0 ** min(power, 100), api.FP32)
+        if power == 127:
+            pool.host_v[0, pool.host_table[0, 0], :, 0, ::3] = 2.0 ** 128 - 2.0 ** 120
+        pool.v.copy_(to_device(pool.host_v, api.FP32))
+        got = decode(pool, to_device(q[1:2], api.FP32), heads, slots=[0]).cpu().numpy().astype(np.float64)
+        want, away, _ = decode_want(pool, q[1:2], [0], [n], dim ** -0.5)
+        assert (np.abs(got - want) <= away + 2.0 ** -24 * np.abs(want) + 2.0 ** -125).all(), power
