@@ -3,11 +3,13 @@
 // out = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q k_j - max): one pass over the keys, the maximum and the sum running along (values already summed are scaled by
 // exp(old max - new max)).  Parts of a sequence give (max, sum, weighted values) that join the same way.
 //
-// What bounds it: reading the cache once.  A step of 16 keys is multiplied with all query heads of its key head, so each key and value is read once whatever the group.
+// What bounds it: reading the cache once.  A step of 16 keys is multiplied with all query heads of its key head, so each key and value is read once for 16 heads of its
+// group (8 with 256 features, and in fp32 with 128: heads_of_pass); larger groups read it again.
 //     S^T [16 keys x 8 heads] = K Q^T, O^T [features x 8 heads] += V^T P^T, by mma.sync with the keys as the 16-row operand: 8 heads fill its columns where tcgen05 would want
 // 128 rows of queries, and a warp needs nobody else: keys and values go from memory to registers as 32-byte pieces (mma_sync.cuh), no shared memory, no barrier.  Pieces of the next
-// step are asked for before this one is multiplied.  7.3 TB/s while walking: 64 sequences of up to 8192 tokens, bf16, 8 heads of keys of 128, 173 us with all else; one of 100003 71 us; 32 of
-// up to 1024, fp16, 12 heads of 64, 17 us, of which 10 are the first loads and the joins; one of 1000, fp32, 9.3 us on the device.
+// step are asked for before this one is multiplied.  64 sequences of up to 8192 tokens, bf16, 8 heads of keys of 128: 170 us, 6.5 TB/s with start, end and join; one of 100003 70 us, 5.9 TB/s; 32 of
+// up to 1024, fp16, 12 heads of 64, 17 us, of which 10 are the first loads and the joins; one of 1000, fp32, 9.3 us on the device; 64 of up to 2000, fp32, 12 heads of 64, 77 us, 5.0 TB/s (the
+// splitting of operands takes its share).
 //
 // Cut: all (sequence, key head) items' steps stand in one line that is dealt to CTAs and then to their warps in equal shares, whatever the lengths (they are known on the
 // device only, and a captured call may see others each time).  A warp's whole items are finished in its registers; at most two it shares with its neighbours.  Shares are

@@ -9,7 +9,7 @@
 // keys and values of a tile go through shared memory for the four warps of a CTA, asked for one tile ahead.  Rows in shared memory are 64 (keys) and 16 bytes (values) longer than a
 // power of two, so that the 16-byte pieces that eight lanes read together lie in different banks.  It is bounded by the instructions around mma.sync (fp32: splitting) and, with one block to a
 // sequence, by its chain of loads, products and exp2: 12 heads of 64, one prompt of 37 tokens in fp32 9 us with the call, 32 prompts of 100 tokens in bf16 12 us (8 of 512 in fp32 92 us,
-// prompt_parts 33; 24 of up to 1024 in bf16 101 us, prompt_tiles 46.5); 8 of 512 with heads of 128 in fp32 197 us.
+// prompt_parts 33; 24 of up to 1024 in bf16 101 us, prompt_tiles 46.5); 8 of 512 with heads of 128 in fp32 194 us.
 // Where there are few blocks, the CTAs of a cluster walk the tiles of one in turn and join maxima, sums and values through each other's shared memory, in the order of their ranks: 8 heads of 128,
 // one query over 30000 keys in bf16 108 us instead of 392 (prompt_tiles), 4 queries of 12 heads of 64 over 2004 keys in fp32 19 instead of 75 (prompt_parts).
 #include "attention_tc.cuh"
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(128) prompt_rows(const Args a) {
 
 // CTAs to a block.  Few blocks leave SMs without work; up to 8 CTAs share a block's keys then, 128 or more each, as long as all of them run at once.  An SM has room for two, heads of 256
 // features for one.  Wide fp32 heads with a mask take two rounds of CTAs: their last blocks have twice the keys of the mean (one prompt of 549 tokens, 21 heads of 128, 84 us instead of 112; bf16
-// heads of 256, two of 400 tokens, take 37 instead of 24).
+// heads of 256, two of 400 tokens, take 37 instead of 24).  Keys by the mean of the sequences: a long one among many short ones is walked by one CTA a block, since lengths are on the device.
 unsigned blocks_of(const Args &a) { return a.q_rows / 64 + (a.sequences < a.q_rows ? a.sequences : a.q_rows); }
 unsigned ranks_of(const Args &a, int type, unsigned sms) {
     const unsigned long long blocks = (unsigned long long)blocks_of(a) * a.heads, rounds = type == ASPEN_B200_FP32 && a.head_dim > 64 && a.masked ? 2 : 1, room = a.head_dim <= 128 ? 2 * sms * rounds : sms;
